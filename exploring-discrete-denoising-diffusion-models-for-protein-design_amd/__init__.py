@@ -13,9 +13,12 @@ from . import tables  # noqa: F401
 from . import graphs  # noqa: F401
 from . import d3pm  # noqa: F401
 from . import protein_generation  # noqa: F401
+from . import finetune  # noqa: F401
 from .d3pm import DiscreteDiffusion, generate_betas  # noqa: F401
 from .protein_generation import (Tokenizer, D3PMLVBLoss, D3PMLVBLossMSA, generate_d3pm,  # noqa: F401
                                  sample_transition_matrix, cumprod_matrix)
+from .finetune import token_logprobs, TopKDistillLoss, PreferenceLoss, PolicyLoss  # noqa: F401
 
 __all__ = ["DiscreteDiffusion", "generate_betas", "Tokenizer", "D3PMLVBLoss", "D3PMLVBLossMSA", "generate_d3pm",
-           "sample_transition_matrix", "cumprod_matrix", "d3pm", "protein_generation", "tables"]
+           "sample_transition_matrix", "cumprod_matrix", "d3pm", "protein_generation", "tables", "finetune",
+           "token_logprobs", "TopKDistillLoss", "PreferenceLoss", "PolicyLoss"]

@@ -34,8 +34,13 @@ class TablesF64(C.Structure):
                 ("lvb_digest", C.c_void_p)]
 
 
+class Logits(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_int), ("V", C.c_int), ("B", C.c_long), ("L", C.c_long),
+                ("stride_b", C.c_long), ("stride_l", C.c_long)]
+
+
 _P, _I, _L, _F, _D, _U64, _SZ = C.c_void_p, C.c_int, C.c_long, C.c_float, C.c_double, C.c_uint64, C.c_size_t
-_T32, _T64 = C.POINTER(TablesF32), C.POINTER(TablesF64)
+_T32, _T64, _Z = C.POINTER(TablesF32), C.POINTER(TablesF64), C.POINTER(Logits)
 
 # name -> (restype, argtypes); must list every function of include/d3pm_hip.h
 SIGNATURES = {
@@ -72,6 +77,12 @@ SIGNATURES = {
     "d3pm_lvb_loss_workspace": (_SZ, [_I, _L, _I]),
     "d3pm_lvb_loss": (_I, [_T64, _P, _L, _P, _P, _P, _P, _I, _L, _I, _I, _D, _P, _P, _P, _SZ, _P]),
     "d3pm_lvb_hybrid_loss": (_I, [_T64, _P, _L, _P, _P, _P, _P, _I, _L, _I, _I, _D, _D, _P, _P, _P, _P, _SZ, _P]),
+    "d3pm_objective_workspace": (_SZ, [_L, _L]),
+    "d3pm_token_logprobs": (_I, [_Z, _P, _I, _P, _F, _P, _P, _P]),
+    "d3pm_token_grad": (_I, [_Z, _P, _I, _F, _P, _P, _I, _I, _P, _P]),
+    "d3pm_topk_distill_loss": (_I, [_Z, _P, _I, _P, _I, _I, _P, _F, _F, _P, _I, _P, _P, _P, _P, _SZ, _P]),
+    "d3pm_policy_loss": (_I, [_Z, _P, _I, _P, _P, _I, _P, _P, _F, _F, _F, _F, _F, _P, _I, _P, _P, _P, _P, _SZ, _P]),
+    "d3pm_preference_loss": (_I, [_Z, _P, _I, _P, _P, _F, _F, _I, _F, _P, _P, _P, _P, _P, _SZ, _P]),
     "d3pm_lvb_reverse_step": (_I, [_T64, _P, _L, _P, _P, _I, _L, _P, _U64, _U64, _P, _D, _L, _P, _P]),
 }
 

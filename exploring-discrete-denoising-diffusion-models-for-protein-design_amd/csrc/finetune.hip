@@ -1,0 +1,929 @@
+// Fine-tuning objectives at the logits of a denoiser or a language model: token log-probabilities, distillation from
+// a teacher's top logits, the preference loss of paired sequences and the clipped policy loss with its KL term, with
+// the gradient at the logits.
+//
+// Every one of them is a function of the rows' softmax, p = exp((z - m) / tau) / S with m the row's maximum and
+// S = sum_v exp((z_v - m) / tau), and its gradient at a row is
+//     dz_v = c (target_v - Q p_v)
+// with one coefficient c of the row, target the token's indicator (Q = 1) or the teacher's distribution over its kept
+// entries (Q = 1, or 0 where none is kept).  The distillation and the policy loss know c as soon as the row's m and S
+// are known, so one pass over a row held in registers gives loss and gradient (k_rows); the preference loss needs the
+// sums of two whole sequences first and the log-probabilities' backward an upstream gradient per row: those write m, S
+// and c per row and a second kernel makes the gradient from them (k_token_grad).
+//
+// All of it moves 2 x (bytes of a row) per row and computes about 20 vector operations per logit (two exponentials,
+// which take four issue slots each), so the memory system bounds it.
+#include "d3pm_device.h"
+
+#include <algorithm>
+#include <cfloat>
+#include <climits>
+#include <cmath>
+
+namespace d3pm {
+namespace ft {
+
+constexpr int MAX_K = 256;              // entries of a teacher's list
+constexpr int MAX_PARTIALS = 8192;      // workgroups of a loss launch: one partial sum each
+
+enum Head { HEAD_LOGPROB = 0, HEAD_PREFERENCE = 1, HEAD_POLICY = 2, HEAD_DISTILL = 3 };
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// ------------------------------------------------------------------------------------------------ element types
+// A 16-byte piece of a row as it lies in memory (rows of odd widths start anywhere: the vector accesses ask for the
+// element's alignment only, which the hardware's global accesses take), its E values as float, and back (one
+// rounding to nearest).
+typedef uint32_t raw_f32 __attribute__((ext_vector_type(4), aligned(4), may_alias));
+typedef uint32_t raw_16 __attribute__((ext_vector_type(4), aligned(2), may_alias));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct F32 {
+  static constexpr int E = 4, SIZE = 4;
+  static constexpr uint32_t NEG_INF = 0xFF800000u;       // as often as it fits a dword
+  typedef raw_f32 Raw;
+  typedef float __attribute__((may_alias)) Elem;
+  static __device__ __forceinline__ void unpack(u32x4 r, float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __builtin_bit_cast(float, (uint32_t)r[i]);
+  }
+  static __device__ __forceinline__ u32x4 pack(const float* f) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, f[i]);
+    return r;
+  }
+  static __device__ __forceinline__ float get(const void* p, long i) { return ((const Elem*)p)[i]; }
+  static __device__ __forceinline__ void put(void* p, long i, float v) { ((Elem*)p)[i] = v; }
+};
+
+struct F16 {
+  static constexpr int E = 8, SIZE = 2;
+  static constexpr uint32_t NEG_INF = 0xFC00FC00u;
+  typedef raw_16 Raw;
+  typedef _Float16 __attribute__((may_alias)) Elem;
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ void unpack(u32x4 r, float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const h2 h = __builtin_bit_cast(h2, (uint32_t)r[i]);
+      f[2 * i] = (float)h[0];
+      f[2 * i + 1] = (float)h[1];
+    }
+  }
+  static __device__ __forceinline__ u32x4 pack(const float* f) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, (h2){(_Float16)f[2 * i], (_Float16)f[2 * i + 1]});
+    return r;
+  }
+  static __device__ __forceinline__ float get(const void* p, long i) { return (float)((const Elem*)p)[i]; }
+  static __device__ __forceinline__ void put(void* p, long i, float v) { ((Elem*)p)[i] = (_Float16)v; }
+};
+
+struct BF16 {
+  static constexpr int E = 8, SIZE = 2;
+  static constexpr uint32_t NEG_INF = 0xFF80FF80u;
+  typedef raw_16 Raw;
+  typedef __bf16 __attribute__((may_alias)) Elem;
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ void unpack(u32x4 r, float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __builtin_bit_cast(float, (uint32_t)(r[i] << 16));
+      f[2 * i + 1] = __builtin_bit_cast(float, (uint32_t)(r[i] & 0xFFFF0000u));
+    }
+  }
+  static __device__ __forceinline__ u32x4 pack(const float* f) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){f[2 * i], f[2 * i + 1]}, b2));
+    return r;
+  }
+  static __device__ __forceinline__ float get(const void* p, long i) { return (float)((const Elem*)p)[i]; }
+  static __device__ __forceinline__ void put(void* p, long i, float v) { ((Elem*)p)[i] = (__bf16)v; }
+};
+
+__device__ __forceinline__ float get_any(const void* p, int dtype, long i) {
+  return dtype == D3PM_F32 ? F32::get(p, i) : dtype == D3PM_F16 ? F16::get(p, i) : BF16::get(p, i);
+}
+// an int32 or int64 index: -1 for any negative one, else at most INT_MAX
+__device__ __forceinline__ int get_int(const void* p, int bytes, long i) {
+  const long v = bytes == 4 ? (long)((const int*)p)[i] : ((const long*)p)[i];
+  return v < 0 ? -1 : v > INT_MAX ? INT_MAX : (int)v;
+}
+
+// ------------------------------------------------------------------------------------------------------ arguments
+struct RowArgs {
+  const void* z; long sb, sl; int L, V, N; int dense;         // dense: row n lies at n * sl
+  const void* tokens; int tok_bytes; const uint8_t* mask;
+  float c_hi, c_lo, inv_tau;                                  // log2(e) / tau in two floats; 1 / tau
+  int head;
+  const float* old_lp; const float* ref_lp; const float* adv; int adv_per_seq; float clip_lo, clip_hi, kl_coeff;
+  const void* t_logits; int t_dtype; const void* t_index; int t_index_bytes; int k;
+  float weight;                                               // of a counted row: out_scale (x tau or / tau) ...
+  const int* count; float inv_count;                          // ... over the count (NULL: inv_count, every row counts)
+  const float* upstream; int only_if_rescaled;                // gradient only: times *upstream; nothing to do at 1
+  float4* stats; float* per_row; double* partial; void* dz;
+};
+
+__device__ __forceinline__ const char* row_ptr(const RowArgs& a, int n, int size) {
+  long at;
+  if (a.dense) at = (long)n * a.sl;
+  else {
+    const unsigned b = (unsigned)n / (unsigned)a.L;
+    at = (long)b * a.sb + (long)((unsigned)n - b * (unsigned)a.L) * a.sl;
+  }
+  return (const char*)a.z + at * size;
+}
+
+// exp((z - m) / tau) of d = z - m <= 0, the constant in two floats: its rounding alone would shift every S the same
+// way (1e-7 at d = -10), which the sum over a sequence of a preference loss would gather up.
+__device__ __forceinline__ float exp_d(float d, float c_hi, float c_lo) { return exp2_hw(fmaf(d, c_hi, d * c_lo)); }
+
+// What a row's token gives once m and S are known: its log-probability, its share of the loss and the coefficient
+// c of its gradient (without the weight).  Comparisons are written so that a NaN stays one.
+struct TokenOut { float lp, loss, c; };
+__device__ __forceinline__ TokenOut token_head(const RowArgs& a, int n, float zy_m, float S) {
+  TokenOut o;
+  o.lp = zy_m * a.inv_tau - logf(S);
+  o.loss = 0.0f;
+  o.c = 1.0f;
+  if (a.head == HEAD_POLICY) {
+    const float A = a.adv[a.adv_per_seq ? (unsigned)n / (unsigned)a.L : (unsigned)n];
+    const float r = expf(o.lp - a.old_lp[n]);
+    const float held_r = r < a.clip_lo ? a.clip_lo : r > a.clip_hi ? a.clip_hi : r;
+    const float free_s = r * A, held_s = held_r * A;
+    const bool clipped = free_s > held_s;
+    o.loss = clipped ? -held_s : -free_s;
+    o.c = clipped ? 0.0f : -free_s;
+    if (a.ref_lp) {
+      const float x = a.ref_lp[n] - o.lp, e = expm1f(x);
+      o.loss = fmaf(a.kl_coeff, e - x, o.loss);
+      o.c = fmaf(-a.kl_coeff, e, o.c);
+    }
+  }
+  return o;
+}
+
+// ------------------------------------------------------------------------------------- one pass, rows in registers
+// A row is held by a group of G lanes, NV 16-byte pieces each (lane g: pieces g, g + G, ...), and one element of the
+// end of the row that fills no piece.  Up to 64 lanes a group is a part of a wave and a workgroup of 256 has 256 / G
+// rows; beyond, a group is a workgroup.
+template <int G>
+struct Shape {
+  static constexpr int WG = G <= 64 ? 256 : G;
+  static constexpr int ROWS = WG / G;
+  static constexpr int GL = G < 64 ? G : 64;        // lanes that a teacher's list is spread over
+};
+
+// m and S of the group's row from its lanes' values: a wave takes its exponentials against its own maximum, so a
+// row of several waves needs one exchange, not two.  The reference is kept off -inf (a wave that has only padding).
+template <typename T, int G, int NV>
+__device__ __forceinline__ void row_stats(const u32x4 (&v)[NV], float edge, const RowArgs& a, float2* red, int wave,
+                                          float& m, float& S) {
+  constexpr int GL = Shape<G>::GL;
+  float f[T::E];
+  float mx = edge;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    T::unpack(v[j], f);
+#pragma unroll
+    for (int e = 0; e < T::E; ++e) mx = fmaxf(mx, f[e]);
+  }
+  mx = fmaxf(group_max<GL>(mx), -FLT_MAX);
+  float s0 = exp_d(edge - mx, a.c_hi, a.c_lo), s1 = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    T::unpack(v[j], f);
+#pragma unroll
+    for (int e = 0; e < T::E; e += 2) {
+      s0 += exp_d(f[e] - mx, a.c_hi, a.c_lo);
+      s1 += exp_d(f[e + 1] - mx, a.c_hi, a.c_lo);
+    }
+  }
+  const float s = group_sum<GL>(s0 + s1);
+  if constexpr (G <= 64) {
+    m = mx;
+    S = s;
+  } else {
+    if ((threadIdx.x & 63) == 0) red[wave] = make_float2(mx, s);
+    __syncthreads();
+    m = -FLT_MAX;
+#pragma unroll
+    for (int w = 0; w < G / 64; ++w) m = fmaxf(m, red[w].x);
+    double sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < G / 64; ++w) sum += (double)(red[w].y * exp_d(red[w].x - m, a.c_hi, a.c_lo));
+    S = (float)sum;
+  }
+}
+
+// The teacher's list of a row.  Loaded before the row's statistics are known: the kept entries' classes and
+// exponentials go to LDS (class -1: not kept), their sums stay with the lanes.
+struct List { int* idx; float* e; float St, A; int kept; };
+template <int GL>
+__device__ __forceinline__ void list_load(const RowArgs& a, int n, int g, List& l) {
+  const long at = (long)n * a.k;
+  float mt = -INFINITY;
+  int kept = 0;
+  for (int i = g; i < a.k; i += GL) {
+    const float t = get_any(a.t_logits, a.t_dtype, at + i);
+    int c = get_int(a.t_index, a.t_index_bytes, at + i);
+    if (c < 0 || t == -INFINITY) c = -1;
+    else {
+      c = min(c, a.V - 1);
+      mt = fmaxf(mt, t);
+      kept = 1;
+    }
+    l.idx[i] = c;
+    l.e[i] = t;
+  }
+  mt = fmaxf(group_max<GL>(mt), -FLT_MAX);          // a NaN entry alone leaves -inf here: its exponential is NaN
+  l.kept = (int)group_max<GL>((float)kept);
+  float St = 0.0f, A = 0.0f;
+  for (int i = g; i < a.k; i += GL) {
+    const float d = l.e[i] - mt;
+    const float e = l.idx[i] < 0 ? 0.0f : exp_d(d, a.c_hi, a.c_lo);
+    St += e;
+    if (e != 0.0f) A = fmaf(e, d * a.inv_tau, A);
+    l.e[i] = e;
+  }
+  l.St = group_sum<GL>(St);
+  l.A = group_sum<GL>(A);
+}
+// tau^2 KL(teacher || student) of the row
+template <typename T, int GL>
+__device__ __forceinline__ float list_loss(const RowArgs& a, const char* row, int g, const List& l, float m, float S) {
+  float Bs = 0.0f;
+  for (int i = g; i < a.k; i += GL) {
+    const float e = l.e[i];
+    if (e != 0.0f) Bs = fmaf(e, (T::get(row, l.idx[i]) - m) * a.inv_tau, Bs);
+  }
+  Bs = group_sum<GL>(Bs);
+  const float tau = 1.0f / a.inv_tau;
+  return l.kept ? tau * tau * ((l.A - Bs) / l.St - logf(l.St) + logf(S)) : 0.0f;
+}
+// gradient elements of the kept classes, c (q - p), over the -c p that the row's pieces hold there; a class listed
+// twice gets the sum of its entries, in the list's order, from each of them
+template <typename T, int GL>
+__device__ __forceinline__ void list_grad(const RowArgs& a, const char* row, char* out, int g, const List& l, float m,
+                                          float inv_S, float c) {
+  const float inv_St = 1.0f / l.St;
+  for (int i = g; i < a.k; i += GL) {
+    const int cls = l.idx[i];
+    if (cls < 0) continue;
+    float q = 0.0f;
+    for (int j = 0; j < a.k; ++j) q += l.idx[j] == cls ? l.e[j] : 0.0f;
+    const float p = exp_d(T::get(row, cls) - m, a.c_hi, a.c_lo) * inv_S;
+    T::put(out, cls, c * (q * inv_St - p));
+  }
+}
+
+// the gradient row of a position that is not counted
+template <typename T, int G>
+__device__ __forceinline__ void zero_row(char* out, int g, int full, int rest) {
+  const u32x4 zero = {0, 0, 0, 0};
+  for (int j = g; j < full; j += G) *(typename T::Raw*)(out + (long)j * 16) = zero;
+  if (g < rest) T::put(out, (long)full * T::E + g, 0.0f);
+}
+
+template <typename T, int G, int NV, bool DISTILL>
+__global__ __launch_bounds__(Shape<G>::WG) void k_rows(RowArgs a) {
+  typedef Shape<G> Sh;
+  constexpr int E = T::E;
+  __shared__ float2 red[2][G > 64 ? G / 64 : 1];
+  __shared__ int kept_flag[2];
+  __shared__ double wg_sum[Sh::ROWS];
+  extern __shared__ char lists[];
+  if (a.only_if_rescaled && *a.upstream == 1.0f) return;
+
+  const int g = threadIdx.x % G, slot = threadIdx.x / G, wave = threadIdx.x >> 6;
+  const int full = a.V / E, rest = a.V - full * E;
+  float w = a.weight * (a.count ? 1.0f / (float)max(*a.count, 1) : a.inv_count);
+  if (a.upstream) w *= *a.upstream;
+  double acc = 0.0;
+  int phase = 0;
+
+  for (int n0 = blockIdx.x * Sh::ROWS; n0 < a.N; n0 += gridDim.x * Sh::ROWS) {
+    const int n = n0 + slot;
+    if (Sh::ROWS > 1 && n >= a.N) break;
+    char* out = a.dz ? (char*)a.dz + (long)n * a.V * T::SIZE : nullptr;
+    if (a.mask && !a.mask[n]) {                      // not counted: nothing of its row is read
+      if (out) zero_row<T, G>(out, g, full, rest);
+      if (g == 0) {
+        if (a.per_row) a.per_row[n] = 0.0f;
+        if (a.stats) a.stats[n] = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
+      }
+      continue;
+    }
+    const char* row = row_ptr(a, n, T::SIZE);
+    u32x4 v[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int at = j * G + g;
+      v[j] = (u32x4){T::NEG_INF, T::NEG_INF, T::NEG_INF, T::NEG_INF};
+      if (at < full) v[j] = *(const typename T::Raw*)(row + (long)at * 16);
+    }
+    const float edge = g < rest ? T::get(row, full * E + g) : -INFINITY;
+    float m, S;
+
+    if constexpr (!DISTILL) {
+      const int y = min(max(get_int(a.tokens, a.tok_bytes, n), 0), a.V - 1);
+      const float zy = T::get(row, y);
+      row_stats<T, G, NV>(v, edge, a, red[phase], wave, m, S);
+      const TokenOut o = token_head(a, n, zy - m, S);
+      if (g == 0) {
+        if (a.per_row) a.per_row[n] = o.lp;
+        if (a.stats) a.stats[n] = make_float4(m, S, a.head == HEAD_LOGPROB ? a.inv_tau : 0.0f, zy - m);
+        acc += (double)o.loss;
+      }
+      if (out) {
+        const float c = w * o.c, scale = -c / S;
+        float f[E];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int at = j * G + g;
+          T::unpack(v[j], f);
+#pragma unroll
+          for (int e = 0; e < E; ++e) f[e] = scale * exp_d(f[e] - m, a.c_hi, a.c_lo);
+          if (at < full) *(typename T::Raw*)(out + (long)at * 16) = T::pack(f);
+        }
+        if (g < rest) T::put(out, full * E + g, scale * exp_d(edge - m, a.c_hi, a.c_lo));
+        // the token's own element, c (1 - p), by the lane that wrote its place above
+        if (g == (y < full * E ? (y / E) % G : y - full * E)) T::put(out, y, -c * expm1f(o.lp));
+      }
+    } else {
+      List l;
+      l.idx = (int*)lists + slot * a.k;
+      l.e = (float*)lists + (Sh::ROWS + slot) * a.k;
+      const bool lister = G <= 64 || wave == 0;      // a row of several waves: the first has the list
+      if (lister) {
+        list_load<Sh::GL>(a, n, g, l);
+        if (G > 64 && g == 0) kept_flag[phase] = l.kept;
+      }
+      row_stats<T, G, NV>(v, edge, a, red[phase], wave, m, S);
+      const int kept = G > 64 ? kept_flag[phase] : l.kept;
+      if (lister) {
+        const float loss = list_loss<T, Sh::GL>(a, row, g, l, m, S);
+        if (g == 0) {
+          if (a.per_row) a.per_row[n] = loss;
+          acc += (double)loss;
+        }
+      }
+      if (out) {
+        const float c = kept ? -w : 0.0f, scale = kept ? w / S : 0.0f;
+        float f[E];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int at = j * G + g;
+          T::unpack(v[j], f);
+#pragma unroll
+          for (int e = 0; e < E; ++e) f[e] = scale * exp_d(f[e] - m, a.c_hi, a.c_lo);
+          if (at < full) *(typename T::Raw*)(out + (long)at * 16) = T::pack(f);
+        }
+        if (g < rest) T::put(out, full * E + g, scale * exp_d(edge - m, a.c_hi, a.c_lo));
+        // the listed classes' elements go over what the pieces' lanes have just written
+        if constexpr (G > 64) __syncthreads();
+        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (lister && kept) list_grad<T, Sh::GL>(a, row, out, g, l, m, 1.0f / S, c);
+      }
+    }
+    phase ^= 1;
+  }
+  if (a.partial) {
+    if (g == 0) wg_sum[slot] = acc;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double s = 0.0;
+      for (int i = 0; i < Sh::ROWS; ++i) s += wg_sum[i];
+      a.partial[blockIdx.x] = s;
+    }
+  }
+}
+
+// -------------------------------------------------------------------------- rows wider than the registers: two reads
+constexpr int WIDE = 1024;
+template <typename T, bool DISTILL>
+__global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
+  constexpr int E = T::E;
+  __shared__ float2 red[2][WIDE / 64];
+  __shared__ int kept_flag[2];
+  extern __shared__ char lists[];
+  if (a.only_if_rescaled && *a.upstream == 1.0f) return;
+  const int g = threadIdx.x, wave = threadIdx.x >> 6;
+  const int full = a.V / E, rest = a.V - full * E;
+  float w = a.weight * (a.count ? 1.0f / (float)max(*a.count, 1) : a.inv_count);
+  if (a.upstream) w *= *a.upstream;
+  double acc = 0.0;
+  int phase = 0;
+  for (int n = blockIdx.x; n < a.N; n += gridDim.x) {
+    char* out = a.dz ? (char*)a.dz + (long)n * a.V * T::SIZE : nullptr;
+    if (a.mask && !a.mask[n]) {
+      if (out) zero_row<T, WIDE>(out, g, full, rest);
+      if (g == 0) {
+        if (a.per_row) a.per_row[n] = 0.0f;
+        if (a.stats) a.stats[n] = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
+      }
+      continue;
+    }
+    const char* row = row_ptr(a, n, T::SIZE);
+    const float edge = g < rest ? T::get(row, full * E + g) : -INFINITY;
+    // the lane's running maximum and sum
+    float mx = fmaxf(edge, -FLT_MAX);
+    float s = exp_d(edge - mx, a.c_hi, a.c_lo);
+    float f[E];
+    for (int j = g; j < full; j += WIDE) {
+      T::unpack(*(const typename T::Raw*)(row + (long)j * 16), f);
+      float top = f[0];
+#pragma unroll
+      for (int e = 1; e < E; ++e) top = fmaxf(top, f[e]);
+      if (top > mx) {
+        s *= exp_d(mx - top, a.c_hi, a.c_lo);
+        mx = top;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) s += exp_d(f[e] - mx, a.c_hi, a.c_lo);
+    }
+    int y = 0;
+    float zy = 0.0f;
+    List l;
+    if constexpr (!DISTILL) {
+      y = min(max(get_int(a.tokens, a.tok_bytes, n), 0), a.V - 1);
+      zy = T::get(row, y);
+    } else {
+      l.idx = (int*)lists;
+      l.e = (float*)lists + a.k;
+      if (wave == 0) {
+        list_load<64>(a, n, g, l);
+        if (g == 0) kept_flag[phase] = l.kept;
+      }
+    }
+    const float mw = group_max<64>(mx);
+    s = group_sum<64>(s * exp_d(mx - mw, a.c_hi, a.c_lo));
+    if ((g & 63) == 0) red[phase][wave] = make_float2(mw, s);
+    __syncthreads();
+    float m = -FLT_MAX;
+    for (int i = 0; i < WIDE / 64; ++i) m = fmaxf(m, red[phase][i].x);
+    double sum = 0.0;
+    for (int i = 0; i < WIDE / 64; ++i) sum += (double)(red[phase][i].y * exp_d(red[phase][i].x - m, a.c_hi, a.c_lo));
+    const float S = (float)sum;
+
+    float c, scale, lp = 0.0f;
+    int kept = 1;
+    if constexpr (!DISTILL) {
+      const TokenOut o = token_head(a, n, zy - m, S);
+      if (g == 0) {
+        if (a.per_row) a.per_row[n] = o.lp;
+        if (a.stats) a.stats[n] = make_float4(m, S, a.head == HEAD_LOGPROB ? a.inv_tau : 0.0f, zy - m);
+        acc += (double)o.loss;
+      }
+      lp = o.lp;
+      c = w * o.c;
+      scale = -c / S;
+    } else {
+      kept = kept_flag[phase];
+      if (wave == 0) {
+        const float loss = list_loss<T, 64>(a, row, g, l, m, S);
+        if (g == 0) {
+          if (a.per_row) a.per_row[n] = loss;
+          acc += (double)loss;
+        }
+      }
+      c = kept ? -w : 0.0f;
+      scale = kept ? w / S : 0.0f;
+    }
+    if (out) {
+      for (int j = g; j < full; j += WIDE) {
+        T::unpack(*(const typename T::Raw*)(row + (long)j * 16), f);
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[e] = scale * exp_d(f[e] - m, a.c_hi, a.c_lo);
+        *(typename T::Raw*)(out + (long)j * 16) = T::pack(f);
+      }
+      if (g < rest) T::put(out, full * E + g, scale * exp_d(edge - m, a.c_hi, a.c_lo));
+      if constexpr (!DISTILL) {
+        if (g == (y < full * E ? (y / E) % WIDE : y - full * E)) T::put(out, y, -c * expm1f(lp));
+      } else {
+        __syncthreads();
+        if (wave == 0 && kept) list_grad<T, 64>(a, row, out, g, l, m, 1.0f / S, c);
+      }
+    }
+    phase ^= 1;
+  }
+  if (a.partial && g == 0) a.partial[blockIdx.x] = acc;
+}
+
+// ------------------------------------------------------------------------------- gradient from the rows' statistics
+// dz = c u (1[v = y] - p): m, S and c from stats, u the upstream gradient of the row (u_stride 1) or of the whole (0).
+// A row's pieces are cut into chunks so that few long rows fill the chip too.
+struct GradArgs {
+  const void* z; long sb, sl; int L, V, N; int dense;
+  const void* tokens; int tok_bytes;
+  float c_hi, c_lo, inv_tau;
+  const float4* stats; const float* upstream; int u_stride; int only_if_rescaled;
+  int lanes, chunk, chunks;          // lanes of a group; pieces of a chunk; chunks of a row
+  void* dz;
+};
+constexpr int GRAD_WG = 256;
+template <typename T>
+__global__ __launch_bounds__(GRAD_WG) void k_token_grad(GradArgs a) {
+  constexpr int E = T::E;
+  if (a.only_if_rescaled && *a.upstream == 1.0f) return;
+  const int g = threadIdx.x & (a.lanes - 1), slot = threadIdx.x / a.lanes, groups = GRAD_WG / a.lanes;
+  const int full = a.V / E, rest = a.V - full * E;
+  const long jobs = (long)a.N * a.chunks;
+  for (long job = (long)blockIdx.x * groups + slot; job < jobs; job += (long)gridDim.x * groups) {
+    const int n = a.chunks == 1 ? (int)job : (int)(job / a.chunks);
+    const int part = a.chunks == 1 ? 0 : (int)(job - (long)n * a.chunks);
+    const int lo = part * a.chunk, hi = min(full, lo + a.chunk);
+    const bool last = part == a.chunks - 1;
+    const float4 st = a.stats[n];
+    const float c = st.z * (a.upstream ? a.upstream[(long)n * a.u_stride] : 1.0f);
+    char* out = (char*)a.dz + (long)n * a.V * T::SIZE;
+    if (c == 0.0f) {                                  // a row that is not counted, or whose upstream gradient is 0
+      const u32x4 zero = {0, 0, 0, 0};
+      for (int j = lo + g; j < hi; j += a.lanes) *(typename T::Raw*)(out + (long)j * 16) = zero;
+      if (last && g < rest) T::put(out, full * E + g, 0.0f);
+      continue;
+    }
+    long at;
+    if (a.dense) at = (long)n * a.sl;
+    else {
+      const unsigned b = (unsigned)n / (unsigned)a.L;
+      at = (long)b * a.sb + (long)((unsigned)n - b * (unsigned)a.L) * a.sl;
+    }
+    const char* row = (const char*)a.z + at * T::SIZE;
+    const float m = st.x, scale = -c / st.y;
+    float f[E];
+#pragma unroll 4
+    for (int j = lo + g; j < hi; j += a.lanes) {
+      T::unpack(*(const typename T::Raw*)(row + (long)j * 16), f);
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = scale * exp_d(f[e] - m, a.c_hi, a.c_lo);
+      *(typename T::Raw*)(out + (long)j * 16) = T::pack(f);
+    }
+    if (last && g < rest) T::put(out, full * E + g, scale * exp_d(T::get(row, full * E + g) - m, a.c_hi, a.c_lo));
+    // the token's own element, c (1 - p), by the lane that wrote its place above
+    const int y = min(max(get_int(a.tokens, a.tok_bytes, n), 0), a.V - 1);
+    const bool mine = y < full * E ? y / E >= lo && y / E < hi && ((y / E - lo) & (a.lanes - 1)) == g
+                                   : last && y - full * E == g;
+    if (mine) T::put(out, y, -c * expm1f(st.w * a.inv_tau - logf(st.y)));
+  }
+}
+
+// ------------------------------------------------------------------------------------------------- small kernels
+constexpr int SUM_WG = 1024;
+__device__ __forceinline__ double block_sum(double v, double* lds) {
+  v = group_sum<64>(v);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double s = 0.0;
+  for (int i = 0; i < (int)(blockDim.x >> 6); ++i) s += lds[i];
+  __syncthreads();
+  return s;
+}
+__global__ __launch_bounds__(SUM_WG) void k_count(const uint8_t* mask, int N, int* count) {
+  __shared__ double lds[SUM_WG / 64];
+  int c = 0;
+  const int words = ((uintptr_t)mask & 15) ? 0 : N / 16;
+  for (int i = threadIdx.x; i < words; i += SUM_WG) {
+    const u32x4 v = ((const u32x4*)mask)[i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t x = v[j] | ((v[j] >> 4) & 0x0F0F0F0Fu);  // any bit of a byte into its lowest
+      x |= (x >> 2) & 0x3F3F3F3Fu;
+      x |= (x >> 1) & 0x7F7F7F7Fu;
+      c += __popc(x & 0x01010101u);
+    }
+  }
+  for (int i = words * 16 + threadIdx.x; i < N; i += SUM_WG) c += mask[i] != 0;
+  const double s = block_sum((double)c, lds);
+  if (threadIdx.x == 0) *count = (int)s;
+}
+// loss = scale / count * sum of the partial sums, in a fixed order
+__global__ __launch_bounds__(SUM_WG) void k_finish(const double* partial, int n, const int* count, double inv_count,
+                                                   float scale, float* loss) {
+  __shared__ double lds[SUM_WG / 64];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += SUM_WG) s += partial[i];
+  s = block_sum(s, lds);
+  if (threadIdx.x == 0) *loss = (float)(s * (double)scale * (count ? 1.0 / (double)max(*count, 1) : inv_count));
+}
+
+struct PairArgs {
+  float4* stats; const float* ref; const uint8_t* mask;
+  int P, L; float beta, smooth; int average; float out_scale;
+  float* rewards; double* pair_loss;
+};
+constexpr int PAIR_WG = 256;
+// A pair's sums in 64 bits (a sequence's log-ratio is a long sum of small differences of large terms), its loss, and
+// the coefficient of its rows' gradients.
+__global__ __launch_bounds__(PAIR_WG) void k_pair(PairArgs a) {
+  __shared__ double lds[PAIR_WG / 64];
+  const int p = blockIdx.x;
+  double D[2], cnt[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const long n0 = (long)(p + h * a.P) * a.L;
+    double s = 0.0, c = 0.0;
+    for (int l = threadIdx.x; l < a.L; l += PAIR_WG) {
+      if (a.mask && !a.mask[n0 + l]) continue;
+      const float4 st = a.stats[n0 + l];
+      s += (double)st.w - log((double)st.y) - (double)(a.ref ? a.ref[n0 + l] : 0.0f);
+      c += 1.0;
+    }
+    D[h] = block_sum(s, lds);
+    cnt[h] = fmax(block_sum(c, lds), 1.0);
+    if (a.average) D[h] /= cnt[h];
+  }
+  const double margin = (double)a.beta * (D[0] - D[1]), e = (double)a.smooth;
+  const double z = exp(-fabs(margin)), soft = log1p(z);
+  const double sig = margin >= 0.0 ? 1.0 / (1.0 + z) : z / (1.0 + z);       // sigma(margin) and sigma(-margin)
+  const double gis = margin >= 0.0 ? z / (1.0 + z) : 1.0 / (1.0 + z);
+  if (threadIdx.x == 0) {
+    a.rewards[p] = (float)((double)a.beta * D[0]);
+    a.rewards[p + a.P] = (float)((double)a.beta * D[1]);
+    const double neg = margin < 0.0 ? -margin : 0.0, pos = margin > 0.0 ? margin : 0.0;
+    a.pair_loss[p] = (1.0 - e) * (soft + neg) + e * (soft + pos);
+  }
+  const double slope = -(double)a.out_scale * (double)a.beta / (double)a.P * ((1.0 - e) * gis - e * sig);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const long n0 = (long)(p + h * a.P) * a.L;
+    const float c = (float)((h ? -slope : slope) / (a.average ? cnt[h] : 1.0));
+    for (int l = threadIdx.x; l < a.L; l += PAIR_WG)
+      if (!a.mask || a.mask[n0 + l]) a.stats[n0 + l].z = c;
+  }
+}
+
+// ----------------------------------------------------------------------------------------------------- host side
+static int check_logits(const d3pm_logits* z, const char* who) {
+  D3PM_CHECK_ARG(z != nullptr, "%s: null logits descriptor", who);
+  D3PM_CHECK_ARG(z->dtype >= D3PM_F32 && z->dtype <= D3PM_BF16, "%s: logits dtype %d", who, z->dtype);
+  D3PM_CHECK_ARG(z->V >= 1 && z->V <= (1 << 27), "%s: V = %d classes, need 1 .. 2^27", who, z->V);
+  D3PM_CHECK_ARG(z->B >= 0 && z->L >= 0 && (z->B == 0 || z->L <= (long)(INT_MAX - 65536) / z->B),
+                 "%s: B = %ld x L = %ld positions, need fewer than 2^31 - 65536", who, z->B, z->L);
+  D3PM_CHECK_ARG(z->stride_b >= 0 && z->stride_l >= 0, "%s: negative strides", who);
+  D3PM_CHECK_ARG(z->data != nullptr || z->B * z->L == 0, "%s: null logits", who);
+  return D3PM_OK;
+}
+static int check_temperature(float t, const char* who) {
+  D3PM_CHECK_ARG(t >= 1e-6f && t <= 1e6f, "%s: temperature %g, need 1e-6 .. 1e6", who, (double)t);
+  return D3PM_OK;
+}
+static int check_int_bytes(int b, const char* what, const char* who) {
+  D3PM_CHECK_ARG(b == 4 || b == 8, "%s: %s of %d bytes, need int32 or int64", who, what, b);
+  return D3PM_OK;
+}
+
+// log2(e) / tau in two floats, the second above 0: a class ruled out with -inf stays -inf in both products of exp_d
+static void set_temperature(float tau, float* c_hi, float* c_lo, float* inv_tau) {
+  const double c = 1.44269504088896340736 / (double)tau;
+  *c_hi = (float)c;
+  if ((double)*c_hi >= c) *c_hi = std::nextafterf(*c_hi, 0.0f);
+  *c_lo = (float)(c - (double)*c_hi);
+  *inv_tau = (float)(1.0 / (double)tau);
+}
+static bool is_dense(const d3pm_logits* z) { return z->B <= 1 || z->stride_b == z->L * z->stride_l; }
+
+static RowArgs row_args(const d3pm_logits* z, float tau) {
+  RowArgs a{};
+  a.z = z->data; a.sb = z->stride_b; a.sl = z->stride_l;
+  a.L = (int)z->L; a.V = z->V; a.N = (int)(z->B * z->L); a.dense = is_dense(z) ? 1 : 0;
+  set_temperature(tau, &a.c_hi, &a.c_lo, &a.inv_tau);
+  a.inv_count = 1.0f;
+  return a;
+}
+
+// Launches the narrowest shape that holds a row; *grid: the workgroups it took (as many partial sums).
+template <typename T, int G, int NV, bool DISTILL>
+static int launch_rows(const RowArgs& a, int* grid, hipStream_t s) {
+  typedef Shape<G> Sh;
+  const int want = (a.N - 1) / Sh::ROWS + 1;
+  // parts of a wave: 8 workgroups of 256 a compute unit; whole workgroups: a row each as long as the partials allow
+  *grid = std::min(want, G <= 64 ? 2048 : MAX_PARTIALS);
+  const size_t lds = DISTILL ? (size_t)Sh::ROWS * a.k * 8 : 0;
+  hipLaunchKernelGGL((k_rows<T, G, NV, DISTILL>), dim3(*grid), dim3(Sh::WG), lds, s, a);
+  D3PM_LAUNCH_CHECK("k_rows");
+  return D3PM_OK;
+}
+template <typename T, bool DISTILL>
+static int dispatch_rows(const RowArgs& a, int* grid, hipStream_t s) {
+  const int full = a.V / T::E;
+  if (full <= 8) return launch_rows<T, 8, 1, DISTILL>(a, grid, s);
+  if (full <= 16) return launch_rows<T, 16, 1, DISTILL>(a, grid, s);
+  if (full <= 32) return launch_rows<T, 32, 1, DISTILL>(a, grid, s);
+  if (full <= 64) return launch_rows<T, 64, 1, DISTILL>(a, grid, s);
+  if (full <= 128) return launch_rows<T, 64, 2, DISTILL>(a, grid, s);
+  if (full <= 256) return launch_rows<T, 64, 4, DISTILL>(a, grid, s);
+  if (full <= 512) return launch_rows<T, 256, 2, DISTILL>(a, grid, s);
+  if (full <= 1024) return launch_rows<T, 256, 4, DISTILL>(a, grid, s);
+  if (full <= 2048) return launch_rows<T, 256, 8, DISTILL>(a, grid, s);
+  if (full <= 4096) return launch_rows<T, 512, 8, DISTILL>(a, grid, s);
+  if (full <= 8192) return launch_rows<T, 512, 16, DISTILL>(a, grid, s);
+  *grid = std::min(a.N, MAX_PARTIALS);
+  hipLaunchKernelGGL((k_rows_wide<T, DISTILL>), dim3(*grid), dim3(WIDE), DISTILL ? (size_t)a.k * 8 : 0, s, a);
+  D3PM_LAUNCH_CHECK("k_rows_wide");
+  return D3PM_OK;
+}
+template <bool DISTILL>
+static int run_rows(const RowArgs& a, int dtype, int* grid, hipStream_t s) {
+  return dtype == D3PM_F32 ? dispatch_rows<F32, DISTILL>(a, grid, s)
+       : dtype == D3PM_F16 ? dispatch_rows<F16, DISTILL>(a, grid, s) : dispatch_rows<BF16, DISTILL>(a, grid, s);
+}
+
+static int run_grad(const d3pm_logits* z, const void* tokens, int tok_bytes, float tau, const float* stats,
+                    const float* upstream, int per_row, int only_if_rescaled, void* dz, hipStream_t s) {
+  GradArgs a{};
+  a.z = z->data; a.sb = z->stride_b; a.sl = z->stride_l;
+  a.L = (int)z->L; a.V = z->V; a.N = (int)(z->B * z->L); a.dense = is_dense(z) ? 1 : 0;
+  a.tokens = tokens; a.tok_bytes = tok_bytes;
+  set_temperature(tau, &a.c_hi, &a.c_lo, &a.inv_tau);
+  a.stats = (const float4*)stats; a.upstream = upstream; a.u_stride = per_row; a.only_if_rescaled = only_if_rescaled;
+  a.dz = dz;
+  const int full = a.V / (z->dtype == D3PM_F32 ? 4 : 8);
+  a.lanes = 8;
+  while (a.lanes < 256 && a.lanes < full) a.lanes <<= 1;
+  a.chunk = a.lanes * 8;
+  a.chunks = std::max(1, (full + a.chunk - 1) / a.chunk);
+  const long jobs = (long)a.N * a.chunks, per = GRAD_WG / a.lanes;
+  const int grid = (int)std::min<long>((jobs + per - 1) / per, 4096);
+  if (z->dtype == D3PM_F32) hipLaunchKernelGGL((k_token_grad<F32>), dim3(grid), dim3(GRAD_WG), 0, s, a);
+  else if (z->dtype == D3PM_F16) hipLaunchKernelGGL((k_token_grad<F16>), dim3(grid), dim3(GRAD_WG), 0, s, a);
+  else hipLaunchKernelGGL((k_token_grad<BF16>), dim3(grid), dim3(GRAD_WG), 0, s, a);
+  D3PM_LAUNCH_CHECK("k_token_grad");
+  return D3PM_OK;
+}
+
+// The count of the mask (first 8 bytes of the workspace) and the partial sums behind it.
+struct Scratch { int* count; double* partial; };
+static int scratch(void* ws, size_t have, long partials, Scratch* out) {
+  D3PM_CHECK_WORKSPACE(ws, have, 8 + 8 * (size_t)partials);
+  out->count = (int*)ws;
+  out->partial = (double*)ws + 1;
+  return D3PM_OK;
+}
+static int run_count(const uint8_t* mask, int N, int* count, hipStream_t s) {
+  hipLaunchKernelGGL(k_count, dim3(1), dim3(SUM_WG), 0, s, mask, N, count);
+  D3PM_LAUNCH_CHECK("k_count");
+  return D3PM_OK;
+}
+static int run_finish(const double* partial, int n, const int* count, double inv_count, float scale, float* loss,
+                      hipStream_t s) {
+  hipLaunchKernelGGL(k_finish, dim3(1), dim3(SUM_WG), 0, s, partial, n, count, inv_count, scale, loss);
+  D3PM_LAUNCH_CHECK("k_finish");
+  return D3PM_OK;
+}
+
+// the part that the distillation and the policy loss share: count, pass over the rows, loss
+template <bool DISTILL>
+static int run_mean_loss(RowArgs& a, int dtype, float out_scale, float* loss, const float* upstream,
+                         int only_if_rescaled, void* ws, size_t ws_bytes, hipStream_t s) {
+  Scratch sc;
+  if (int rc = scratch(ws, ws_bytes, MAX_PARTIALS, &sc)) return rc;
+  const double inv = 1.0 / (double)std::max(a.N, 1);
+  a.inv_count = (float)inv;
+  a.upstream = upstream;
+  a.only_if_rescaled = upstream ? only_if_rescaled : 0;
+  int grid = 0;
+  if (a.N > 0) {
+    if (a.mask) {
+      if (int rc = run_count(a.mask, a.N, sc.count, s)) return rc;
+      a.count = sc.count;
+    }
+    a.partial = loss ? sc.partial : nullptr;
+    if (int rc = run_rows<DISTILL>(a, dtype, &grid, s)) return rc;
+  }
+  if (!loss) return D3PM_OK;
+  return run_finish(sc.partial, grid, a.count, inv, out_scale, loss, s);
+}
+
+}  // namespace ft
+}  // namespace d3pm
+
+using namespace d3pm;
+using namespace d3pm::ft;
+
+extern "C" size_t d3pm_objective_workspace(long B, long L) {
+  (void)L;
+  return 8 + 8 * (size_t)std::max<long>(MAX_PARTIALS, B);
+}
+
+extern "C" int d3pm_token_logprobs(const d3pm_logits* z, const void* tokens, int tok_bytes, const uint8_t* mask,
+                                   float temperature, float* logprobs, float* row_stats, void* stream) {
+  const char* who = "d3pm_token_logprobs";
+  if (int rc = check_logits(z, who)) return rc;
+  if (int rc = check_temperature(temperature, who)) return rc;
+  if (int rc = check_int_bytes(tok_bytes, "tokens", who)) return rc;
+  if (z->B * z->L == 0) return D3PM_OK;
+  D3PM_CHECK_ARG(tokens && logprobs, "%s: null pointer", who);
+  RowArgs a = row_args(z, temperature);
+  a.head = HEAD_LOGPROB;
+  a.tokens = tokens; a.tok_bytes = tok_bytes; a.mask = mask;
+  a.per_row = logprobs; a.stats = (float4*)row_stats;
+  int grid;
+  return run_rows<false>(a, z->dtype, &grid, (hipStream_t)stream);
+}
+
+extern "C" int d3pm_token_grad(const d3pm_logits* z, const void* tokens, int tok_bytes, float temperature,
+                               const float* row_stats, const float* upstream, int upstream_per_row,
+                               int only_if_rescaled, void* dlogits, void* stream) {
+  const char* who = "d3pm_token_grad";
+  if (int rc = check_logits(z, who)) return rc;
+  if (int rc = check_temperature(temperature, who)) return rc;
+  if (int rc = check_int_bytes(tok_bytes, "tokens", who)) return rc;
+  D3PM_CHECK_ARG(!only_if_rescaled || (upstream && !upstream_per_row), "%s: only_if_rescaled needs one upstream gradient", who);
+  if (z->B * z->L == 0) return D3PM_OK;
+  D3PM_CHECK_ARG(tokens && row_stats && dlogits, "%s: null pointer", who);
+  return run_grad(z, tokens, tok_bytes, temperature, row_stats, upstream, upstream_per_row ? 1 : 0, only_if_rescaled,
+                  dlogits, (hipStream_t)stream);
+}
+
+extern "C" int d3pm_topk_distill_loss(const d3pm_logits* z, const void* teacher_logits, int teacher_dtype,
+                                      const void* teacher_index, int index_bytes, int k, const uint8_t* mask,
+                                      float temperature, float out_scale, const float* upstream, int only_if_rescaled,
+                                      float* loss, float* per_token, void* dlogits, void* workspace,
+                                      size_t workspace_bytes, void* stream) {
+  const char* who = "d3pm_topk_distill_loss";
+  if (int rc = check_logits(z, who)) return rc;
+  if (int rc = check_temperature(temperature, who)) return rc;
+  if (int rc = check_int_bytes(index_bytes, "teacher_index", who)) return rc;
+  D3PM_CHECK_ARG(teacher_dtype >= D3PM_F32 && teacher_dtype <= D3PM_BF16, "%s: teacher dtype %d", who, teacher_dtype);
+  D3PM_CHECK_ARG(k >= 1 && k <= MAX_K, "%s: k = %d entries, need 1 .. %d", who, k, MAX_K);
+  D3PM_CHECK_ARG(z->B * z->L == 0 || (teacher_logits && teacher_index), "%s: null teacher", who);
+  D3PM_CHECK_ARG(std::isfinite(out_scale), "%s: out_scale is not finite", who);
+  RowArgs a = row_args(z, temperature);
+  a.head = HEAD_DISTILL;
+  a.mask = mask;
+  a.t_logits = teacher_logits; a.t_dtype = teacher_dtype;
+  a.t_index = teacher_index; a.t_index_bytes = index_bytes; a.k = k;
+  a.weight = out_scale * temperature;
+  a.per_row = per_token; a.dz = dlogits;
+  return run_mean_loss<true>(a, z->dtype, out_scale, loss, upstream, only_if_rescaled, workspace, workspace_bytes,
+                             (hipStream_t)stream);
+}
+
+extern "C" int d3pm_policy_loss(const d3pm_logits* z, const void* tokens, int tok_bytes, const float* old_logprobs,
+                                const float* advantages, int advantages_per_sequence, const float* ref_logprobs,
+                                const uint8_t* mask, float temperature, float clip_low, float clip_high,
+                                float kl_coeff, float out_scale, const float* upstream, int only_if_rescaled,
+                                float* loss, float* logprobs, void* dlogits, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+  const char* who = "d3pm_policy_loss";
+  if (int rc = check_logits(z, who)) return rc;
+  if (int rc = check_temperature(temperature, who)) return rc;
+  if (int rc = check_int_bytes(tok_bytes, "tokens", who)) return rc;
+  D3PM_CHECK_ARG(clip_low >= 0.0f && clip_low <= 1.0f && clip_high >= 0.0f, "%s: clip range [1 - %g, 1 + %g]", who,
+                 (double)clip_low, (double)clip_high);
+  D3PM_CHECK_ARG(std::isfinite(kl_coeff) && std::isfinite(out_scale), "%s: kl_coeff or out_scale is not finite", who);
+  D3PM_CHECK_ARG(z->B * z->L == 0 || (tokens && old_logprobs && advantages), "%s: null pointer", who);
+  D3PM_CHECK_ARG(kl_coeff == 0.0f || ref_logprobs || z->B * z->L == 0, "%s: kl_coeff without ref_logprobs", who);
+  RowArgs a = row_args(z, temperature);
+  a.head = HEAD_POLICY;
+  a.tokens = tokens; a.tok_bytes = tok_bytes; a.mask = mask;
+  a.old_lp = old_logprobs; a.adv = advantages; a.adv_per_seq = advantages_per_sequence ? 1 : 0;
+  a.ref_lp = kl_coeff == 0.0f ? nullptr : ref_logprobs;
+  a.clip_lo = 1.0f - clip_low; a.clip_hi = 1.0f + clip_high; a.kl_coeff = kl_coeff;
+  a.weight = out_scale / temperature;
+  a.per_row = logprobs; a.dz = dlogits;
+  return run_mean_loss<false>(a, z->dtype, out_scale, loss, upstream, only_if_rescaled, workspace, workspace_bytes,
+                              (hipStream_t)stream);
+}
+
+extern "C" int d3pm_preference_loss(const d3pm_logits* z, const void* tokens, int tok_bytes, const float* ref_logprobs,
+                                    const uint8_t* mask, float beta, float label_smoothing, int average,
+                                    float out_scale, float* loss, float* rewards, float* row_stats, void* dlogits,
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "d3pm_preference_loss";
+  if (int rc = check_logits(z, who)) return rc;
+  if (int rc = check_int_bytes(tok_bytes, "tokens", who)) return rc;
+  D3PM_CHECK_ARG(z->B >= 2 && z->B % 2 == 0, "%s: B = %ld sequences, need pairs", who, z->B);
+  D3PM_CHECK_ARG(std::isfinite(beta) && std::isfinite(out_scale), "%s: beta or out_scale is not finite", who);
+  D3PM_CHECK_ARG(label_smoothing >= 0.0f && label_smoothing <= 1.0f, "%s: label_smoothing %g", who, (double)label_smoothing);
+  D3PM_CHECK_ARG(loss && rewards, "%s: null output", who);
+  D3PM_CHECK_ARG(z->L == 0 || (tokens && row_stats), "%s: null pointer", who);
+  const int P = (int)(z->B / 2);
+  Scratch sc;
+  if (int rc = scratch(workspace, workspace_bytes, P, &sc)) return rc;
+  hipStream_t s = (hipStream_t)stream;
+  RowArgs a = row_args(z, 1.0f);
+  if (a.N > 0) {
+    a.head = HEAD_PREFERENCE;
+    a.tokens = tokens; a.tok_bytes = tok_bytes; a.mask = mask;
+    a.stats = (float4*)row_stats;
+    int grid;
+    if (int rc = run_rows<false>(a, z->dtype, &grid, s)) return rc;
+  }
+  PairArgs pa{};
+  pa.stats = (float4*)row_stats;
+  pa.ref = ref_logprobs; pa.mask = mask;
+  pa.P = P; pa.L = (int)z->L; pa.beta = beta; pa.smooth = label_smoothing; pa.average = average; pa.out_scale = out_scale;
+  pa.rewards = rewards; pa.pair_loss = sc.partial;
+  hipLaunchKernelGGL(k_pair, dim3(P), dim3(PAIR_WG), 0, s, pa);
+  D3PM_LAUNCH_CHECK("k_pair");
+  if (int rc = run_finish(sc.partial, P, nullptr, 1.0 / (double)P, out_scale, loss, s)) return rc;
+  if (!dlogits || a.N == 0) return D3PM_OK;
+  return run_grad(z, tokens, tok_bytes, 1.0f, row_stats, nullptr, 0, 0, dlogits, s);
+}

@@ -609,11 +609,234 @@ std::tuple<Tensor, Tensor> corrupt(const Tensor& qbar_digest, const Tensor& qone
   return {x_t, probs};
 }
 
+// ---- fine-tuning objectives: losses at logits [..., V] of float32, float16 or bfloat16, any strides
+int float_dtype(const Tensor& t, const char* what) {
+  const auto st = t.scalar_type();
+  TORCH_CHECK_TYPE(st == at::kFloat || st == at::kHalf || st == at::kBFloat16, "d3pm_mi355x: ", what,
+                   " must be float32, float16 or bfloat16, got ", st);
+  return st == at::kFloat ? D3PM_F32 : st == at::kHalf ? D3PM_F16 : D3PM_BF16;
+}
+void need_same_device(const Tensor& t, const Tensor& z, const char* what) {
+  TORCH_CHECK(t.device() == z.device(), "d3pm_mi355x: ", what, " is on ", t.device(), ", the logits on ", z.device());
+}
+// The library's view of logits [B, ..., V]: `rows` keeps the tensor that it points into (a copy where the middle
+// dimensions cannot be walked with one stride, or the classes do not lie side by side).
+struct LogitsView { Tensor rows; d3pm_logits desc; };
+LogitsView logits_view(const Tensor& z, const Tensor& per_row, const char* per_row_name) {
+  TORCH_CHECK(z.is_cuda(), "d3pm_mi355x: logits must live on an MI355X (device='cuda'); there is no CPU path");
+  TORCH_CHECK_VALUE(z.dim() == per_row.dim() + 1 && z.dim() >= 2 && z.sizes().slice(0, z.dim() - 1) == per_row.sizes(),
+                    "d3pm_mi355x: logits must have the shape of ", per_row_name, " and a trailing class dimension, got ",
+                    z.sizes(), " and ", per_row.sizes());
+  const int64_t nd = z.dim(), V = z.size(-1);
+  TORCH_CHECK_VALUE(V >= 1 && V <= (1 << 27), "d3pm_mi355x: logits have ", V, " classes, need 1 .. 2^27");
+  LogitsView v{z, {}};
+  v.desc.dtype = float_dtype(z, "logits");
+  v.desc.V = (int)V;
+  v.desc.B = z.size(0);
+  v.desc.L = v.desc.B ? per_row.numel() / v.desc.B : 0;
+  bool walk = V == 1 || z.stride(-1) == 1;
+  int64_t inner = -1, next = 0;                 // stride of the innermost middle dimension; what the next one must be
+  for (int64_t i = nd - 2; i >= 1 && walk; --i) {
+    if (z.size(i) == 1) continue;
+    if (inner < 0) inner = z.stride(i);
+    else walk = z.stride(i) == next;
+    next = z.stride(i) * z.size(i);
+  }
+  if (!walk) v.rows = z.contiguous();
+  v.desc.stride_b = walk ? z.stride(0) : v.desc.L * V;
+  v.desc.stride_l = !walk ? V : inner >= 0 ? inner : v.desc.stride_b;
+  v.desc.data = v.rows.data_ptr();
+  return v;
+}
+const uint8_t* mask_ptr(const OptTensor& m, const Tensor& per_row, const Tensor& z) {
+  if (!m.has_value() || !m->defined()) return nullptr;
+  need_device(*m, "mask");
+  need_same_device(*m, z, "mask");
+  TORCH_CHECK_TYPE(m->scalar_type() == at::kBool, "d3pm_mi355x: mask must be bool, got ", m->scalar_type());
+  need_same_shape(*m, per_row, "mask and the logits' positions");
+  return (const uint8_t*)m->data_ptr();
+}
+const float* row_f32(const Tensor& t, const Tensor& per_row, const Tensor& z, const char* what) {
+  need_same_device(t, z, what);
+  need_same_shape(t, per_row, what);
+  return f32(t, what);
+}
+int token_bytes(const Tensor& t, const Tensor& z, const char* what) {
+  need_same_device(t, z, what);
+  return tok_bytes(t, what);
+}
+const float* upstream_ptr(const Tensor& u, const Tensor& z) {
+  need_same_device(u, z, "upstream");
+  need_numel(u, 1, "upstream");
+  return f32(u, "upstream");
+}
+void need_grad_like(const Tensor& dz, const Tensor& z) {
+  need_device(dz, "dlogits");
+  need_same_device(dz, z, "dlogits");
+  need_same_shape(dz, z, "dlogits and logits");
+  TORCH_CHECK_TYPE(dz.scalar_type() == z.scalar_type(), "d3pm_mi355x: dlogits must have the logits' type");
+}
+Tensor objective_workspace(const d3pm_logits& d, const Tensor& z, size_t* bytes) {
+  *bytes = d3pm_objective_workspace(d.B, d.L);
+  return at::empty({(int64_t)(*bytes / 8 + 1)}, z.options().dtype(at::kDouble));
+}
+Tensor grad_buffer(const Tensor& z, bool want) {
+  return want ? at::empty(z.sizes(), z.options().memory_format(at::MemoryFormat::Contiguous))
+              : at::empty({0}, z.options());
+}
+
+// log_softmax(logits / temperature) at the tokens, float32; stats [.., 4]: what token_grad_ takes
+std::tuple<Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& tokens, const OptTensor& mask,
+                                          double temperature, bool want_stats) {
+  D3PM_GUARD(logits);
+  auto v = logits_view(logits, tokens, "tokens");
+  auto fo = logits.options().dtype(at::kFloat);
+  Tensor lp = at::empty(tokens.sizes(), fo), stats = at::empty({want_stats ? tokens.numel() : 0, 4}, fo);
+  check_rc(d3pm_token_logprobs(&v.desc, tokens.data_ptr(), token_bytes(tokens, logits, "tokens"),
+                               mask_ptr(mask, tokens, logits), (float)temperature, lp.data_ptr<float>(),
+                               want_stats ? stats.data_ptr<float>() : nullptr, stream()));
+  return {lp, stats};
+}
+
+// the gradient at the logits from the rows' statistics, into dlogits
+void token_grad_(const Tensor& logits, const Tensor& tokens, double temperature, const Tensor& stats,
+                 const Tensor& upstream, bool per_row, bool only_if_rescaled, Tensor dlogits) {
+  D3PM_GUARD(logits);
+  auto v = logits_view(logits, tokens, "tokens");
+  need_grad_like(dlogits, logits);
+  need_same_device(stats, logits, "stats");
+  need_numel(stats, tokens.numel() * 4, "stats");
+  const float* u = per_row ? row_f32(upstream, tokens, logits, "upstream and tokens") : upstream_ptr(upstream, logits);
+  check_rc(d3pm_token_grad(&v.desc, tokens.data_ptr(), token_bytes(tokens, logits, "tokens"), (float)temperature,
+                           f32(stats, "stats"), u, per_row, only_if_rescaled, dlogits.data_ptr(), stream()));
+}
+
+struct Teacher { int dtype, index_bytes, k; };
+Teacher check_teacher(const Tensor& tl, const Tensor& ti, const Tensor& z) {
+  need_device(tl, "teacher_logits"); need_device(ti, "teacher_index");
+  need_same_device(tl, z, "teacher_logits"); need_same_device(ti, z, "teacher_index");
+  need_same_shape(tl, ti, "teacher_logits and teacher_index");
+  const int64_t k = tl.dim() ? tl.size(-1) : 0;
+  TORCH_CHECK_VALUE(tl.dim() == z.dim() && tl.sizes().slice(0, z.dim() - 1) == z.sizes().slice(0, z.dim() - 1),
+                    "d3pm_mi355x: teacher_logits must be [.., k] over the logits' positions, got ", tl.sizes(), " for ",
+                    z.sizes());
+  TORCH_CHECK_VALUE(k >= 1 && k <= 256, "d3pm_mi355x: the teacher's lists have ", k, " entries, need 1 .. 256");
+  return {float_dtype(tl, "teacher_logits"), tok_bytes(ti, "teacher_index"), (int)k};
+}
+
+// (loss [], per_token, dlogits): distillation from a teacher's top logits
+std::tuple<Tensor, Tensor, Tensor> topk_distill_loss(const Tensor& logits, const Tensor& teacher_logits,
+                                                     const Tensor& teacher_index, const OptTensor& mask,
+                                                     double temperature, double out_scale, bool want_grad) {
+  D3PM_GUARD(logits);
+  const Teacher t = check_teacher(teacher_logits, teacher_index, logits);
+  auto fo = logits.options().dtype(at::kFloat);
+  Tensor loss = at::empty({}, fo), per = at::empty(logits.sizes().slice(0, logits.dim() - 1), fo);
+  auto v = logits_view(logits, per, "the teacher's positions");
+  Tensor dz = grad_buffer(logits, want_grad);
+  size_t wsb;
+  Tensor ws = objective_workspace(v.desc, logits, &wsb);
+  check_rc(d3pm_topk_distill_loss(&v.desc, teacher_logits.data_ptr(), t.dtype, teacher_index.data_ptr(), t.index_bytes,
+                                  t.k, mask_ptr(mask, per, logits), (float)temperature, (float)out_scale, nullptr, 0,
+                                  loss.data_ptr<float>(), per.data_ptr<float>(), want_grad ? dz.data_ptr() : nullptr,
+                                  ws.data_ptr(), wsb, stream()));
+  return {loss, per, dz};
+}
+// its gradient alone, times upstream, into dlogits
+void topk_distill_grad_(const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_index,
+                        const OptTensor& mask, double temperature, double out_scale, const Tensor& upstream,
+                        bool only_if_rescaled, Tensor dlogits) {
+  D3PM_GUARD(logits);
+  const Teacher t = check_teacher(teacher_logits, teacher_index, logits);
+  const Tensor rows = logits.select(-1, 0);
+  auto v = logits_view(logits, rows, "the teacher's positions");
+  need_grad_like(dlogits, logits);
+  size_t wsb;
+  Tensor ws = objective_workspace(v.desc, logits, &wsb);
+  check_rc(d3pm_topk_distill_loss(&v.desc, teacher_logits.data_ptr(), t.dtype, teacher_index.data_ptr(), t.index_bytes,
+                                  t.k, mask_ptr(mask, rows, logits), (float)temperature, (float)out_scale,
+                                  upstream_ptr(upstream, logits), only_if_rescaled, nullptr, nullptr, dlogits.data_ptr(),
+                                  ws.data_ptr(), wsb, stream()));
+}
+
+struct PolicyIn { const float* old_lp; const float* adv; int per_seq; const float* ref; };
+PolicyIn check_policy(const Tensor& tokens, const Tensor& old_lp, const Tensor& adv, const OptTensor& ref, const Tensor& z) {
+  PolicyIn p{};
+  p.old_lp = row_f32(old_lp, tokens, z, "old_logprobs and tokens");
+  p.per_seq = adv.dim() == 1 && tokens.dim() > 1;
+  if (p.per_seq) {
+    need_numel(adv, tokens.size(0), "advantages (one per sequence)");
+    need_same_device(adv, z, "advantages");
+    p.adv = f32(adv, "advantages");
+  } else p.adv = row_f32(adv, tokens, z, "advantages and tokens");
+  p.ref = ref.has_value() && ref->defined() ? row_f32(*ref, tokens, z, "ref_logprobs and tokens") : nullptr;
+  return p;
+}
+// (loss [], logprobs, dlogits): clipped policy loss with a KL term
+std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs,
+                                               const Tensor& advantages, const OptTensor& ref_logprobs,
+                                               const OptTensor& mask, double temperature, double clip_low,
+                                               double clip_high, double kl_coeff, double out_scale, bool want_grad) {
+  D3PM_GUARD(logits);
+  auto v = logits_view(logits, tokens, "tokens");
+  const PolicyIn p = check_policy(tokens, old_logprobs, advantages, ref_logprobs, logits);
+  auto fo = logits.options().dtype(at::kFloat);
+  Tensor loss = at::empty({}, fo), lp = at::empty(tokens.sizes(), fo), dz = grad_buffer(logits, want_grad);
+  size_t wsb;
+  Tensor ws = objective_workspace(v.desc, logits, &wsb);
+  check_rc(d3pm_policy_loss(&v.desc, tokens.data_ptr(), token_bytes(tokens, logits, "tokens"), p.old_lp, p.adv, p.per_seq,
+                            p.ref, mask_ptr(mask, tokens, logits), (float)temperature, (float)clip_low, (float)clip_high,
+                            (float)kl_coeff, (float)out_scale, nullptr, 0, loss.data_ptr<float>(), lp.data_ptr<float>(),
+                            want_grad ? dz.data_ptr() : nullptr, ws.data_ptr(), wsb, stream()));
+  return {loss, lp, dz};
+}
+// its gradient alone, times upstream, into dlogits
+void policy_grad_(const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs, const Tensor& advantages,
+                  const OptTensor& ref_logprobs, const OptTensor& mask, double temperature, double clip_low,
+                  double clip_high, double kl_coeff, double out_scale, const Tensor& upstream, bool only_if_rescaled,
+                  Tensor dlogits) {
+  D3PM_GUARD(logits);
+  auto v = logits_view(logits, tokens, "tokens");
+  const PolicyIn p = check_policy(tokens, old_logprobs, advantages, ref_logprobs, logits);
+  need_grad_like(dlogits, logits);
+  size_t wsb;
+  Tensor ws = objective_workspace(v.desc, logits, &wsb);
+  check_rc(d3pm_policy_loss(&v.desc, tokens.data_ptr(), token_bytes(tokens, logits, "tokens"), p.old_lp, p.adv, p.per_seq,
+                            p.ref, mask_ptr(mask, tokens, logits), (float)temperature, (float)clip_low, (float)clip_high,
+                            (float)kl_coeff, (float)out_scale, upstream_ptr(upstream, logits), only_if_rescaled, nullptr,
+                            nullptr, dlogits.data_ptr(), ws.data_ptr(), wsb, stream()));
+}
+
+// (loss [], rewards [B], stats, dlogits): preference loss of the pairs (p, p + B / 2)
+std::tuple<Tensor, Tensor, Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& tokens,
+                                                           const OptTensor& ref_logprobs, const OptTensor& mask,
+                                                           double beta, double label_smoothing, bool average,
+                                                           double out_scale, bool want_grad) {
+  D3PM_GUARD(logits);
+  auto v = logits_view(logits, tokens, "tokens");
+  const float* ref = ref_logprobs.has_value() && ref_logprobs->defined()
+                         ? row_f32(*ref_logprobs, tokens, logits, "ref_logprobs and tokens") : nullptr;
+  auto fo = logits.options().dtype(at::kFloat);
+  Tensor loss = at::empty({}, fo), rewards = at::empty({v.desc.B}, fo), stats = at::empty({tokens.numel(), 4}, fo);
+  Tensor dz = grad_buffer(logits, want_grad);
+  size_t wsb;
+  Tensor ws = objective_workspace(v.desc, logits, &wsb);
+  check_rc(d3pm_preference_loss(&v.desc, tokens.data_ptr(), token_bytes(tokens, logits, "tokens"), ref,
+                                mask_ptr(mask, tokens, logits), (float)beta, (float)label_smoothing, average,
+                                (float)out_scale, loss.data_ptr<float>(), rewards.data_ptr<float>(),
+                                stats.data_ptr<float>(), want_grad ? dz.data_ptr() : nullptr, ws.data_ptr(), wsb, stream()));
+  return {loss, rewards, stats, dz};
+}
+
 }  // namespace
 
 #define D3PM_TB "Tensor[] tables, int K, int T, bool structured, float eps, "
 #define D3PM_PT "Tensor qbar_digest, Tensor qone_digest, Tensor lvb_digest, int K, int T, "
 #define D3PM_LOSS_ARGS "Tensor logits, Tensor x0, Tensor x_t, Tensor t, int loss_type, float hybrid_coeff, float grad_scale, "
+#define D3PM_DISTILL_ARGS "Tensor logits, Tensor teacher_logits, Tensor teacher_index, Tensor? mask, float temperature, " \
+                          "float out_scale, "
+#define D3PM_POLICY_ARGS "Tensor logits, Tensor tokens, Tensor old_logprobs, Tensor advantages, Tensor? ref_logprobs, " \
+                         "Tensor? mask, float temperature, float clip_low, float clip_high, float kl_coeff, float out_scale, "
 
 TORCH_LIBRARY(d3pm_mi355x, m) {
   m.def("q_probs(" D3PM_TB "Tensor x0, Tensor t) -> Tensor");
@@ -650,6 +873,15 @@ TORCH_LIBRARY(d3pm_mi355x, m) {
   m.def("lvb_reverse_step(" D3PM_PT "Tensor pred, Tensor x_t, Tensor t, Tensor? expo, int seed, int offset, "
         "Tensor? offset_dev, float last_class_div, int exclude_last_prefix) -> Tensor");
   m.def("corrupt(" D3PM_PT "Tensor x0, Tensor t, Tensor? expo, int seed, int offset, bool want_probs) -> (Tensor, Tensor)");
+  m.def("token_logprobs(Tensor logits, Tensor tokens, Tensor? mask, float temperature, bool want_stats) -> (Tensor, Tensor)");
+  m.def("token_grad_(Tensor logits, Tensor tokens, float temperature, Tensor stats, Tensor upstream, bool per_row, "
+        "bool only_if_rescaled, Tensor(a!) dlogits) -> ()");
+  m.def("topk_distill_loss(" D3PM_DISTILL_ARGS "bool want_grad) -> (Tensor, Tensor, Tensor)");
+  m.def("topk_distill_grad_(" D3PM_DISTILL_ARGS "Tensor upstream, bool only_if_rescaled, Tensor(a!) dlogits) -> ()");
+  m.def("policy_loss(" D3PM_POLICY_ARGS "bool want_grad) -> (Tensor, Tensor, Tensor)");
+  m.def("policy_grad_(" D3PM_POLICY_ARGS "Tensor upstream, bool only_if_rescaled, Tensor(a!) dlogits) -> ()");
+  m.def("preference_loss(Tensor logits, Tensor tokens, Tensor? ref_logprobs, Tensor? mask, float beta, "
+        "float label_smoothing, bool average, float out_scale, bool want_grad) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(d3pm_mi355x, CUDA, m) {
@@ -680,4 +912,11 @@ TORCH_LIBRARY_IMPL(d3pm_mi355x, CUDA, m) {
   m.impl("lvb_hybrid_loss", lvb_hybrid_loss);
   m.impl("lvb_reverse_step", lvb_reverse_step);
   m.impl("corrupt", corrupt);
+  m.impl("token_logprobs", token_logprobs);
+  m.impl("token_grad_", token_grad_);
+  m.impl("topk_distill_loss", topk_distill_loss);
+  m.impl("topk_distill_grad_", topk_distill_grad_);
+  m.impl("policy_loss", policy_loss);
+  m.impl("policy_grad_", policy_grad_);
+  m.impl("preference_loss", preference_loss);
 }

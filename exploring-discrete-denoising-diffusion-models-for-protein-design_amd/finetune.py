@@ -1,0 +1,243 @@
+"""Fine-tuning objectives at a denoiser's (or a language model's) logits, with the loss modules' manner of the
+package: the gradient at the logits comes out of the launch that computes the loss.
+
+  token_logprobs    log-probabilities of given tokens (the reference and old models' side of the losses below)
+  TopKDistillLoss   distillation from a teacher's top logits
+  PreferenceLoss    pairs of sequences, the first of each preferred: -log sigmoid of the difference of log-ratios
+  PolicyLoss        clipped ratio of new to old probabilities times an advantage, with a KL term
+
+Logits are float32, float16 or bfloat16 ``[..., V]`` on the GPU with any strides; everything is computed in float32
+(sums over rows and sequences in float64) and the gradient is rounded once, to the logits' type.  ``mask`` (bool, the
+tokens' shape) says which positions count: the others' logits and labels are not looked at (they may hold NaN, or
+tokens that are none), their outputs and gradients are 0.  Tokens and classes outside ``[0, V)`` are clamped into it
+(a negative ``teacher_index`` marks an entry that is not there).  Only the logits are differentiated; any other
+floating input that requires a gradient is refused.
+
+``out_scale=`` multiplies a loss and its gradient.  The gradient of the launch is that for an upstream gradient of 1,
+so a constant factor (a loss scaler's, 1 / accumulated batches) costs nothing there, while any other upstream gradient
+makes ``backward`` compute the gradient again."""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._ops import ops
+
+
+def _tokens(x: torch.Tensor) -> torch.Tensor:
+    if x.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"tokens and classes must be int32 or int64, got {x.dtype}")
+    return x.contiguous()
+
+
+def _constant(x: Optional[torch.Tensor], what: str) -> Optional[torch.Tensor]:
+    """A float32 input that the loss is not differentiated by."""
+    if x is None:
+        return None
+    if x.requires_grad:
+        raise ValueError(f"{what} is a constant of this loss and must not require a gradient (detach it)")
+    return x.contiguous() if x.dtype == torch.float32 else x.to(torch.float32).contiguous()
+
+
+def _mask(mask: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    if mask is None:
+        return None
+    if mask.dtype != torch.bool:
+        raise TypeError(f"mask must be bool, got {mask.dtype}")
+    return mask.contiguous()
+
+
+def _temperature(x: float) -> float:
+    x = float(x)
+    if not 1e-6 <= x <= 1e6:
+        raise ValueError(f"temperature must be in [1e-6, 1e6], got {x}")
+    return x
+
+
+def _finite(x: float, what: str) -> float:
+    x = float(x)
+    if not math.isfinite(x):
+        raise ValueError(f"{what} must be finite, got {x}")
+    return x
+
+
+def _hand_over(ctx, fill):
+    """The gradient buffer of the forward launch, with `fill(buffer, only_if_rescaled)` run on it; a second backward
+    (retain_graph) gets a buffer of its own."""
+    logits = ctx.saved_tensors[0]
+    dz, ctx.dz = ctx.dz, None
+    again = dz is None
+    if again:
+        dz = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    fill(dz, not again)
+    return dz
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, mask, temperature):
+        lp, stats = ops.token_logprobs(logits, tokens, mask, temperature, ctx.needs_input_grad[0])
+        ctx.save_for_backward(logits, tokens, stats)
+        ctx.temperature = temperature
+        return lp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        logits, tokens, stats = ctx.saved_tensors
+        dz = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        ops.token_grad_(logits, tokens, ctx.temperature, stats, g.contiguous(), True, False, dz)
+        return dz, None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, mask: Optional[torch.Tensor] = None,
+                   temperature: float = 1.0) -> torch.Tensor:
+    """``log_softmax(logits / temperature)`` at ``tokens`` (logits ``[..., V]``, tokens ``[...]``), float32 of the
+    tokens' shape, 0 where ``mask`` is false; differentiable by the logits."""
+    _lib.require_device(logits, tokens, mask)
+    tokens, mask, temperature = _tokens(tokens), _mask(mask), _temperature(temperature)
+    if not (torch.is_grad_enabled() and logits.requires_grad):
+        return ops.token_logprobs(logits, tokens, mask, temperature, False)[0]
+    return _TokenLogprobs.apply(logits, tokens, mask, temperature)
+
+
+class _Distill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher_logits, teacher_index, mask, temperature, out_scale):
+        loss, per, dz = ops.topk_distill_loss(logits, teacher_logits, teacher_index, mask, temperature, out_scale,
+                                              ctx.needs_input_grad[0])
+        ctx.save_for_backward(logits, teacher_logits, teacher_index, mask)
+        ctx.dz, ctx.args = dz, (temperature, out_scale)
+        ctx.mark_non_differentiable(per)
+        return loss, per
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _per):
+        saved = ctx.saved_tensors
+        return (_hand_over(ctx, lambda dz, only: ops.topk_distill_grad_(*saved, *ctx.args, g, only, dz)),) + (None,) * 5
+
+
+class TopKDistillLoss(torch.nn.Module):
+    """Distillation from the ``k`` best logits that a teacher gave per position.
+
+    With ``q = softmax(teacher_logits / temperature)`` over the kept entries of a position (those with an index of at
+    least 0 and a logit above -inf), ``forward`` returns the mean over the counted positions of
+    ``temperature**2 * KL(q || softmax(logits / temperature))``, times ``out_scale``.  logits ``[..., V]``,
+    teacher_logits and teacher_index ``[..., k]`` with k up to 256; a class listed twice has the sum of its entries,
+    a position that keeps none adds 0.  ``per_token`` holds the positions' terms of the last call."""
+
+    def __init__(self, temperature: float = 1.0):
+        super().__init__()
+        self.temperature = _temperature(temperature)
+        self.per_token = None
+
+    def forward(self, logits, teacher_logits, teacher_index, mask=None, out_scale=1.0):
+        _lib.require_device(logits, teacher_logits, teacher_index, mask)
+        if teacher_logits.requires_grad:
+            raise ValueError("teacher_logits is a constant of this loss and must not require a gradient (detach it)")
+        args = (teacher_logits.contiguous(), _tokens(teacher_index), _mask(mask), self.temperature,
+                _finite(out_scale, "out_scale"))
+        if torch.is_grad_enabled() and logits.requires_grad:
+            loss, self.per_token = _Distill.apply(logits, *args)
+        else:
+            loss, self.per_token, _ = ops.topk_distill_loss(logits, *args, False)
+        return loss
+
+
+class _Policy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, old, adv, ref, mask, *args):
+        loss, lp, dz = ops.policy_loss(logits, tokens, old, adv, ref, mask, *args, ctx.needs_input_grad[0])
+        ctx.save_for_backward(logits, tokens, old, adv, ref, mask)
+        ctx.dz, ctx.args = dz, args
+        ctx.mark_non_differentiable(lp)
+        return loss, lp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _lp):
+        saved = ctx.saved_tensors
+        return (_hand_over(ctx, lambda dz, only: ops.policy_grad_(*saved, *ctx.args, g, only, dz)),) + (None,) * 10
+
+
+class PolicyLoss(torch.nn.Module):
+    """Clipped policy loss with a KL term.
+
+    With ``lp`` the tokens' log-probabilities at ``temperature``, ``r = exp(lp - old_logprobs)`` and
+    ``x = ref_logprobs - lp``, ``forward`` returns the mean over the counted positions of
+    ``-min(r * A, clip(r, 1 - clip_low, 1 + clip_high) * A) + kl_coeff * (exp(x) - x - 1)``, times ``out_scale``.
+    logits ``[..., V]``; tokens, old_logprobs, ref_logprobs ``[...]``; advantages ``[...]``, or ``[B]`` for one per
+    sequence of tokens ``[B, L]``.  ``logprobs`` holds ``lp`` of the last call (0 where a position is not counted)."""
+
+    def __init__(self, clip_low: float = 0.2, clip_high: float = 0.2, kl_coeff: float = 0.0, temperature: float = 1.0):
+        super().__init__()
+        self.clip_low, self.clip_high = _finite(clip_low, "clip_low"), float(clip_high)
+        if not (0.0 <= self.clip_low <= 1.0 and self.clip_high >= 0.0):
+            raise ValueError(f"clip range [1 - {clip_low}, 1 + {clip_high}]: need 0 <= clip_low <= 1, clip_high >= 0")
+        self.kl_coeff = _finite(kl_coeff, "kl_coeff")
+        self.temperature = _temperature(temperature)
+        self.logprobs = None
+
+    def forward(self, logits, tokens, old_logprobs, advantages, ref_logprobs=None, mask=None, out_scale=1.0):
+        _lib.require_device(logits, tokens, old_logprobs, advantages, ref_logprobs, mask)
+        if self.kl_coeff != 0.0 and ref_logprobs is None:
+            raise ValueError("kl_coeff needs ref_logprobs")
+        args = (_tokens(tokens), _constant(old_logprobs, "old_logprobs"), _constant(advantages, "advantages"),
+                _constant(ref_logprobs, "ref_logprobs"), _mask(mask), self.temperature, self.clip_low, self.clip_high,
+                self.kl_coeff, _finite(out_scale, "out_scale"))
+        if torch.is_grad_enabled() and logits.requires_grad:
+            loss, self.logprobs = _Policy.apply(logits, *args)
+        else:
+            loss, self.logprobs, _ = ops.policy_loss(logits, *args, False)
+        return loss
+
+
+class _Preference(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, ref, mask, *args):
+        loss, rewards, stats, dz = ops.preference_loss(logits, tokens, ref, mask, *args, ctx.needs_input_grad[0])
+        ctx.save_for_backward(logits, tokens, stats)
+        ctx.dz = dz
+        ctx.mark_non_differentiable(rewards)
+        return loss, rewards
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _rewards):
+        logits, tokens, stats = ctx.saved_tensors
+        return (_hand_over(ctx, lambda dz, only: ops.token_grad_(logits, tokens, 1.0, stats, g, False, only, dz)),) + \
+            (None,) * 7
+
+
+class PreferenceLoss(torch.nn.Module):
+    """Preference loss of pairs of sequences.
+
+    logits ``[2 P, L, V]`` and tokens ``[2 P, L]`` hold the P preferred sequences first, then in the same order the
+    ones that they are preferred to; ref_logprobs ``[2 P, L]`` are the tokens' log-probabilities under the reference
+    model (``token_logprobs``; None: 0).  With ``D`` a sequence's sum of ``lp - ref_logprobs`` over its counted
+    positions (their mean with ``average``) and ``m = beta * (D_preferred - D_other)``, ``forward`` returns the mean
+    over the pairs of ``-(1 - label_smoothing) * log sigmoid(m) - label_smoothing * log sigmoid(-m)``, times
+    ``out_scale``.  ``rewards`` holds ``beta * D`` ``[2 P]`` of the last call."""
+
+    def __init__(self, beta: float = 0.1, label_smoothing: float = 0.0, average: bool = False):
+        super().__init__()
+        self.beta, self.label_smoothing = _finite(beta, "beta"), _finite(label_smoothing, "label_smoothing")
+        if not 0.0 <= self.label_smoothing <= 1.0:
+            raise ValueError(f"label_smoothing must be in [0, 1], got {label_smoothing}")
+        self.average = bool(average)
+        self.rewards = None
+
+    def forward(self, logits, tokens, ref_logprobs=None, mask=None, out_scale=1.0):
+        _lib.require_device(logits, tokens, ref_logprobs, mask)
+        args = (_tokens(tokens), _constant(ref_logprobs, "ref_logprobs"), _mask(mask), self.beta, self.label_smoothing,
+                self.average, _finite(out_scale, "out_scale"))
+        if torch.is_grad_enabled() and logits.requires_grad:
+            loss, self.rewards = _Preference.apply(logits, *args)
+        else:
+            loss, self.rewards = ops.preference_loss(logits, *args, False)[:2]
+        return loss

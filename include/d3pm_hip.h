@@ -386,6 +386,96 @@ int d3pm_lvb_reverse_step(const d3pm_tables_f64* tb, const float* pred, long ld,
                           uint64_t offset, const uint64_t* offset_dev, double last_class_div,
                           long exclude_last_prefix, int64_t* out, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Fine-tuning objectives (no counterpart in the reference): losses at the
+ * logits of a denoiser or a language model and their gradient there, for a
+ * model that is distilled or tuned to preferences or rewards after its
+ * training.  All arithmetic in float32, sums over rows and sequences in
+ * float64; results are repeatable bit for bit.
+ *
+ * mask uint8 [B,L], 0 where a position is not counted (NULL: every position
+ * is): its logits row and its entries of the other inputs are not looked at,
+ * its outputs are 0.  Tokens are clamped to [0, V-1] as everywhere in this
+ * header.  A row whose logits hold a NaN or +inf, or nothing but -inf, gives
+ * NaN where it is counted.  Gradients go to dlogits [B,L,V], contiguous, of
+ * the logits' type, rounded once to nearest.
+ * --------------------------------------------------------------------- */
+#define D3PM_F32  0
+#define D3PM_F16  1
+#define D3PM_BF16 2
+
+/* Logits [B,L,V]: element (b,l,v) lies at b*stride_b + l*stride_l + v. */
+typedef struct d3pm_logits {
+  const void* data;          /* aligned to its elements */
+  int dtype, V;              /* 1 <= V <= 2^27          */
+  long B, L;                 /* B*L < 2^31 - 65536      */
+  long stride_b, stride_l;   /* in elements, >= 0       */
+} d3pm_logits;
+
+/* Workspace (bytes) of the three losses below for B sequences of L positions.
+ * Contents irrelevant; each call in flight needs its own. */
+size_t d3pm_objective_workspace(long B, long L);
+
+/* logprobs[b,l] = log_softmax(z[b,l,:] / temperature)[tokens[b,l]], float32
+ * [B,L].  row_stats (may be NULL) float32 [B,L,4], 16-byte aligned: what
+ * d3pm_token_grad takes. */
+int d3pm_token_logprobs(const d3pm_logits* z, const void* tokens, int tok_bytes, const uint8_t* mask,
+                        float temperature, float* logprobs, float* row_stats, void* stream);
+
+/* Gradient of d3pm_token_logprobs (upstream float32 [B,L], upstream_per_row
+ * != 0) or of d3pm_preference_loss (one upstream float32, upstream_per_row ==
+ * 0, temperature 1; NULL: 1) from the row_stats that they left.
+ * only_if_rescaled: dlogits holds the gradient for an upstream of 1 already,
+ * as the loss call wrote it, and is left alone if *upstream is 1. */
+int d3pm_token_grad(const d3pm_logits* z, const void* tokens, int tok_bytes, float temperature,
+                    const float* row_stats, const float* upstream, int upstream_per_row, int only_if_rescaled,
+                    void* dlogits, void* stream);
+
+/* Distillation from a teacher's top logits.  q = softmax(teacher / temperature)
+ * over the row's kept entries, those with an index >= 0 and a logit above -inf
+ * (an index beyond V-1 counts as V-1; a class listed twice has the sum of its
+ * entries; a row that keeps none adds nothing):
+ *   loss = out_scale / max(counted positions, 1)
+ *          * sum temperature^2 KL(q || softmax(z / temperature))
+ *   teacher_logits [B,L,k] of teacher_dtype, teacher_index int32 / int64
+ *   [B,L,k], 1 <= k <= 256
+ *   per_token float32 [B,L]: temperature^2 KL (may be NULL)
+ *   dlogits may be NULL (no gradient).  upstream (may be NULL) multiplies the
+ *   gradient; loss == NULL: the call makes the gradient alone, and with
+ *   only_if_rescaled leaves dlogits as it is if *upstream is 1. */
+int d3pm_topk_distill_loss(const d3pm_logits* z, const void* teacher_logits, int teacher_dtype,
+                           const void* teacher_index, int index_bytes, int k, const uint8_t* mask, float temperature,
+                           float out_scale, const float* upstream, int only_if_rescaled, float* loss, float* per_token,
+                           void* dlogits, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Clipped policy loss with a KL term.  With lp the token's log-probability at
+ * `temperature`, r = exp(lp - old_logprobs), A the advantage, x = ref - lp:
+ *   loss = out_scale / max(counted positions, 1)
+ *          * sum -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+ *                + kl_coeff (exp(x) - x - 1)
+ *   advantages float32 [B,L], or [B] with advantages_per_sequence;
+ *   ref_logprobs may be NULL where kl_coeff is 0
+ *   logprobs float32 [B,L]: lp (may be NULL)
+ * upstream, only_if_rescaled, loss, dlogits as for d3pm_topk_distill_loss. */
+int d3pm_policy_loss(const d3pm_logits* z, const void* tokens, int tok_bytes, const float* old_logprobs,
+                     const float* advantages, int advantages_per_sequence, const float* ref_logprobs,
+                     const uint8_t* mask, float temperature, float clip_low, float clip_high, float kl_coeff,
+                     float out_scale, const float* upstream, int only_if_rescaled, float* loss, float* logprobs,
+                     void* dlogits, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Preference loss of B/2 pairs: sequence p < B/2 is preferred to p + B/2.
+ * D_b = sum over the counted positions of lp - ref_logprobs (float32 [B,L],
+ * NULL: 0), divided by their number with `average`; m = beta (D_p - D_{p+B/2}):
+ *   loss = out_scale / (B/2) * sum -(1 - label_smoothing) log sigmoid(m)
+ *                                  - label_smoothing log sigmoid(-m)
+ *   rewards float32 [B]: beta D_b
+ *   row_stats float32 [B,L,4], 16-byte aligned: written here, for
+ *   d3pm_token_grad; dlogits may be NULL. */
+int d3pm_preference_loss(const d3pm_logits* z, const void* tokens, int tok_bytes, const float* ref_logprobs,
+                         const uint8_t* mask, float beta, float label_smoothing, int average, float out_scale,
+                         float* loss, float* rewards, float* row_stats, void* dlogits, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
