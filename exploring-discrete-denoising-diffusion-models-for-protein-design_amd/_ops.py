@@ -25,7 +25,7 @@ OP_NAMES = ("q_probs", "q_sample", "q_sample_draw_t", "q_posterior_logits", "q_p
             "hybrid_loss_step", "hybrid_loss_then_q_sample", "hybrid_loss_static_", "scale_rows_", "p_sample", "prior_bpd",
             "logistic_logits", "logistic_logits_backward", "build_tables", "protein_uniform_tables", "cumprod",
             "digest_f32", "digest_f64", "table_to_f32", "table_split_f16x2", "table_fingerprints", "lvb_digest", "lvb_loss", "lvb_hybrid_loss", "lvb_reverse_step", "corrupt",
-            "token_logprobs", "token_grad_", "topk_distill_loss", "topk_distill_grad_", "policy_loss", "policy_grad_", "preference_loss")
+            "token_logprobs", "topk_distill_loss", "policy_loss", "preference_loss")
 
 
 def i64(x: int) -> int:

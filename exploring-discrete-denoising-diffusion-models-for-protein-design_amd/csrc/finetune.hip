@@ -115,6 +115,13 @@ __device__ __forceinline__ int get_int(const void* p, int bytes, long i) {
   return v < 0 ? -1 : v > INT_MAX ? INT_MAX : (int)v;
 }
 
+// A piece of a gradient row: nothing in the launch reads it again, and the caches are better kept for the logits
+// (2 % of a launch at 32 k classes and more).
+template <typename T>
+__device__ __forceinline__ void store_piece(char* p, u32x4 v) {
+  __builtin_nontemporal_store((typename T::Raw)v, (typename T::Raw*)p);
+}
+
 // ------------------------------------------------------------------------------------------------------ arguments
 struct RowArgs {
   const void* z; long sb, sl; int L, V, N; int dense;         // dense: row n lies at n * sl
@@ -143,8 +150,25 @@ __device__ __forceinline__ const char* row_ptr(const RowArgs& a, int n, int size
 // way (1e-7 at d = -10), which the sum over a sequence of a preference loss would gather up.
 __device__ __forceinline__ float exp_d(float d, float c_hi, float c_lo) { return exp2_hw(fmaf(d, c_hi, d * c_lo)); }
 
+__device__ __forceinline__ float rcp_acc(float x) {      // v_rcp_f32 and one step of Newton's: 1 ulp
+  const float r = __builtin_amdgcn_rcpf(x);
+  return fmaf(fmaf(-x, r, 1.0f), r, r);
+}
+// exp(x): log2(e) in two floats (the second above 0: an infinite x stays what it is)
+__device__ __forceinline__ float exp_any(float x) { return exp2_hw(fmaf(x, 1.44269502f, x * 1.92596299e-8f)); }
+// exp(x) - 1 - x: near 0 its series (up to 0.35 the next term is 9e-8 of it), where the difference would cancel
+__device__ __forceinline__ float exp_rest(float x) {
+  float q = fmaf(x, 1.0f / 5040.0f, 1.0f / 720.0f);
+  q = fmaf(x, q, 1.0f / 120.0f);
+  q = fmaf(x, q, 1.0f / 24.0f);
+  q = fmaf(x, q, 1.0f / 6.0f);
+  q = fmaf(x, q, 0.5f);
+  return fabsf(x) < 0.35f ? x * x * q : exp_any(x) - 1.0f - x;
+}
+
 // What a row's token gives once m and S are known: its log-probability, its share of the loss and the coefficient
-// c of its gradient (without the weight).  Comparisons are written so that a NaN stays one.
+// c of its gradient (without the weight).  Comparisons are written so that a NaN stays one.  Every lane of the row
+// computes this: at 32 classes its instructions are most of the launch, hence the short forms above.
 struct TokenOut { float lp, loss, c; };
 __device__ __forceinline__ TokenOut token_head(const RowArgs& a, int n, float zy_m, float S) {
   TokenOut o;
@@ -153,19 +177,23 @@ __device__ __forceinline__ TokenOut token_head(const RowArgs& a, int n, float zy
   o.c = 1.0f;
   if (a.head == HEAD_POLICY) {
     const float A = a.adv[a.adv_per_seq ? (unsigned)n / (unsigned)a.L : (unsigned)n];
-    const float r = expf(o.lp - a.old_lp[n]);
+    const float r = exp_any(o.lp - a.old_lp[n]);
     const float held_r = r < a.clip_lo ? a.clip_lo : r > a.clip_hi ? a.clip_hi : r;
     const float free_s = r * A, held_s = held_r * A;
     const bool clipped = free_s > held_s;
     o.loss = clipped ? -held_s : -free_s;
     o.c = clipped ? 0.0f : -free_s;
     if (a.ref_lp) {
-      const float x = a.ref_lp[n] - o.lp, e = expm1f(x);
-      o.loss = fmaf(a.kl_coeff, e - x, o.loss);
-      o.c = fmaf(-a.kl_coeff, e, o.c);
+      const float x = a.ref_lp[n] - o.lp, q = exp_rest(x);
+      o.loss = fmaf(a.kl_coeff, q, o.loss);
+      o.c = fmaf(-a.kl_coeff, x + q, o.c);
     }
   }
   return o;
+}
+// c (1 - p) of the token: S less its own exponential is exact where that is the row's largest
+__device__ __forceinline__ float token_grad(float c, float zy_m, float S, float inv_S, float c_hi, float c_lo) {
+  return c * (S - exp_d(zy_m, c_hi, c_lo)) * inv_S;
 }
 
 // ------------------------------------------------------------------------------------- one pass, rows in registers
@@ -179,10 +207,38 @@ struct Shape {
   static constexpr int GL = G < 64 ? G : 64;        // lanes that a teacher's list is spread over
 };
 
+// How a row falls into 16-byte pieces and the elements at its ends that fill none.  Rows of odd widths start anywhere;
+// with PEEL their pieces begin at the first 16-byte boundary (a piece across two cache lines costs two accesses).
+// Lane g of the row has the end element `edge(g)`, if there is one.
+template <typename T, bool PEEL>
+struct Cut {
+  int head, full, rest, V;
+  __device__ __forceinline__ Cut(const char* row, int V_) : V(V_) {
+    head = PEEL ? min((int)((-(uintptr_t)row & 15) / T::SIZE), V) : 0;
+    full = (V - head) / T::E;
+    rest = V - head - full * T::E;
+  }
+  __device__ __forceinline__ bool has_edge(int g) const { return g < head + rest; }
+  __device__ __forceinline__ int edge(int g) const { return g < head ? g : g + full * T::E; }
+  // the lane of G that holds class y
+  __device__ __forceinline__ int lane_of(int y, int G) const {
+    const int in = y - head;
+    return in < 0 ? y : in < full * T::E ? (in / T::E) % G : y - full * T::E;
+  }
+};
+
+// Keeps the compiler from carrying the unpacked values of one sweep over a row into the next: they take twice the
+// registers of the 16-bit pieces that they are unpacked from (220 instead of 64 + 36 at 16 pieces a lane).
+template <int NV>
+__device__ __forceinline__ void fresh(u32x4 (&v)[NV]) {
+#pragma unroll
+  for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(v[j]));
+}
+
 // m and S of the group's row from its lanes' values: a wave takes its exponentials against its own maximum, so a
 // row of several waves needs one exchange, not two.  The reference is kept off -inf (a wave that has only padding).
 template <typename T, int G, int NV>
-__device__ __forceinline__ void row_stats(const u32x4 (&v)[NV], float edge, const RowArgs& a, float2* red, int wave,
+__device__ __forceinline__ void row_stats(u32x4 (&v)[NV], float edge, const RowArgs& a, float2* red, int wave,
                                           float& m, float& S) {
   constexpr int GL = Shape<G>::GL;
   float f[T::E];
@@ -194,6 +250,7 @@ __device__ __forceinline__ void row_stats(const u32x4 (&v)[NV], float edge, cons
     for (int e = 0; e < T::E; ++e) mx = fmaxf(mx, f[e]);
   }
   mx = fmaxf(group_max<GL>(mx), -FLT_MAX);
+  fresh<NV>(v);
   float s0 = exp_d(edge - mx, a.c_hi, a.c_lo), s1 = 0.0f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
@@ -204,6 +261,7 @@ __device__ __forceinline__ void row_stats(const u32x4 (&v)[NV], float edge, cons
       s1 += exp_d(f[e + 1] - mx, a.c_hi, a.c_lo);
     }
   }
+  fresh<NV>(v);
   const float s = group_sum<GL>(s0 + s1);
   if constexpr (G <= 64) {
     m = mx;
@@ -283,36 +341,39 @@ __device__ __forceinline__ void list_grad(const RowArgs& a, const char* row, cha
 }
 
 // the gradient row of a position that is not counted
-template <typename T, int G>
-__device__ __forceinline__ void zero_row(char* out, int g, int full, int rest) {
+template <typename T, bool PEEL>
+__device__ __forceinline__ void zero_row(char* out, int V, int g, int G) {
+  const Cut<T, PEEL> cut(out, V);
   const u32x4 zero = {0, 0, 0, 0};
-  for (int j = g; j < full; j += G) *(typename T::Raw*)(out + (long)j * 16) = zero;
-  if (g < rest) T::put(out, (long)full * T::E + g, 0.0f);
+  char* body = out + cut.head * T::SIZE;
+  for (int j = g; j < cut.full; j += G) *(typename T::Raw*)(body + (uint32_t)j * 16u) = zero;
+  if (cut.has_edge(g)) T::put(out, cut.edge(g), 0.0f);
 }
 
 template <typename T, int G, int NV, bool DISTILL>
 __global__ __launch_bounds__(Shape<G>::WG) void k_rows(RowArgs a) {
   typedef Shape<G> Sh;
   constexpr int E = T::E;
+  constexpr bool PEEL = G >= 64;       // (a row of fewer lanes has no lane for every end element)
   __shared__ float2 red[2][G > 64 ? G / 64 : 1];
   __shared__ int kept_flag[2];
   __shared__ double wg_sum[Sh::ROWS];
   extern __shared__ char lists[];
   if (a.only_if_rescaled && *a.upstream == 1.0f) return;
 
-  const int g = threadIdx.x % G, slot = threadIdx.x / G, wave = threadIdx.x >> 6;
-  const int full = a.V / E, rest = a.V - full * E;
+  const int g = threadIdx.x % G, slot = Sh::ROWS == 1 ? 0 : threadIdx.x / G, wave = threadIdx.x >> 6;
   float w = a.weight * (a.count ? 1.0f / (float)max(*a.count, 1) : a.inv_count);
   if (a.upstream) w *= *a.upstream;
   double acc = 0.0;
   int phase = 0;
 
   for (int n0 = blockIdx.x * Sh::ROWS; n0 < a.N; n0 += gridDim.x * Sh::ROWS) {
-    const int n = n0 + slot;
+    int n = n0 + slot;
     if (Sh::ROWS > 1 && n >= a.N) break;
+    if constexpr (G == 64) n = __builtin_amdgcn_readfirstlane(n);        // the row of a whole wave: scalar addresses
     char* out = a.dz ? (char*)a.dz + (long)n * a.V * T::SIZE : nullptr;
     if (a.mask && !a.mask[n]) {                      // not counted: nothing of its row is read
-      if (out) zero_row<T, G>(out, g, full, rest);
+      if (out) zero_row<T, PEEL>(out, a.V, g, G);
       if (g == 0) {
         if (a.per_row) a.per_row[n] = 0.0f;
         if (a.stats) a.stats[n] = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
@@ -320,14 +381,16 @@ __global__ __launch_bounds__(Shape<G>::WG) void k_rows(RowArgs a) {
       continue;
     }
     const char* row = row_ptr(a, n, T::SIZE);
+    const Cut<T, PEEL> cut(row, a.V);
+    const char* body = row + cut.head * T::SIZE;
+    char* obody = out + cut.head * T::SIZE;
     u32x4 v[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int at = j * G + g;
       v[j] = (u32x4){T::NEG_INF, T::NEG_INF, T::NEG_INF, T::NEG_INF};
-      if (at < full) v[j] = *(const typename T::Raw*)(row + (long)at * 16);
+      if (j * G + g < cut.full) v[j] = *(const typename T::Raw*)(body + j * (G * 16) + (uint32_t)g * 16u);
     }
-    const float edge = g < rest ? T::get(row, full * E + g) : -INFINITY;
+    const float edge = cut.has_edge(g) ? T::get(row, cut.edge(g)) : -INFINITY;
     float m, S;
 
     if constexpr (!DISTILL) {
@@ -341,19 +404,18 @@ __global__ __launch_bounds__(Shape<G>::WG) void k_rows(RowArgs a) {
         acc += (double)o.loss;
       }
       if (out) {
-        const float c = w * o.c, scale = -c / S;
+        const float c = w * o.c, inv_S = rcp_acc(S), scale = -c * inv_S;
         float f[E];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          const int at = j * G + g;
           T::unpack(v[j], f);
 #pragma unroll
           for (int e = 0; e < E; ++e) f[e] = scale * exp_d(f[e] - m, a.c_hi, a.c_lo);
-          if (at < full) *(typename T::Raw*)(out + (long)at * 16) = T::pack(f);
+          if (j * G + g < cut.full) store_piece<T>(obody + j * (G * 16) + (uint32_t)g * 16u, T::pack(f));
         }
-        if (g < rest) T::put(out, full * E + g, scale * exp_d(edge - m, a.c_hi, a.c_lo));
+        if (cut.has_edge(g)) T::put(out, cut.edge(g), scale * exp_d(edge - m, a.c_hi, a.c_lo));
         // the token's own element, c (1 - p), by the lane that wrote its place above
-        if (g == (y < full * E ? (y / E) % G : y - full * E)) T::put(out, y, -c * expm1f(o.lp));
+        if (g == cut.lane_of(y, G)) T::put(out, y, token_grad(c, zy - m, S, inv_S, a.c_hi, a.c_lo));
       }
     } else {
       List l;
@@ -374,21 +436,20 @@ __global__ __launch_bounds__(Shape<G>::WG) void k_rows(RowArgs a) {
         }
       }
       if (out) {
-        const float c = kept ? -w : 0.0f, scale = kept ? w / S : 0.0f;
+        const float inv_S = rcp_acc(S), c = kept ? -w : 0.0f, scale = kept ? w * inv_S : 0.0f;
         float f[E];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          const int at = j * G + g;
           T::unpack(v[j], f);
 #pragma unroll
           for (int e = 0; e < E; ++e) f[e] = scale * exp_d(f[e] - m, a.c_hi, a.c_lo);
-          if (at < full) *(typename T::Raw*)(out + (long)at * 16) = T::pack(f);
+          if (j * G + g < cut.full) store_piece<T>(obody + j * (G * 16) + (uint32_t)g * 16u, T::pack(f));
         }
-        if (g < rest) T::put(out, full * E + g, scale * exp_d(edge - m, a.c_hi, a.c_lo));
+        if (cut.has_edge(g)) T::put(out, cut.edge(g), scale * exp_d(edge - m, a.c_hi, a.c_lo));
         // the listed classes' elements go over what the pieces' lanes have just written
         if constexpr (G > 64) __syncthreads();
         else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (lister && kept) list_grad<T, Sh::GL>(a, row, out, g, l, m, 1.0f / S, c);
+        if (lister && kept) list_grad<T, Sh::GL>(a, row, out, g, l, m, inv_S, c);
       }
     }
     phase ^= 1;
@@ -414,7 +475,6 @@ __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
   extern __shared__ char lists[];
   if (a.only_if_rescaled && *a.upstream == 1.0f) return;
   const int g = threadIdx.x, wave = threadIdx.x >> 6;
-  const int full = a.V / E, rest = a.V - full * E;
   float w = a.weight * (a.count ? 1.0f / (float)max(*a.count, 1) : a.inv_count);
   if (a.upstream) w *= *a.upstream;
   double acc = 0.0;
@@ -422,7 +482,7 @@ __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
   for (int n = blockIdx.x; n < a.N; n += gridDim.x) {
     char* out = a.dz ? (char*)a.dz + (long)n * a.V * T::SIZE : nullptr;
     if (a.mask && !a.mask[n]) {
-      if (out) zero_row<T, WIDE>(out, g, full, rest);
+      if (out) zero_row<T, true>(out, a.V, g, WIDE);
       if (g == 0) {
         if (a.per_row) a.per_row[n] = 0.0f;
         if (a.stats) a.stats[n] = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
@@ -430,22 +490,36 @@ __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
       continue;
     }
     const char* row = row_ptr(a, n, T::SIZE);
-    const float edge = g < rest ? T::get(row, full * E + g) : -INFINITY;
+    const Cut<T, true> cut(row, a.V);
+    const char* body = row + cut.head * T::SIZE;
+    char* obody = out + cut.head * T::SIZE;
+    const float edge = cut.has_edge(g) ? T::get(row, cut.edge(g)) : -INFINITY;
     // the lane's running maximum and sum
     float mx = fmaxf(edge, -FLT_MAX);
     float s = exp_d(edge - mx, a.c_hi, a.c_lo);
     float f[E];
-    for (int j = g; j < full; j += WIDE) {
-      T::unpack(*(const typename T::Raw*)(row + (long)j * 16), f);
-      float top = f[0];
+    for (int j = g; j < cut.full; j += 4 * WIDE) {       // four pieces on their way at a time
+      u32x4 v[4];
 #pragma unroll
-      for (int e = 1; e < E; ++e) top = fmaxf(top, f[e]);
-      if (top > mx) {
-        s *= exp_d(mx - top, a.c_hi, a.c_lo);
-        mx = top;
+      for (int u = 0; u < 4; ++u) {
+        v[u] = (u32x4){T::NEG_INF, T::NEG_INF, T::NEG_INF, T::NEG_INF};
+        if (j + u * WIDE < cut.full) v[u] = *(const typename T::Raw*)(body + u * (WIDE * 16) + (uint32_t)j * 16u);
       }
+      float top = mx;
 #pragma unroll
-      for (int e = 0; e < E; ++e) s += exp_d(f[e] - mx, a.c_hi, a.c_lo);
+      for (int u = 0; u < 4; ++u) {
+        T::unpack(v[u], f);
+#pragma unroll
+        for (int e = 0; e < E; ++e) top = fmaxf(top, f[e]);
+      }
+      s *= exp_d(mx - top, a.c_hi, a.c_lo);
+      mx = top;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        T::unpack(v[u], f);
+#pragma unroll
+        for (int e = 0; e < E; ++e) s += exp_d(f[e] - mx, a.c_hi, a.c_lo);
+      }
     }
     int y = 0;
     float zy = 0.0f;
@@ -471,7 +545,8 @@ __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
     for (int i = 0; i < WIDE / 64; ++i) sum += (double)(red[phase][i].y * exp_d(red[phase][i].x - m, a.c_hi, a.c_lo));
     const float S = (float)sum;
 
-    float c, scale, lp = 0.0f;
+    float c, scale;
+    const float inv_S = rcp_acc(S);
     int kept = 1;
     if constexpr (!DISTILL) {
       const TokenOut o = token_head(a, n, zy - m, S);
@@ -480,9 +555,8 @@ __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
         if (a.stats) a.stats[n] = make_float4(m, S, a.head == HEAD_LOGPROB ? a.inv_tau : 0.0f, zy - m);
         acc += (double)o.loss;
       }
-      lp = o.lp;
       c = w * o.c;
-      scale = -c / S;
+      scale = -c * inv_S;
     } else {
       kept = kept_flag[phase];
       if (wave == 0) {
@@ -493,21 +567,22 @@ __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
         }
       }
       c = kept ? -w : 0.0f;
-      scale = kept ? w / S : 0.0f;
+      scale = kept ? w * inv_S : 0.0f;
     }
     if (out) {
-      for (int j = g; j < full; j += WIDE) {
-        T::unpack(*(const typename T::Raw*)(row + (long)j * 16), f);
+#pragma unroll 4
+      for (int j = g; j < cut.full; j += WIDE) {
+        T::unpack(*(const typename T::Raw*)(body + (uint32_t)j * 16u), f);
 #pragma unroll
         for (int e = 0; e < E; ++e) f[e] = scale * exp_d(f[e] - m, a.c_hi, a.c_lo);
-        *(typename T::Raw*)(out + (long)j * 16) = T::pack(f);
+        store_piece<T>(obody + (uint32_t)j * 16u, T::pack(f));
       }
-      if (g < rest) T::put(out, full * E + g, scale * exp_d(edge - m, a.c_hi, a.c_lo));
+      if (cut.has_edge(g)) T::put(out, cut.edge(g), scale * exp_d(edge - m, a.c_hi, a.c_lo));
       if constexpr (!DISTILL) {
-        if (g == (y < full * E ? (y / E) % WIDE : y - full * E)) T::put(out, y, -c * expm1f(lp));
+        if (g == cut.lane_of(y, WIDE)) T::put(out, y, token_grad(c, zy - m, S, inv_S, a.c_hi, a.c_lo));
       } else {
         __syncthreads();
-        if (wave == 0 && kept) list_grad<T, 64>(a, row, out, g, l, m, 1.0f / S, c);
+        if (wave == 0 && kept) list_grad<T, 64>(a, row, out, g, l, m, inv_S, c);
       }
     }
     phase ^= 1;
@@ -527,25 +602,26 @@ struct GradArgs {
   void* dz;
 };
 constexpr int GRAD_WG = 256;
-template <typename T>
+template <typename T, bool PEEL>
 __global__ __launch_bounds__(GRAD_WG) void k_token_grad(GradArgs a) {
   constexpr int E = T::E;
   if (a.only_if_rescaled && *a.upstream == 1.0f) return;
   const int g = threadIdx.x & (a.lanes - 1), slot = threadIdx.x / a.lanes, groups = GRAD_WG / a.lanes;
-  const int full = a.V / E, rest = a.V - full * E;
   const long jobs = (long)a.N * a.chunks;
   for (long job = (long)blockIdx.x * groups + slot; job < jobs; job += (long)gridDim.x * groups) {
     const int n = a.chunks == 1 ? (int)job : (int)(job / a.chunks);
     const int part = a.chunks == 1 ? 0 : (int)(job - (long)n * a.chunks);
-    const int lo = part * a.chunk, hi = min(full, lo + a.chunk);
     const bool last = part == a.chunks - 1;
     const float4 st = a.stats[n];
     const float c = st.z * (a.upstream ? a.upstream[(long)n * a.u_stride] : 1.0f);
     char* out = (char*)a.dz + (long)n * a.V * T::SIZE;
     if (c == 0.0f) {                                  // a row that is not counted, or whose upstream gradient is 0
+      const Cut<T, PEEL> cut(out, a.V);
       const u32x4 zero = {0, 0, 0, 0};
-      for (int j = lo + g; j < hi; j += a.lanes) *(typename T::Raw*)(out + (long)j * 16) = zero;
-      if (last && g < rest) T::put(out, full * E + g, 0.0f);
+      char* obody = out + cut.head * T::SIZE;
+      const int hi = min(cut.full, (part + 1) * a.chunk);
+      for (int j = part * a.chunk + g; j < hi; j += a.lanes) *(typename T::Raw*)(obody + (uint32_t)j * 16u) = zero;
+      if (last && cut.has_edge(g)) T::put(out, cut.edge(g), 0.0f);
       continue;
     }
     long at;
@@ -555,21 +631,28 @@ __global__ __launch_bounds__(GRAD_WG) void k_token_grad(GradArgs a) {
       at = (long)b * a.sb + (long)((unsigned)n - b * (unsigned)a.L) * a.sl;
     }
     const char* row = (const char*)a.z + at * T::SIZE;
-    const float m = st.x, scale = -c / st.y;
+    const Cut<T, PEEL> cut(row, a.V);
+    const char* body = row + cut.head * T::SIZE;
+    char* obody = out + cut.head * T::SIZE;
+    const int lo = part * a.chunk, hi = min(cut.full, lo + a.chunk);
+    const float m = st.x, inv_S = rcp_acc(st.y), scale = -c * inv_S;
     float f[E];
 #pragma unroll 4
     for (int j = lo + g; j < hi; j += a.lanes) {
-      T::unpack(*(const typename T::Raw*)(row + (long)j * 16), f);
+      T::unpack(*(const typename T::Raw*)(body + (uint32_t)j * 16u), f);
 #pragma unroll
       for (int e = 0; e < E; ++e) f[e] = scale * exp_d(f[e] - m, a.c_hi, a.c_lo);
-      *(typename T::Raw*)(out + (long)j * 16) = T::pack(f);
+      store_piece<T>(obody + (uint32_t)j * 16u, T::pack(f));
     }
-    if (last && g < rest) T::put(out, full * E + g, scale * exp_d(T::get(row, full * E + g) - m, a.c_hi, a.c_lo));
+    if (last && cut.has_edge(g)) {
+      const int i = cut.edge(g);
+      T::put(out, i, scale * exp_d(T::get(row, i) - m, a.c_hi, a.c_lo));
+    }
     // the token's own element, c (1 - p), by the lane that wrote its place above
-    const int y = min(max(get_int(a.tokens, a.tok_bytes, n), 0), a.V - 1);
-    const bool mine = y < full * E ? y / E >= lo && y / E < hi && ((y / E - lo) & (a.lanes - 1)) == g
-                                   : last && y - full * E == g;
-    if (mine) T::put(out, y, -c * expm1f(st.w * a.inv_tau - logf(st.y)));
+    const int y = min(max(get_int(a.tokens, a.tok_bytes, n), 0), a.V - 1), in = y - cut.head;
+    const bool piece = in >= 0 && in < cut.full * E;
+    if (piece ? in / E >= lo && in / E < hi && ((in / E - lo) & (a.lanes - 1)) == g : last && cut.lane_of(y, 1) == g)
+      T::put(out, y, token_grad(c, st.w, st.y, inv_S, a.c_hi, a.c_lo));
   }
 }
 
@@ -697,7 +780,10 @@ static RowArgs row_args(const d3pm_logits* z, float tau) {
   return a;
 }
 
-// Launches the narrowest shape that holds a row; *grid: the workgroups it took (as many partial sums).
+// Launches the shape that holds a row in the fewest lanes of up to four pieces each, beyond 512 lanes in more pieces:
+// few lanes a row share the row's own arithmetic and short reductions among more rows of a wave (32 x 32 images of 256
+// float32 classes: 57 us at 16 lanes of 4 pieces, 70 at 32 of 2, 100 at 64 of 1; 32 k bf16 classes: 103 us at 512 x 8,
+// 111 at 256 x 16, 142 at 1024 x 4).  *grid: the workgroups it took (as many partial sums).
 template <typename T, int G, int NV, bool DISTILL>
 static int launch_rows(const RowArgs& a, int* grid, hipStream_t s) {
   typedef Shape<G> Sh;
@@ -713,16 +799,17 @@ template <typename T, bool DISTILL>
 static int dispatch_rows(const RowArgs& a, int* grid, hipStream_t s) {
   const int full = a.V / T::E;
   if (full <= 8) return launch_rows<T, 8, 1, DISTILL>(a, grid, s);
-  if (full <= 16) return launch_rows<T, 16, 1, DISTILL>(a, grid, s);
-  if (full <= 32) return launch_rows<T, 32, 1, DISTILL>(a, grid, s);
-  if (full <= 64) return launch_rows<T, 64, 1, DISTILL>(a, grid, s);
-  if (full <= 128) return launch_rows<T, 64, 2, DISTILL>(a, grid, s);
+  if (full <= 16) return launch_rows<T, 8, 2, DISTILL>(a, grid, s);
+  if (full <= 32) return launch_rows<T, 8, 4, DISTILL>(a, grid, s);
+  if (full <= 64) return launch_rows<T, 16, 4, DISTILL>(a, grid, s);
+  if (full <= 128) return launch_rows<T, 32, 4, DISTILL>(a, grid, s);
   if (full <= 256) return launch_rows<T, 64, 4, DISTILL>(a, grid, s);
-  if (full <= 512) return launch_rows<T, 256, 2, DISTILL>(a, grid, s);
+  if (full <= 512) return launch_rows<T, 128, 4, DISTILL>(a, grid, s);
   if (full <= 1024) return launch_rows<T, 256, 4, DISTILL>(a, grid, s);
-  if (full <= 2048) return launch_rows<T, 256, 8, DISTILL>(a, grid, s);
+  if (full <= 2048) return launch_rows<T, 512, 4, DISTILL>(a, grid, s);
   if (full <= 4096) return launch_rows<T, 512, 8, DISTILL>(a, grid, s);
   if (full <= 8192) return launch_rows<T, 512, 16, DISTILL>(a, grid, s);
+  if (full <= 16384) return launch_rows<T, 1024, 16, DISTILL>(a, grid, s);
   *grid = std::min(a.N, MAX_PARTIALS);
   hipLaunchKernelGGL((k_rows_wide<T, DISTILL>), dim3(*grid), dim3(WIDE), DISTILL ? (size_t)a.k * 8 : 0, s, a);
   D3PM_LAUNCH_CHECK("k_rows_wide");
@@ -734,6 +821,13 @@ static int run_rows(const RowArgs& a, int dtype, int* grid, hipStream_t s) {
        : dtype == D3PM_F16 ? dispatch_rows<F16, DISTILL>(a, grid, s) : dispatch_rows<BF16, DISTILL>(a, grid, s);
 }
 
+template <typename T>
+static int launch_grad(const GradArgs& a, bool peel, int grid, hipStream_t s) {
+  if (peel) hipLaunchKernelGGL((k_token_grad<T, true>), dim3(grid), dim3(GRAD_WG), 0, s, a);
+  else hipLaunchKernelGGL((k_token_grad<T, false>), dim3(grid), dim3(GRAD_WG), 0, s, a);
+  D3PM_LAUNCH_CHECK("k_token_grad");
+  return D3PM_OK;
+}
 static int run_grad(const d3pm_logits* z, const void* tokens, int tok_bytes, float tau, const float* stats,
                     const float* upstream, int per_row, int only_if_rescaled, void* dz, hipStream_t s) {
   GradArgs a{};
@@ -750,11 +844,9 @@ static int run_grad(const d3pm_logits* z, const void* tokens, int tok_bytes, flo
   a.chunks = std::max(1, (full + a.chunk - 1) / a.chunk);
   const long jobs = (long)a.N * a.chunks, per = GRAD_WG / a.lanes;
   const int grid = (int)std::min<long>((jobs + per - 1) / per, 4096);
-  if (z->dtype == D3PM_F32) hipLaunchKernelGGL((k_token_grad<F32>), dim3(grid), dim3(GRAD_WG), 0, s, a);
-  else if (z->dtype == D3PM_F16) hipLaunchKernelGGL((k_token_grad<F16>), dim3(grid), dim3(GRAD_WG), 0, s, a);
-  else hipLaunchKernelGGL((k_token_grad<BF16>), dim3(grid), dim3(GRAD_WG), 0, s, a);
-  D3PM_LAUNCH_CHECK("k_token_grad");
-  return D3PM_OK;
+  const bool peel = a.lanes >= 64;                   // a lane for every end element
+  if (z->dtype == D3PM_F32) return launch_grad<F32>(a, peel, grid, s);
+  return z->dtype == D3PM_F16 ? launch_grad<F16>(a, peel, grid, s) : launch_grad<BF16>(a, peel, grid, s);
 }
 
 // The count of the mask (first 8 bytes of the workspace) and the partial sums behind it.

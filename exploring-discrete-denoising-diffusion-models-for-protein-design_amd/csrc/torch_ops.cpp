@@ -3,7 +3,7 @@
 // A thin shim: every operator checks its tensors, allocates its outputs (and workspace) with torch's
 // allocator, and calls the C ABI of libd3pm_hip.so (include/d3pm_hip.h) on torch's current HIP stream.  No
 // arithmetic happens here.  The operators carry the reference function they stand for in their schema comment;
-// autograd nodes live in the Python facade, which calls these operators.  Status codes of the library become
+// autograd nodes live in the Python facade, which calls these operators (those of the fine-tuning objectives live here).  Status codes of the library become
 // the exceptions the reference raises: D3PM_EINVAL -> ValueError, D3PM_EUNSUPPORTED -> NotImplementedError,
 // D3PM_EHIP -> RuntimeError.  Every operator makes the device of its first tensor current for the call and checks
 // every tensor's element count against the batch it describes before a pointer reaches the library: a mis-shaped
@@ -11,6 +11,10 @@
 #include <ATen/ATen.h>
 #include <ATen/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
 
 #include <tuple>
@@ -622,18 +626,18 @@ void need_same_device(const Tensor& t, const Tensor& z, const char* what) {
 // The library's view of logits [B, ..., V]: `rows` keeps the tensor that it points into (a copy where the middle
 // dimensions cannot be walked with one stride, or the classes do not lie side by side).
 struct LogitsView { Tensor rows; d3pm_logits desc; };
-LogitsView logits_view(const Tensor& z, const Tensor& per_row, const char* per_row_name) {
+LogitsView logits_view(const Tensor& z, at::IntArrayRef per_row, const char* per_row_name) {
   TORCH_CHECK(z.is_cuda(), "d3pm_mi355x: logits must live on an MI355X (device='cuda'); there is no CPU path");
-  TORCH_CHECK_VALUE(z.dim() == per_row.dim() + 1 && z.dim() >= 2 && z.sizes().slice(0, z.dim() - 1) == per_row.sizes(),
+  TORCH_CHECK_VALUE(z.dim() >= 2 && z.sizes().slice(0, z.dim() - 1) == per_row,
                     "d3pm_mi355x: logits must have the shape of ", per_row_name, " and a trailing class dimension, got ",
-                    z.sizes(), " and ", per_row.sizes());
+                    z.sizes(), " and ", per_row);
   const int64_t nd = z.dim(), V = z.size(-1);
   TORCH_CHECK_VALUE(V >= 1 && V <= (1 << 27), "d3pm_mi355x: logits have ", V, " classes, need 1 .. 2^27");
   LogitsView v{z, {}};
   v.desc.dtype = float_dtype(z, "logits");
   v.desc.V = (int)V;
   v.desc.B = z.size(0);
-  v.desc.L = v.desc.B ? per_row.numel() / v.desc.B : 0;
+  v.desc.L = v.desc.B ? z.numel() / V / v.desc.B : 0;
   bool walk = V == 1 || z.stride(-1) == 1;
   int64_t inner = -1, next = 0;                 // stride of the innermost middle dimension; what the next one must be
   for (int64_t i = nd - 2; i >= 1 && walk; --i) {
@@ -648,12 +652,13 @@ LogitsView logits_view(const Tensor& z, const Tensor& per_row, const char* per_r
   v.desc.data = v.rows.data_ptr();
   return v;
 }
-const uint8_t* mask_ptr(const OptTensor& m, const Tensor& per_row, const Tensor& z) {
+const uint8_t* mask_ptr(const OptTensor& m, at::IntArrayRef per_row, const Tensor& z) {
   if (!m.has_value() || !m->defined()) return nullptr;
   need_device(*m, "mask");
   need_same_device(*m, z, "mask");
   TORCH_CHECK_TYPE(m->scalar_type() == at::kBool, "d3pm_mi355x: mask must be bool, got ", m->scalar_type());
-  need_same_shape(*m, per_row, "mask and the logits' positions");
+  TORCH_CHECK_VALUE(m->sizes() == per_row, "d3pm_mi355x: mask must have the shape of the logits' positions, got ",
+                    m->sizes(), " and ", per_row);
   return (const uint8_t*)m->data_ptr();
 }
 const float* row_f32(const Tensor& t, const Tensor& per_row, const Tensor& z, const char* what) {
@@ -670,162 +675,319 @@ const float* upstream_ptr(const Tensor& u, const Tensor& z) {
   need_numel(u, 1, "upstream");
   return f32(u, "upstream");
 }
-void need_grad_like(const Tensor& dz, const Tensor& z) {
-  need_device(dz, "dlogits");
-  need_same_device(dz, z, "dlogits");
-  need_same_shape(dz, z, "dlogits and logits");
-  TORCH_CHECK_TYPE(dz.scalar_type() == z.scalar_type(), "d3pm_mi355x: dlogits must have the logits' type");
-}
 Tensor objective_workspace(const d3pm_logits& d, const Tensor& z, size_t* bytes) {
   *bytes = d3pm_objective_workspace(d.B, d.L);
   return at::empty({(int64_t)(*bytes / 8 + 1)}, z.options().dtype(at::kDouble));
 }
-Tensor grad_buffer(const Tensor& z, bool want) {
-  return want ? at::empty(z.sizes(), z.options().memory_format(at::MemoryFormat::Contiguous))
-              : at::empty({0}, z.options());
-}
+Tensor grad_buffer(const Tensor& z) { return at::empty(z.sizes(), z.options().memory_format(at::MemoryFormat::Contiguous)); }
 
-// log_softmax(logits / temperature) at the tokens, float32; stats [.., 4]: what token_grad_ takes
-std::tuple<Tensor, Tensor> token_logprobs(const Tensor& logits, const Tensor& tokens, const OptTensor& mask,
-                                          double temperature, bool want_stats) {
+// The autograd nodes of these losses are C++: at the sizes where the host is the bound (a protein batch), a Python
+// node and its saved tensors took 45 us of a 92 us forward and backward.  A node keeps what its gradient needs, and
+// the gradient buffer that the loss launch filled for an upstream gradient of 1; backward hands that buffer over
+// after a launch that does it again only if the upstream gradient is another number, and a second backward
+// (retain_graph) fills a buffer of its own.
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+
+struct ObjectiveNode : public torch::autograd::Node {
+  SavedVariable logits_;
+  std::vector<SavedVariable> saved_;
+  Tensor dz_;
+  bool released_ = false;
+
+  void save(const Tensor& logits, std::initializer_list<Tensor> others) {
+    logits_ = SavedVariable(logits, false);
+    for (const Tensor& t : others) saved_.emplace_back(t, false);
+    set_next_edges(torch::autograd::collect_next_edges(logits));
+  }
+  // the gradient for `upstream` into dz; only_if_rescaled: dz holds that for an upstream gradient of 1
+  virtual void fill(const Tensor& logits, const std::vector<Tensor>& saved, const Tensor& upstream,
+                    bool only_if_rescaled, Tensor& dz) = 0;
+
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    TORCH_CHECK(!released_, torch::autograd::ERR_BACKWARD_TWICE);
+    if (!grads[0].defined() || !task_should_compute_output(0)) return variable_list(1);
+    const bool twice = at::GradMode::is_enabled();
+    Tensor dz;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const Tensor logits = logits_.unpack(getptr());
+      std::vector<Tensor> saved;
+      for (const auto& v : saved_) saved.push_back(v.unpack(getptr()));
+      const Tensor upstream = grads[0].contiguous();
+      const bool first = dz_.defined();
+      dz = first ? std::move(dz_) : at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
+      dz_.reset();
+      fill(logits, saved, upstream, first, dz);
+    }
+    if (!twice) return {std::move(dz)};
+    // create_graph: the gradient is a value; differentiating it is an error, not a zero
+    auto error = std::make_shared<torch::autograd::DelayedError>("d3pm_mi355x: the gradient of " + name() + " cannot be differentiated", 1);
+    return (*error)({std::move(dz)});
+  }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    logits_.reset_data();
+    for (auto& v : saved_) v.reset_data();
+    dz_.reset();
+    released_ = true;
+  }
+};
+template <typename N>
+std::shared_ptr<N> new_node() { return std::shared_ptr<N>(new N(), torch::autograd::deleteNode); }
+bool differentiated(const Tensor& logits) { return at::GradMode::is_enabled() && logits.requires_grad(); }
+void need_constant(const Tensor& t, const char* what) {
+  TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && t.requires_grad()), "d3pm_mi355x: ", what, " is a constant of this loss and must not require a gradient (detach it)");
+}
+void need_constant(const OptTensor& t, const char* what) {
+  if (t.has_value() && t->defined()) need_constant(*t, what);
+}
+Tensor opt(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+
+// ---- log_softmax(logits / temperature) at the tokens, float32; stats [.., 4]: what its gradient is made from
+std::tuple<Tensor, Tensor> token_logprobs_run(const Tensor& logits, const Tensor& tokens, const OptTensor& mask,
+                                              double temperature, bool want_stats) {
   D3PM_GUARD(logits);
-  auto v = logits_view(logits, tokens, "tokens");
+  auto v = logits_view(logits, tokens.sizes(), "tokens");
   auto fo = logits.options().dtype(at::kFloat);
-  Tensor lp = at::empty(tokens.sizes(), fo), stats = at::empty({want_stats ? tokens.numel() : 0, 4}, fo);
+  Tensor lp = at::empty(tokens.sizes(), fo), stats;
+  if (want_stats) stats = at::empty({tokens.numel(), 4}, fo);
   check_rc(d3pm_token_logprobs(&v.desc, tokens.data_ptr(), token_bytes(tokens, logits, "tokens"),
-                               mask_ptr(mask, tokens, logits), (float)temperature, lp.data_ptr<float>(),
+                               mask_ptr(mask, tokens.sizes(), logits), (float)temperature, lp.data_ptr<float>(),
                                want_stats ? stats.data_ptr<float>() : nullptr, stream()));
   return {lp, stats};
 }
-
-// the gradient at the logits from the rows' statistics, into dlogits
-void token_grad_(const Tensor& logits, const Tensor& tokens, double temperature, const Tensor& stats,
-                 const Tensor& upstream, bool per_row, bool only_if_rescaled, Tensor dlogits) {
+// the gradient at the logits from the rows' statistics
+void token_grad_run(const Tensor& logits, const Tensor& tokens, double temperature, const Tensor& stats,
+                    const Tensor& upstream, bool per_row, bool only_if_rescaled, Tensor& dz) {
   D3PM_GUARD(logits);
-  auto v = logits_view(logits, tokens, "tokens");
-  need_grad_like(dlogits, logits);
-  need_same_device(stats, logits, "stats");
-  need_numel(stats, tokens.numel() * 4, "stats");
+  auto v = logits_view(logits, tokens.sizes(), "tokens");
   const float* u = per_row ? row_f32(upstream, tokens, logits, "upstream and tokens") : upstream_ptr(upstream, logits);
   check_rc(d3pm_token_grad(&v.desc, tokens.data_ptr(), token_bytes(tokens, logits, "tokens"), (float)temperature,
-                           f32(stats, "stats"), u, per_row, only_if_rescaled, dlogits.data_ptr(), stream()));
+                           f32(stats, "stats"), u, per_row, only_if_rescaled, dz.data_ptr(), stream()));
+}
+struct TokenLogprobsBackward : public ObjectiveNode {
+  double temperature;
+  std::string name() const override { return "TokenLogprobs"; }
+  void fill(const Tensor& logits, const std::vector<Tensor>& s, const Tensor& upstream, bool, Tensor& dz) override {
+    token_grad_run(logits, s[0], temperature, s[1], upstream, true, false, dz);
+  }
+};
+Tensor token_logprobs(const Tensor& logits, const Tensor& tokens, const OptTensor& mask, double temperature) {
+  return std::get<0>(token_logprobs_run(logits, tokens, mask, temperature, false));
+}
+Tensor token_logprobs_autograd(const Tensor& logits, const Tensor& tokens, const OptTensor& mask, double temperature) {
+  const bool want = differentiated(logits);
+  Tensor lp, stats;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    std::tie(lp, stats) = token_logprobs_run(logits, tokens, mask, temperature, want);
+  }
+  if (want) {
+    auto node = new_node<TokenLogprobsBackward>();
+    node->save(logits, {tokens, stats});
+    node->temperature = temperature;
+    torch::autograd::set_history(lp, node);
+  }
+  return lp;
 }
 
+// ---- distillation from a teacher's top logits
 struct Teacher { int dtype, index_bytes, k; };
 Teacher check_teacher(const Tensor& tl, const Tensor& ti, const Tensor& z) {
   need_device(tl, "teacher_logits"); need_device(ti, "teacher_index");
   need_same_device(tl, z, "teacher_logits"); need_same_device(ti, z, "teacher_index");
   need_same_shape(tl, ti, "teacher_logits and teacher_index");
   const int64_t k = tl.dim() ? tl.size(-1) : 0;
-  TORCH_CHECK_VALUE(tl.dim() == z.dim() && tl.sizes().slice(0, z.dim() - 1) == z.sizes().slice(0, z.dim() - 1),
+  TORCH_CHECK_VALUE(z.dim() >= 2 && tl.dim() == z.dim() &&
+                        tl.sizes().slice(0, z.dim() - 1) == z.sizes().slice(0, z.dim() - 1),
                     "d3pm_mi355x: teacher_logits must be [.., k] over the logits' positions, got ", tl.sizes(), " for ",
                     z.sizes());
   TORCH_CHECK_VALUE(k >= 1 && k <= 256, "d3pm_mi355x: the teacher's lists have ", k, " entries, need 1 .. 256");
   return {float_dtype(tl, "teacher_logits"), tok_bytes(ti, "teacher_index"), (int)k};
 }
-
-// (loss [], per_token, dlogits): distillation from a teacher's top logits
-std::tuple<Tensor, Tensor, Tensor> topk_distill_loss(const Tensor& logits, const Tensor& teacher_logits,
-                                                     const Tensor& teacher_index, const OptTensor& mask,
-                                                     double temperature, double out_scale, bool want_grad) {
+struct DistillArgs { double temperature, out_scale; };
+// loss and per may be null (the gradient alone, times upstream), dz too (no gradient)
+void distill_run(const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_index, const OptTensor& mask,
+                 const DistillArgs& args, const float* upstream, bool only_if_rescaled, Tensor* loss, Tensor* per,
+                 const Tensor& dz) {
   D3PM_GUARD(logits);
   const Teacher t = check_teacher(teacher_logits, teacher_index, logits);
-  auto fo = logits.options().dtype(at::kFloat);
-  Tensor loss = at::empty({}, fo), per = at::empty(logits.sizes().slice(0, logits.dim() - 1), fo);
-  auto v = logits_view(logits, per, "the teacher's positions");
-  Tensor dz = grad_buffer(logits, want_grad);
+  auto v = logits_view(logits, logits.sizes().slice(0, logits.dim() - 1), "the teacher's positions");
+  if (loss) {
+    auto fo = logits.options().dtype(at::kFloat);
+    *loss = at::empty({}, fo);
+    *per = at::empty(logits.sizes().slice(0, logits.dim() - 1), fo);
+  }
   size_t wsb;
   Tensor ws = objective_workspace(v.desc, logits, &wsb);
   check_rc(d3pm_topk_distill_loss(&v.desc, teacher_logits.data_ptr(), t.dtype, teacher_index.data_ptr(), t.index_bytes,
-                                  t.k, mask_ptr(mask, per, logits), (float)temperature, (float)out_scale, nullptr, 0,
-                                  loss.data_ptr<float>(), per.data_ptr<float>(), want_grad ? dz.data_ptr() : nullptr,
-                                  ws.data_ptr(), wsb, stream()));
-  return {loss, per, dz};
+                                  t.k, mask_ptr(mask, logits.sizes().slice(0, logits.dim() - 1), logits),
+                                  (float)args.temperature, (float)args.out_scale, upstream, only_if_rescaled,
+                                  loss ? loss->data_ptr<float>() : nullptr, per ? per->data_ptr<float>() : nullptr,
+                                  dz.defined() ? dz.data_ptr() : nullptr, ws.data_ptr(), wsb, stream()));
 }
-// its gradient alone, times upstream, into dlogits
-void topk_distill_grad_(const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_index,
-                        const OptTensor& mask, double temperature, double out_scale, const Tensor& upstream,
-                        bool only_if_rescaled, Tensor dlogits) {
-  D3PM_GUARD(logits);
-  const Teacher t = check_teacher(teacher_logits, teacher_index, logits);
-  const Tensor rows = logits.select(-1, 0);
-  auto v = logits_view(logits, rows, "the teacher's positions");
-  need_grad_like(dlogits, logits);
-  size_t wsb;
-  Tensor ws = objective_workspace(v.desc, logits, &wsb);
-  check_rc(d3pm_topk_distill_loss(&v.desc, teacher_logits.data_ptr(), t.dtype, teacher_index.data_ptr(), t.index_bytes,
-                                  t.k, mask_ptr(mask, rows, logits), (float)temperature, (float)out_scale,
-                                  upstream_ptr(upstream, logits), only_if_rescaled, nullptr, nullptr, dlogits.data_ptr(),
-                                  ws.data_ptr(), wsb, stream()));
+struct DistillBackward : public ObjectiveNode {
+  DistillArgs args;
+  std::string name() const override { return "TopKDistillLoss"; }
+  void fill(const Tensor& logits, const std::vector<Tensor>& s, const Tensor& upstream, bool only, Tensor& dz) override {
+    distill_run(logits, s[0], s[1], s[2], args, upstream_ptr(upstream, logits), only, nullptr, nullptr, dz);
+  }
+};
+// (loss [], per_token)
+std::tuple<Tensor, Tensor> topk_distill_loss(const Tensor& logits, const Tensor& teacher_logits,
+                                             const Tensor& teacher_index, const OptTensor& mask, double temperature,
+                                             double out_scale) {
+  Tensor loss, per;
+  distill_run(logits, teacher_logits, teacher_index, mask, {temperature, out_scale}, nullptr, false, &loss, &per, Tensor());
+  return {loss, per};
 }
-
-struct PolicyIn { const float* old_lp; const float* adv; int per_seq; const float* ref; };
-PolicyIn check_policy(const Tensor& tokens, const Tensor& old_lp, const Tensor& adv, const OptTensor& ref, const Tensor& z) {
-  PolicyIn p{};
-  p.old_lp = row_f32(old_lp, tokens, z, "old_logprobs and tokens");
-  p.per_seq = adv.dim() == 1 && tokens.dim() > 1;
-  if (p.per_seq) {
-    need_numel(adv, tokens.size(0), "advantages (one per sequence)");
-    need_same_device(adv, z, "advantages");
-    p.adv = f32(adv, "advantages");
-  } else p.adv = row_f32(adv, tokens, z, "advantages and tokens");
-  p.ref = ref.has_value() && ref->defined() ? row_f32(*ref, tokens, z, "ref_logprobs and tokens") : nullptr;
-  return p;
-}
-// (loss [], logprobs, dlogits): clipped policy loss with a KL term
-std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs,
-                                               const Tensor& advantages, const OptTensor& ref_logprobs,
-                                               const OptTensor& mask, double temperature, double clip_low,
-                                               double clip_high, double kl_coeff, double out_scale, bool want_grad) {
-  D3PM_GUARD(logits);
-  auto v = logits_view(logits, tokens, "tokens");
-  const PolicyIn p = check_policy(tokens, old_logprobs, advantages, ref_logprobs, logits);
-  auto fo = logits.options().dtype(at::kFloat);
-  Tensor loss = at::empty({}, fo), lp = at::empty(tokens.sizes(), fo), dz = grad_buffer(logits, want_grad);
-  size_t wsb;
-  Tensor ws = objective_workspace(v.desc, logits, &wsb);
-  check_rc(d3pm_policy_loss(&v.desc, tokens.data_ptr(), token_bytes(tokens, logits, "tokens"), p.old_lp, p.adv, p.per_seq,
-                            p.ref, mask_ptr(mask, tokens, logits), (float)temperature, (float)clip_low, (float)clip_high,
-                            (float)kl_coeff, (float)out_scale, nullptr, 0, loss.data_ptr<float>(), lp.data_ptr<float>(),
-                            want_grad ? dz.data_ptr() : nullptr, ws.data_ptr(), wsb, stream()));
-  return {loss, lp, dz};
-}
-// its gradient alone, times upstream, into dlogits
-void policy_grad_(const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs, const Tensor& advantages,
-                  const OptTensor& ref_logprobs, const OptTensor& mask, double temperature, double clip_low,
-                  double clip_high, double kl_coeff, double out_scale, const Tensor& upstream, bool only_if_rescaled,
-                  Tensor dlogits) {
-  D3PM_GUARD(logits);
-  auto v = logits_view(logits, tokens, "tokens");
-  const PolicyIn p = check_policy(tokens, old_logprobs, advantages, ref_logprobs, logits);
-  need_grad_like(dlogits, logits);
-  size_t wsb;
-  Tensor ws = objective_workspace(v.desc, logits, &wsb);
-  check_rc(d3pm_policy_loss(&v.desc, tokens.data_ptr(), token_bytes(tokens, logits, "tokens"), p.old_lp, p.adv, p.per_seq,
-                            p.ref, mask_ptr(mask, tokens, logits), (float)temperature, (float)clip_low, (float)clip_high,
-                            (float)kl_coeff, (float)out_scale, upstream_ptr(upstream, logits), only_if_rescaled, nullptr,
-                            nullptr, dlogits.data_ptr(), ws.data_ptr(), wsb, stream()));
+std::tuple<Tensor, Tensor> topk_distill_loss_autograd(const Tensor& logits, const Tensor& teacher_logits,
+                                                      const Tensor& teacher_index, const OptTensor& mask,
+                                                      double temperature, double out_scale) {
+  need_constant(teacher_logits, "teacher_logits");
+  const bool want = differentiated(logits);
+  Tensor loss, per, dz;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    if (want) dz = grad_buffer(logits);
+    distill_run(logits, teacher_logits, teacher_index, mask, {temperature, out_scale}, nullptr, false, &loss, &per, dz);
+  }
+  if (want) {
+    auto node = new_node<DistillBackward>();
+    node->save(logits, {teacher_logits, teacher_index, opt(mask)});
+    node->dz_ = std::move(dz);
+    node->args = {temperature, out_scale};
+    torch::autograd::set_history(loss, node);
+  }
+  return {loss, per};
 }
 
-// (loss [], rewards [B], stats, dlogits): preference loss of the pairs (p, p + B / 2)
-std::tuple<Tensor, Tensor, Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& tokens,
-                                                           const OptTensor& ref_logprobs, const OptTensor& mask,
-                                                           double beta, double label_smoothing, bool average,
-                                                           double out_scale, bool want_grad) {
+// ---- clipped policy loss with a KL term
+struct PolicyArgs { double temperature, clip_low, clip_high, kl_coeff, out_scale; };
+void policy_run(const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs, const Tensor& advantages,
+                const OptTensor& ref_logprobs, const OptTensor& mask, const PolicyArgs& args, const float* upstream,
+                bool only_if_rescaled, Tensor* loss, Tensor* lp, const Tensor& dz) {
   D3PM_GUARD(logits);
-  auto v = logits_view(logits, tokens, "tokens");
+  auto v = logits_view(logits, tokens.sizes(), "tokens");
+  const float* old_lp = row_f32(old_logprobs, tokens, logits, "old_logprobs and tokens");
+  const bool per_seq = advantages.dim() == 1 && tokens.dim() > 1;
+  if (per_seq) {
+    need_numel(advantages, tokens.size(0), "advantages (one per sequence)");
+    need_same_device(advantages, logits, "advantages");
+  } else need_same_shape(advantages, tokens, "advantages and tokens");
+  need_same_device(advantages, logits, "advantages");
+  const float* ref = ref_logprobs.has_value() && ref_logprobs->defined()
+                         ? row_f32(*ref_logprobs, tokens, logits, "ref_logprobs and tokens") : nullptr;
+  if (loss) {
+    auto fo = logits.options().dtype(at::kFloat);
+    *loss = at::empty({}, fo);
+    *lp = at::empty(tokens.sizes(), fo);
+  }
+  size_t wsb;
+  Tensor ws = objective_workspace(v.desc, logits, &wsb);
+  check_rc(d3pm_policy_loss(&v.desc, tokens.data_ptr(), token_bytes(tokens, logits, "tokens"), old_lp,
+                            f32(advantages, "advantages"), per_seq, ref, mask_ptr(mask, tokens.sizes(), logits),
+                            (float)args.temperature, (float)args.clip_low, (float)args.clip_high, (float)args.kl_coeff,
+                            (float)args.out_scale, upstream, only_if_rescaled, loss ? loss->data_ptr<float>() : nullptr,
+                            lp ? lp->data_ptr<float>() : nullptr, dz.defined() ? dz.data_ptr() : nullptr, ws.data_ptr(),
+                            wsb, stream()));
+}
+struct PolicyBackward : public ObjectiveNode {
+  PolicyArgs args;
+  std::string name() const override { return "PolicyLoss"; }
+  void fill(const Tensor& logits, const std::vector<Tensor>& s, const Tensor& upstream, bool only, Tensor& dz) override {
+    policy_run(logits, s[0], s[1], s[2], s[3], s[4], args, upstream_ptr(upstream, logits), only, nullptr, nullptr, dz);
+  }
+};
+// (loss [], logprobs)
+std::tuple<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs,
+                                       const Tensor& advantages, const OptTensor& ref_logprobs, const OptTensor& mask,
+                                       double temperature, double clip_low, double clip_high, double kl_coeff,
+                                       double out_scale) {
+  Tensor loss, lp;
+  policy_run(logits, tokens, old_logprobs, advantages, ref_logprobs, mask,
+             {temperature, clip_low, clip_high, kl_coeff, out_scale}, nullptr, false, &loss, &lp, Tensor());
+  return {loss, lp};
+}
+std::tuple<Tensor, Tensor> policy_loss_autograd(const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs,
+                                                const Tensor& advantages, const OptTensor& ref_logprobs,
+                                                const OptTensor& mask, double temperature, double clip_low,
+                                                double clip_high, double kl_coeff, double out_scale) {
+  need_constant(old_logprobs, "old_logprobs");
+  need_constant(advantages, "advantages");
+  need_constant(ref_logprobs, "ref_logprobs");
+  const bool want = differentiated(logits);
+  const PolicyArgs args{temperature, clip_low, clip_high, kl_coeff, out_scale};
+  Tensor loss, lp, dz;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    if (want) dz = grad_buffer(logits);
+    policy_run(logits, tokens, old_logprobs, advantages, ref_logprobs, mask, args, nullptr, false, &loss, &lp, dz);
+  }
+  if (want) {
+    auto node = new_node<PolicyBackward>();
+    node->save(logits, {tokens, old_logprobs, advantages, opt(ref_logprobs), opt(mask)});
+    node->dz_ = std::move(dz);
+    node->args = args;
+    torch::autograd::set_history(loss, node);
+  }
+  return {loss, lp};
+}
+
+// ---- preference loss of the pairs (p, p + B / 2)
+void preference_run(const Tensor& logits, const Tensor& tokens, const OptTensor& ref_logprobs, const OptTensor& mask,
+                    double beta, double label_smoothing, bool average, double out_scale, Tensor* loss, Tensor* rewards,
+                    Tensor* stats, const Tensor& dz) {
+  D3PM_GUARD(logits);
+  auto v = logits_view(logits, tokens.sizes(), "tokens");
   const float* ref = ref_logprobs.has_value() && ref_logprobs->defined()
                          ? row_f32(*ref_logprobs, tokens, logits, "ref_logprobs and tokens") : nullptr;
   auto fo = logits.options().dtype(at::kFloat);
-  Tensor loss = at::empty({}, fo), rewards = at::empty({v.desc.B}, fo), stats = at::empty({tokens.numel(), 4}, fo);
-  Tensor dz = grad_buffer(logits, want_grad);
+  *loss = at::empty({}, fo);
+  *rewards = at::empty({v.desc.B}, fo);
+  *stats = at::empty({tokens.numel(), 4}, fo);
   size_t wsb;
   Tensor ws = objective_workspace(v.desc, logits, &wsb);
   check_rc(d3pm_preference_loss(&v.desc, tokens.data_ptr(), token_bytes(tokens, logits, "tokens"), ref,
-                                mask_ptr(mask, tokens, logits), (float)beta, (float)label_smoothing, average,
-                                (float)out_scale, loss.data_ptr<float>(), rewards.data_ptr<float>(),
-                                stats.data_ptr<float>(), want_grad ? dz.data_ptr() : nullptr, ws.data_ptr(), wsb, stream()));
-  return {loss, rewards, stats, dz};
+                                mask_ptr(mask, tokens.sizes(), logits), (float)beta, (float)label_smoothing, average,
+                                (float)out_scale, loss->data_ptr<float>(), rewards->data_ptr<float>(),
+                                stats->data_ptr<float>(), dz.defined() ? dz.data_ptr() : nullptr, ws.data_ptr(), wsb,
+                                stream()));
+}
+struct PreferenceBackward : public ObjectiveNode {
+  std::string name() const override { return "PreferenceLoss"; }
+  void fill(const Tensor& logits, const std::vector<Tensor>& s, const Tensor& upstream, bool only, Tensor& dz) override {
+    token_grad_run(logits, s[0], 1.0, s[1], upstream, false, only, dz);
+  }
+};
+// (loss [], rewards [B])
+std::tuple<Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& tokens, const OptTensor& ref_logprobs,
+                                           const OptTensor& mask, double beta, double label_smoothing, bool average,
+                                           double out_scale) {
+  Tensor loss, rewards, stats;
+  preference_run(logits, tokens, ref_logprobs, mask, beta, label_smoothing, average, out_scale, &loss, &rewards, &stats, Tensor());
+  return {loss, rewards};
+}
+std::tuple<Tensor, Tensor> preference_loss_autograd(const Tensor& logits, const Tensor& tokens,
+                                                    const OptTensor& ref_logprobs, const OptTensor& mask, double beta,
+                                                    double label_smoothing, bool average, double out_scale) {
+  need_constant(ref_logprobs, "ref_logprobs");
+  const bool want = differentiated(logits);
+  Tensor loss, rewards, stats, dz;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    if (want) dz = grad_buffer(logits);
+    preference_run(logits, tokens, ref_logprobs, mask, beta, label_smoothing, average, out_scale, &loss, &rewards, &stats, dz);
+  }
+  if (want) {
+    auto node = new_node<PreferenceBackward>();
+    node->save(logits, {tokens, stats});
+    node->dz_ = std::move(dz);
+    torch::autograd::set_history(loss, node);
+  }
+  return {loss, rewards};
 }
 
 }  // namespace
@@ -833,10 +995,6 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> preference_loss(const Tensor& logits,
 #define D3PM_TB "Tensor[] tables, int K, int T, bool structured, float eps, "
 #define D3PM_PT "Tensor qbar_digest, Tensor qone_digest, Tensor lvb_digest, int K, int T, "
 #define D3PM_LOSS_ARGS "Tensor logits, Tensor x0, Tensor x_t, Tensor t, int loss_type, float hybrid_coeff, float grad_scale, "
-#define D3PM_DISTILL_ARGS "Tensor logits, Tensor teacher_logits, Tensor teacher_index, Tensor? mask, float temperature, " \
-                          "float out_scale, "
-#define D3PM_POLICY_ARGS "Tensor logits, Tensor tokens, Tensor old_logprobs, Tensor advantages, Tensor? ref_logprobs, " \
-                         "Tensor? mask, float temperature, float clip_low, float clip_high, float kl_coeff, float out_scale, "
 
 TORCH_LIBRARY(d3pm_mi355x, m) {
   m.def("q_probs(" D3PM_TB "Tensor x0, Tensor t) -> Tensor");
@@ -873,15 +1031,13 @@ TORCH_LIBRARY(d3pm_mi355x, m) {
   m.def("lvb_reverse_step(" D3PM_PT "Tensor pred, Tensor x_t, Tensor t, Tensor? expo, int seed, int offset, "
         "Tensor? offset_dev, float last_class_div, int exclude_last_prefix) -> Tensor");
   m.def("corrupt(" D3PM_PT "Tensor x0, Tensor t, Tensor? expo, int seed, int offset, bool want_probs) -> (Tensor, Tensor)");
-  m.def("token_logprobs(Tensor logits, Tensor tokens, Tensor? mask, float temperature, bool want_stats) -> (Tensor, Tensor)");
-  m.def("token_grad_(Tensor logits, Tensor tokens, float temperature, Tensor stats, Tensor upstream, bool per_row, "
-        "bool only_if_rescaled, Tensor(a!) dlogits) -> ()");
-  m.def("topk_distill_loss(" D3PM_DISTILL_ARGS "bool want_grad) -> (Tensor, Tensor, Tensor)");
-  m.def("topk_distill_grad_(" D3PM_DISTILL_ARGS "Tensor upstream, bool only_if_rescaled, Tensor(a!) dlogits) -> ()");
-  m.def("policy_loss(" D3PM_POLICY_ARGS "bool want_grad) -> (Tensor, Tensor, Tensor)");
-  m.def("policy_grad_(" D3PM_POLICY_ARGS "Tensor upstream, bool only_if_rescaled, Tensor(a!) dlogits) -> ()");
+  m.def("token_logprobs(Tensor logits, Tensor tokens, Tensor? mask, float temperature) -> Tensor");
+  m.def("topk_distill_loss(Tensor logits, Tensor teacher_logits, Tensor teacher_index, Tensor? mask, float temperature, "
+        "float out_scale) -> (Tensor, Tensor)");
+  m.def("policy_loss(Tensor logits, Tensor tokens, Tensor old_logprobs, Tensor advantages, Tensor? ref_logprobs, "
+        "Tensor? mask, float temperature, float clip_low, float clip_high, float kl_coeff, float out_scale) -> (Tensor, Tensor)");
   m.def("preference_loss(Tensor logits, Tensor tokens, Tensor? ref_logprobs, Tensor? mask, float beta, "
-        "float label_smoothing, bool average, float out_scale, bool want_grad) -> (Tensor, Tensor, Tensor, Tensor)");
+        "float label_smoothing, bool average, float out_scale) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(d3pm_mi355x, CUDA, m) {
@@ -913,10 +1069,15 @@ TORCH_LIBRARY_IMPL(d3pm_mi355x, CUDA, m) {
   m.impl("lvb_reverse_step", lvb_reverse_step);
   m.impl("corrupt", corrupt);
   m.impl("token_logprobs", token_logprobs);
-  m.impl("token_grad_", token_grad_);
   m.impl("topk_distill_loss", topk_distill_loss);
-  m.impl("topk_distill_grad_", topk_distill_grad_);
   m.impl("policy_loss", policy_loss);
-  m.impl("policy_grad_", policy_grad_);
   m.impl("preference_loss", preference_loss);
+}
+
+// the fine-tuning objectives bring their own autograd nodes
+TORCH_LIBRARY_IMPL(d3pm_mi355x, AutogradCUDA, m) {
+  m.impl("token_logprobs", token_logprobs_autograd);
+  m.impl("topk_distill_loss", topk_distill_loss_autograd);
+  m.impl("policy_loss", policy_loss_autograd);
+  m.impl("preference_loss", preference_loss_autograd);
 }

@@ -22,7 +22,6 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._ops import ops
@@ -34,13 +33,8 @@ def _tokens(x: torch.Tensor) -> torch.Tensor:
     return x.contiguous()
 
 
-def _constant(x: Optional[torch.Tensor], what: str) -> Optional[torch.Tensor]:
-    """A float32 input that the loss is not differentiated by."""
-    if x is None:
-        return None
-    if x.requires_grad:
-        raise ValueError(f"{what} is a constant of this loss and must not require a gradient (detach it)")
-    return x.contiguous() if x.dtype == torch.float32 else x.to(torch.float32).contiguous()
+def _float32(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return None if x is None else x.to(torch.float32).contiguous()
 
 
 def _mask(mask: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -65,61 +59,13 @@ def _finite(x: float, what: str) -> float:
     return x
 
 
-def _hand_over(ctx, fill):
-    """The gradient buffer of the forward launch, with `fill(buffer, only_if_rescaled)` run on it; a second backward
-    (retain_graph) gets a buffer of its own."""
-    logits = ctx.saved_tensors[0]
-    dz, ctx.dz = ctx.dz, None
-    again = dz is None
-    if again:
-        dz = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    fill(dz, not again)
-    return dz
-
-
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, mask, temperature):
-        lp, stats = ops.token_logprobs(logits, tokens, mask, temperature, ctx.needs_input_grad[0])
-        ctx.save_for_backward(logits, tokens, stats)
-        ctx.temperature = temperature
-        return lp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        logits, tokens, stats = ctx.saved_tensors
-        dz = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        ops.token_grad_(logits, tokens, ctx.temperature, stats, g.contiguous(), True, False, dz)
-        return dz, None, None, None
-
-
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, mask: Optional[torch.Tensor] = None,
                    temperature: float = 1.0) -> torch.Tensor:
     """``log_softmax(logits / temperature)`` at ``tokens`` (logits ``[..., V]``, tokens ``[...]``), float32 of the
     tokens' shape, 0 where ``mask`` is false; differentiable by the logits."""
     _lib.require_device(logits, tokens, mask)
     tokens, mask, temperature = _tokens(tokens), _mask(mask), _temperature(temperature)
-    if not (torch.is_grad_enabled() and logits.requires_grad):
-        return ops.token_logprobs(logits, tokens, mask, temperature, False)[0]
-    return _TokenLogprobs.apply(logits, tokens, mask, temperature)
-
-
-class _Distill(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, teacher_logits, teacher_index, mask, temperature, out_scale):
-        loss, per, dz = ops.topk_distill_loss(logits, teacher_logits, teacher_index, mask, temperature, out_scale,
-                                              ctx.needs_input_grad[0])
-        ctx.save_for_backward(logits, teacher_logits, teacher_index, mask)
-        ctx.dz, ctx.args = dz, (temperature, out_scale)
-        ctx.mark_non_differentiable(per)
-        return loss, per
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, _per):
-        saved = ctx.saved_tensors
-        return (_hand_over(ctx, lambda dz, only: ops.topk_distill_grad_(*saved, *ctx.args, g, only, dz)),) + (None,) * 5
+    return ops.token_logprobs(logits, tokens, mask, temperature)
 
 
 class TopKDistillLoss(torch.nn.Module):
@@ -138,31 +84,9 @@ class TopKDistillLoss(torch.nn.Module):
 
     def forward(self, logits, teacher_logits, teacher_index, mask=None, out_scale=1.0):
         _lib.require_device(logits, teacher_logits, teacher_index, mask)
-        if teacher_logits.requires_grad:
-            raise ValueError("teacher_logits is a constant of this loss and must not require a gradient (detach it)")
-        args = (teacher_logits.contiguous(), _tokens(teacher_index), _mask(mask), self.temperature,
-                _finite(out_scale, "out_scale"))
-        if torch.is_grad_enabled() and logits.requires_grad:
-            loss, self.per_token = _Distill.apply(logits, *args)
-        else:
-            loss, self.per_token, _ = ops.topk_distill_loss(logits, *args, False)
+        loss, self.per_token = ops.topk_distill_loss(logits, teacher_logits.contiguous(), _tokens(teacher_index),
+                                                     _mask(mask), self.temperature, _finite(out_scale, "out_scale"))
         return loss
-
-
-class _Policy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, old, adv, ref, mask, *args):
-        loss, lp, dz = ops.policy_loss(logits, tokens, old, adv, ref, mask, *args, ctx.needs_input_grad[0])
-        ctx.save_for_backward(logits, tokens, old, adv, ref, mask)
-        ctx.dz, ctx.args = dz, args
-        ctx.mark_non_differentiable(lp)
-        return loss, lp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, _lp):
-        saved = ctx.saved_tensors
-        return (_hand_over(ctx, lambda dz, only: ops.policy_grad_(*saved, *ctx.args, g, only, dz)),) + (None,) * 10
 
 
 class PolicyLoss(torch.nn.Module):
@@ -187,31 +111,10 @@ class PolicyLoss(torch.nn.Module):
         _lib.require_device(logits, tokens, old_logprobs, advantages, ref_logprobs, mask)
         if self.kl_coeff != 0.0 and ref_logprobs is None:
             raise ValueError("kl_coeff needs ref_logprobs")
-        args = (_tokens(tokens), _constant(old_logprobs, "old_logprobs"), _constant(advantages, "advantages"),
-                _constant(ref_logprobs, "ref_logprobs"), _mask(mask), self.temperature, self.clip_low, self.clip_high,
-                self.kl_coeff, _finite(out_scale, "out_scale"))
-        if torch.is_grad_enabled() and logits.requires_grad:
-            loss, self.logprobs = _Policy.apply(logits, *args)
-        else:
-            loss, self.logprobs, _ = ops.policy_loss(logits, *args, False)
+        loss, self.logprobs = ops.policy_loss(logits, _tokens(tokens), _float32(old_logprobs), _float32(advantages),
+                                              _float32(ref_logprobs), _mask(mask), self.temperature, self.clip_low,
+                                              self.clip_high, self.kl_coeff, _finite(out_scale, "out_scale"))
         return loss
-
-
-class _Preference(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, ref, mask, *args):
-        loss, rewards, stats, dz = ops.preference_loss(logits, tokens, ref, mask, *args, ctx.needs_input_grad[0])
-        ctx.save_for_backward(logits, tokens, stats)
-        ctx.dz = dz
-        ctx.mark_non_differentiable(rewards)
-        return loss, rewards
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, _rewards):
-        logits, tokens, stats = ctx.saved_tensors
-        return (_hand_over(ctx, lambda dz, only: ops.token_grad_(logits, tokens, 1.0, stats, g, False, only, dz)),) + \
-            (None,) * 7
 
 
 class PreferenceLoss(torch.nn.Module):
@@ -234,10 +137,6 @@ class PreferenceLoss(torch.nn.Module):
 
     def forward(self, logits, tokens, ref_logprobs=None, mask=None, out_scale=1.0):
         _lib.require_device(logits, tokens, ref_logprobs, mask)
-        args = (_tokens(tokens), _constant(ref_logprobs, "ref_logprobs"), _mask(mask), self.beta, self.label_smoothing,
-                self.average, _finite(out_scale, "out_scale"))
-        if torch.is_grad_enabled() and logits.requires_grad:
-            loss, self.rewards = _Preference.apply(logits, *args)
-        else:
-            loss, self.rewards = ops.preference_loss(logits, *args, False)[:2]
+        loss, self.rewards = ops.preference_loss(logits, _tokens(tokens), _float32(ref_logprobs), _mask(mask), self.beta,
+                                                 self.label_smoothing, self.average, _finite(out_scale, "out_scale"))
         return loss

@@ -118,7 +118,7 @@ def reference(name, d, average=False, scale=1.0):
             mag = (r * A).abs() + CFG["kl"] * (torch.exp(x) + 1)
             cmag = (abs(scale) * mag * w / count / tau).detach()[..., None]
             out = {"loss": loss, "lp": lp * w}
-            out["loss_tol"] = abs(scale) * float((mag * w).sum() / count) * 2 * TOL
+            out["loss_tol"] = abs(scale) * float(((mag * w).sum() / count).detach()) * 2 * TOL
         if "lp" in out:
             out["lp_tol"] = TOL + 4 * EPS * out["lp"].detach().abs()
     p = logp.detach().exp()
