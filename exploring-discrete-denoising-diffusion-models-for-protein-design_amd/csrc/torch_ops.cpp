@@ -652,15 +652,19 @@ LogitsView logits_view(const Tensor& z, at::IntArrayRef per_row, const char* per
   v.desc.data = v.rows.data_ptr();
   return v;
 }
-const uint8_t* mask_ptr(const OptTensor& m, at::IntArrayRef per_row, const Tensor& z) {
-  if (!m.has_value() || !m->defined()) return nullptr;
-  need_device(*m, "mask");
-  need_same_device(*m, z, "mask");
-  TORCH_CHECK_TYPE(m->scalar_type() == at::kBool, "d3pm_mi355x: mask must be bool, got ", m->scalar_type());
-  TORCH_CHECK_VALUE(m->sizes() == per_row, "d3pm_mi355x: mask must have the shape of the logits' positions, got ",
-                    m->sizes(), " and ", per_row);
-  return (const uint8_t*)m->data_ptr();
+const uint8_t* mask_ptr(const Tensor& m, at::IntArrayRef per_row, const Tensor& z) {
+  if (!m.defined()) return nullptr;
+  need_device(m, "mask");
+  need_same_device(m, z, "mask");
+  TORCH_CHECK_TYPE(m.scalar_type() == at::kBool, "d3pm_mi355x: mask must be bool, got ", m.scalar_type());
+  TORCH_CHECK_VALUE(m.sizes() == per_row, "d3pm_mi355x: mask must have the shape of the logits' positions, got ",
+                    m.sizes(), " and ", per_row);
+  return (const uint8_t*)m.data_ptr();
 }
+// inputs as the library takes them: dense, float32
+Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+Tensor dense_f32(const Tensor& t) { return t.defined() ? (t.scalar_type() == at::kFloat ? t : t.to(at::kFloat)).contiguous() : t; }
+Tensor opt(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 const float* row_f32(const Tensor& t, const Tensor& per_row, const Tensor& z, const char* what) {
   need_same_device(t, z, what);
   need_same_shape(t, per_row, what);
@@ -668,6 +672,8 @@ const float* row_f32(const Tensor& t, const Tensor& per_row, const Tensor& z, co
 }
 int token_bytes(const Tensor& t, const Tensor& z, const char* what) {
   need_same_device(t, z, what);
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kLong || t.scalar_type() == at::kInt, "d3pm_mi355x: ", what,
+                   " must be int32 or int64, got ", t.scalar_type());
   return tok_bytes(t, what);
 }
 const float* upstream_ptr(const Tensor& u, const Tensor& z) {
@@ -675,9 +681,8 @@ const float* upstream_ptr(const Tensor& u, const Tensor& z) {
   need_numel(u, 1, "upstream");
   return f32(u, "upstream");
 }
-Tensor objective_workspace(const d3pm_logits& d, const Tensor& z, size_t* bytes) {
-  *bytes = d3pm_objective_workspace(d.B, d.L);
-  return at::empty({(int64_t)(*bytes / 8 + 1)}, z.options().dtype(at::kDouble));
+Tensor objective_workspace(const d3pm_logits& d, const Tensor& z) {
+  return at::empty({(int64_t)(d3pm_objective_workspace(d.B, d.L) / 8 + 1)}, z.options().dtype(at::kDouble));
 }
 Tensor grad_buffer(const Tensor& z) { return at::empty(z.sizes(), z.options().memory_format(at::MemoryFormat::Contiguous)); }
 
@@ -738,15 +743,11 @@ template <typename N>
 std::shared_ptr<N> new_node() { return std::shared_ptr<N>(new N(), torch::autograd::deleteNode); }
 bool differentiated(const Tensor& logits) { return at::GradMode::is_enabled() && logits.requires_grad(); }
 void need_constant(const Tensor& t, const char* what) {
-  TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && t.requires_grad()), "d3pm_mi355x: ", what, " is a constant of this loss and must not require a gradient (detach it)");
+  TORCH_CHECK_VALUE(!(t.defined() && at::GradMode::is_enabled() && t.requires_grad()), "d3pm_mi355x: ", what, " is a constant of this loss and must not require a gradient (detach it)");
 }
-void need_constant(const OptTensor& t, const char* what) {
-  if (t.has_value() && t->defined()) need_constant(*t, what);
-}
-Tensor opt(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 
 // ---- log_softmax(logits / temperature) at the tokens, float32; stats [.., 4]: what its gradient is made from
-std::tuple<Tensor, Tensor> token_logprobs_run(const Tensor& logits, const Tensor& tokens, const OptTensor& mask,
+std::tuple<Tensor, Tensor> token_logprobs_run(const Tensor& logits, const Tensor& tokens, const Tensor& mask,
                                               double temperature, bool want_stats) {
   D3PM_GUARD(logits);
   auto v = logits_view(logits, tokens.sizes(), "tokens");
@@ -774,15 +775,13 @@ struct TokenLogprobsBackward : public ObjectiveNode {
     token_grad_run(logits, s[0], temperature, s[1], upstream, true, false, dz);
   }
 };
-Tensor token_logprobs(const Tensor& logits, const Tensor& tokens, const OptTensor& mask, double temperature) {
-  return std::get<0>(token_logprobs_run(logits, tokens, mask, temperature, false));
-}
-Tensor token_logprobs_autograd(const Tensor& logits, const Tensor& tokens, const OptTensor& mask, double temperature) {
+Tensor token_logprobs(const Tensor& logits, const Tensor& tokens_, const OptTensor& mask_, double temperature) {
   const bool want = differentiated(logits);
-  Tensor lp, stats;
+  Tensor tokens, lp, stats;
   {
     at::AutoDispatchBelowADInplaceOrView below;
-    std::tie(lp, stats) = token_logprobs_run(logits, tokens, mask, temperature, want);
+    tokens = dense(tokens_);
+    std::tie(lp, stats) = token_logprobs_run(logits, tokens, dense(opt(mask_)), temperature, want);
   }
   if (want) {
     auto node = new_node<TokenLogprobsBackward>();
@@ -794,71 +793,63 @@ Tensor token_logprobs_autograd(const Tensor& logits, const Tensor& tokens, const
 }
 
 // ---- distillation from a teacher's top logits
-struct Teacher { int dtype, index_bytes, k; };
-Teacher check_teacher(const Tensor& tl, const Tensor& ti, const Tensor& z) {
-  need_device(tl, "teacher_logits"); need_device(ti, "teacher_index");
-  need_same_device(tl, z, "teacher_logits"); need_same_device(ti, z, "teacher_index");
-  need_same_shape(tl, ti, "teacher_logits and teacher_index");
-  const int64_t k = tl.dim() ? tl.size(-1) : 0;
-  TORCH_CHECK_VALUE(z.dim() >= 2 && tl.dim() == z.dim() &&
-                        tl.sizes().slice(0, z.dim() - 1) == z.sizes().slice(0, z.dim() - 1),
-                    "d3pm_mi355x: teacher_logits must be [.., k] over the logits' positions, got ", tl.sizes(), " for ",
-                    z.sizes());
-  TORCH_CHECK_VALUE(k >= 1 && k <= 256, "d3pm_mi355x: the teacher's lists have ", k, " entries, need 1 .. 256");
-  return {float_dtype(tl, "teacher_logits"), tok_bytes(ti, "teacher_index"), (int)k};
-}
 struct DistillArgs { double temperature, out_scale; };
-// loss and per may be null (the gradient alone, times upstream), dz too (no gradient)
-void distill_run(const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_index, const OptTensor& mask,
+// loss and per may be null (the gradient alone, times upstream), dz too (no gradient); ws: the loss call's workspace
+void distill_run(const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_index, const Tensor& mask,
                  const DistillArgs& args, const float* upstream, bool only_if_rescaled, Tensor* loss, Tensor* per,
-                 const Tensor& dz) {
+                 const Tensor& dz, Tensor& ws) {
   D3PM_GUARD(logits);
-  const Teacher t = check_teacher(teacher_logits, teacher_index, logits);
-  auto v = logits_view(logits, logits.sizes().slice(0, logits.dim() - 1), "the teacher's positions");
+  const auto rows = logits.sizes().slice(0, std::max<int64_t>(logits.dim(), 1) - 1);
+  auto v = logits_view(logits, rows, "the teacher's positions");
+  need_device(teacher_logits, "teacher_logits");
+  need_same_device(teacher_logits, logits, "teacher_logits");
+  need_same_shape(teacher_logits, teacher_index, "teacher_logits and teacher_index");
+  TORCH_CHECK_VALUE(teacher_logits.dim() == logits.dim() && teacher_logits.sizes().slice(0, logits.dim() - 1) == rows,
+                    "d3pm_mi355x: teacher_logits must be [.., k] over the logits' positions, got ",
+                    teacher_logits.sizes(), " for ", logits.sizes());
+  const int64_t k = teacher_logits.size(-1);
+  TORCH_CHECK_VALUE(k >= 1 && k <= 256, "d3pm_mi355x: the teacher's lists have ", k, " entries, need 1 .. 256");
+  const int t_dtype = float_dtype(teacher_logits, "teacher_logits");
+  const int i_bytes = token_bytes(teacher_index, logits, "teacher_index");
+  const uint8_t* m = mask_ptr(mask, rows, logits);
   if (loss) {
     auto fo = logits.options().dtype(at::kFloat);
     *loss = at::empty({}, fo);
-    *per = at::empty(logits.sizes().slice(0, logits.dim() - 1), fo);
+    *per = at::empty(rows, fo);
+    ws = objective_workspace(v.desc, logits);
   }
-  size_t wsb;
-  Tensor ws = objective_workspace(v.desc, logits, &wsb);
-  check_rc(d3pm_topk_distill_loss(&v.desc, teacher_logits.data_ptr(), t.dtype, teacher_index.data_ptr(), t.index_bytes,
-                                  t.k, mask_ptr(mask, logits.sizes().slice(0, logits.dim() - 1), logits),
-                                  (float)args.temperature, (float)args.out_scale, upstream, only_if_rescaled,
+  check_rc(d3pm_topk_distill_loss(&v.desc, teacher_logits.data_ptr(), t_dtype, teacher_index.data_ptr(), i_bytes, (int)k,
+                                  m, (float)args.temperature, (float)args.out_scale, upstream, only_if_rescaled,
                                   loss ? loss->data_ptr<float>() : nullptr, per ? per->data_ptr<float>() : nullptr,
-                                  dz.defined() ? dz.data_ptr() : nullptr, ws.data_ptr(), wsb, stream()));
+                                  dz.defined() ? dz.data_ptr() : nullptr, ws.data_ptr(), ws.nbytes(), stream()));
 }
 struct DistillBackward : public ObjectiveNode {
   DistillArgs args;
   std::string name() const override { return "TopKDistillLoss"; }
   void fill(const Tensor& logits, const std::vector<Tensor>& s, const Tensor& upstream, bool only, Tensor& dz) override {
-    distill_run(logits, s[0], s[1], s[2], args, upstream_ptr(upstream, logits), only, nullptr, nullptr, dz);
+    Tensor ws = s[3];
+    distill_run(logits, s[0], s[1], s[2], args, upstream_ptr(upstream, logits), only, nullptr, nullptr, dz, ws);
   }
 };
 // (loss [], per_token)
-std::tuple<Tensor, Tensor> topk_distill_loss(const Tensor& logits, const Tensor& teacher_logits,
-                                             const Tensor& teacher_index, const OptTensor& mask, double temperature,
+std::tuple<Tensor, Tensor> topk_distill_loss(const Tensor& logits, const Tensor& teacher_logits_,
+                                             const Tensor& teacher_index_, const OptTensor& mask_, double temperature,
                                              double out_scale) {
-  Tensor loss, per;
-  distill_run(logits, teacher_logits, teacher_index, mask, {temperature, out_scale}, nullptr, false, &loss, &per, Tensor());
-  return {loss, per};
-}
-std::tuple<Tensor, Tensor> topk_distill_loss_autograd(const Tensor& logits, const Tensor& teacher_logits,
-                                                      const Tensor& teacher_index, const OptTensor& mask,
-                                                      double temperature, double out_scale) {
-  need_constant(teacher_logits, "teacher_logits");
+  need_constant(teacher_logits_, "teacher_logits");
   const bool want = differentiated(logits);
-  Tensor loss, per, dz;
+  const DistillArgs args{temperature, out_scale};
+  Tensor teacher_logits, teacher_index, mask, loss, per, dz, ws;
   {
     at::AutoDispatchBelowADInplaceOrView below;
+    teacher_logits = dense(teacher_logits_); teacher_index = dense(teacher_index_); mask = dense(opt(mask_));
     if (want) dz = grad_buffer(logits);
-    distill_run(logits, teacher_logits, teacher_index, mask, {temperature, out_scale}, nullptr, false, &loss, &per, dz);
+    distill_run(logits, teacher_logits, teacher_index, mask, args, nullptr, false, &loss, &per, dz, ws);
   }
   if (want) {
     auto node = new_node<DistillBackward>();
-    node->save(logits, {teacher_logits, teacher_index, opt(mask)});
+    node->save(logits, {teacher_logits, teacher_index, mask, ws});
     node->dz_ = std::move(dz);
-    node->args = {temperature, out_scale};
+    node->args = args;
     torch::autograd::set_history(loss, node);
   }
   return {loss, per};
@@ -867,68 +858,60 @@ std::tuple<Tensor, Tensor> topk_distill_loss_autograd(const Tensor& logits, cons
 // ---- clipped policy loss with a KL term
 struct PolicyArgs { double temperature, clip_low, clip_high, kl_coeff, out_scale; };
 void policy_run(const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs, const Tensor& advantages,
-                const OptTensor& ref_logprobs, const OptTensor& mask, const PolicyArgs& args, const float* upstream,
-                bool only_if_rescaled, Tensor* loss, Tensor* lp, const Tensor& dz) {
+                const Tensor& ref_logprobs, const Tensor& mask, const PolicyArgs& args, const float* upstream,
+                bool only_if_rescaled, Tensor* loss, Tensor* lp, const Tensor& dz, Tensor& ws) {
   D3PM_GUARD(logits);
   auto v = logits_view(logits, tokens.sizes(), "tokens");
+  const int t_bytes = token_bytes(tokens, logits, "tokens");
   const float* old_lp = row_f32(old_logprobs, tokens, logits, "old_logprobs and tokens");
   const bool per_seq = advantages.dim() == 1 && tokens.dim() > 1;
-  if (per_seq) {
-    need_numel(advantages, tokens.size(0), "advantages (one per sequence)");
-    need_same_device(advantages, logits, "advantages");
-  } else need_same_shape(advantages, tokens, "advantages and tokens");
+  if (per_seq) need_numel(advantages, tokens.size(0), "advantages (one per sequence)");
+  else need_same_shape(advantages, tokens, "advantages and tokens");
   need_same_device(advantages, logits, "advantages");
-  const float* ref = ref_logprobs.has_value() && ref_logprobs->defined()
-                         ? row_f32(*ref_logprobs, tokens, logits, "ref_logprobs and tokens") : nullptr;
+  const float* adv = f32(advantages, "advantages");
+  const float* ref = ref_logprobs.defined() ? row_f32(ref_logprobs, tokens, logits, "ref_logprobs and tokens") : nullptr;
+  const uint8_t* m = mask_ptr(mask, tokens.sizes(), logits);
   if (loss) {
     auto fo = logits.options().dtype(at::kFloat);
     *loss = at::empty({}, fo);
     *lp = at::empty(tokens.sizes(), fo);
+    ws = objective_workspace(v.desc, logits);
   }
-  size_t wsb;
-  Tensor ws = objective_workspace(v.desc, logits, &wsb);
-  check_rc(d3pm_policy_loss(&v.desc, tokens.data_ptr(), token_bytes(tokens, logits, "tokens"), old_lp,
-                            f32(advantages, "advantages"), per_seq, ref, mask_ptr(mask, tokens.sizes(), logits),
-                            (float)args.temperature, (float)args.clip_low, (float)args.clip_high, (float)args.kl_coeff,
-                            (float)args.out_scale, upstream, only_if_rescaled, loss ? loss->data_ptr<float>() : nullptr,
+  check_rc(d3pm_policy_loss(&v.desc, tokens.data_ptr(), t_bytes, old_lp, adv, per_seq, ref, m, (float)args.temperature,
+                            (float)args.clip_low, (float)args.clip_high, (float)args.kl_coeff, (float)args.out_scale,
+                            upstream, only_if_rescaled, loss ? loss->data_ptr<float>() : nullptr,
                             lp ? lp->data_ptr<float>() : nullptr, dz.defined() ? dz.data_ptr() : nullptr, ws.data_ptr(),
-                            wsb, stream()));
+                            ws.nbytes(), stream()));
 }
 struct PolicyBackward : public ObjectiveNode {
   PolicyArgs args;
   std::string name() const override { return "PolicyLoss"; }
   void fill(const Tensor& logits, const std::vector<Tensor>& s, const Tensor& upstream, bool only, Tensor& dz) override {
-    policy_run(logits, s[0], s[1], s[2], s[3], s[4], args, upstream_ptr(upstream, logits), only, nullptr, nullptr, dz);
+    Tensor ws = s[5];
+    policy_run(logits, s[0], s[1], s[2], s[3], s[4], args, upstream_ptr(upstream, logits), only, nullptr, nullptr, dz, ws);
   }
 };
 // (loss [], logprobs)
-std::tuple<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs,
-                                       const Tensor& advantages, const OptTensor& ref_logprobs, const OptTensor& mask,
+std::tuple<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& tokens_, const Tensor& old_logprobs_,
+                                       const Tensor& advantages_, const OptTensor& ref_logprobs_, const OptTensor& mask_,
                                        double temperature, double clip_low, double clip_high, double kl_coeff,
                                        double out_scale) {
-  Tensor loss, lp;
-  policy_run(logits, tokens, old_logprobs, advantages, ref_logprobs, mask,
-             {temperature, clip_low, clip_high, kl_coeff, out_scale}, nullptr, false, &loss, &lp, Tensor());
-  return {loss, lp};
-}
-std::tuple<Tensor, Tensor> policy_loss_autograd(const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs,
-                                                const Tensor& advantages, const OptTensor& ref_logprobs,
-                                                const OptTensor& mask, double temperature, double clip_low,
-                                                double clip_high, double kl_coeff, double out_scale) {
-  need_constant(old_logprobs, "old_logprobs");
-  need_constant(advantages, "advantages");
-  need_constant(ref_logprobs, "ref_logprobs");
+  need_constant(old_logprobs_, "old_logprobs");
+  need_constant(advantages_, "advantages");
+  need_constant(opt(ref_logprobs_), "ref_logprobs");
   const bool want = differentiated(logits);
   const PolicyArgs args{temperature, clip_low, clip_high, kl_coeff, out_scale};
-  Tensor loss, lp, dz;
+  Tensor tokens, old_logprobs, advantages, ref_logprobs, mask, loss, lp, dz, ws;
   {
     at::AutoDispatchBelowADInplaceOrView below;
+    tokens = dense(tokens_); old_logprobs = dense_f32(old_logprobs_); advantages = dense_f32(advantages_);
+    ref_logprobs = dense_f32(opt(ref_logprobs_)); mask = dense(opt(mask_));
     if (want) dz = grad_buffer(logits);
-    policy_run(logits, tokens, old_logprobs, advantages, ref_logprobs, mask, args, nullptr, false, &loss, &lp, dz);
+    policy_run(logits, tokens, old_logprobs, advantages, ref_logprobs, mask, args, nullptr, false, &loss, &lp, dz, ws);
   }
   if (want) {
     auto node = new_node<PolicyBackward>();
-    node->save(logits, {tokens, old_logprobs, advantages, opt(ref_logprobs), opt(mask)});
+    node->save(logits, {tokens, old_logprobs, advantages, ref_logprobs, mask, ws});
     node->dz_ = std::move(dz);
     node->args = args;
     torch::autograd::set_history(loss, node);
@@ -937,25 +920,6 @@ std::tuple<Tensor, Tensor> policy_loss_autograd(const Tensor& logits, const Tens
 }
 
 // ---- preference loss of the pairs (p, p + B / 2)
-void preference_run(const Tensor& logits, const Tensor& tokens, const OptTensor& ref_logprobs, const OptTensor& mask,
-                    double beta, double label_smoothing, bool average, double out_scale, Tensor* loss, Tensor* rewards,
-                    Tensor* stats, const Tensor& dz) {
-  D3PM_GUARD(logits);
-  auto v = logits_view(logits, tokens.sizes(), "tokens");
-  const float* ref = ref_logprobs.has_value() && ref_logprobs->defined()
-                         ? row_f32(*ref_logprobs, tokens, logits, "ref_logprobs and tokens") : nullptr;
-  auto fo = logits.options().dtype(at::kFloat);
-  *loss = at::empty({}, fo);
-  *rewards = at::empty({v.desc.B}, fo);
-  *stats = at::empty({tokens.numel(), 4}, fo);
-  size_t wsb;
-  Tensor ws = objective_workspace(v.desc, logits, &wsb);
-  check_rc(d3pm_preference_loss(&v.desc, tokens.data_ptr(), token_bytes(tokens, logits, "tokens"), ref,
-                                mask_ptr(mask, tokens.sizes(), logits), (float)beta, (float)label_smoothing, average,
-                                (float)out_scale, loss->data_ptr<float>(), rewards->data_ptr<float>(),
-                                stats->data_ptr<float>(), dz.defined() ? dz.data_ptr() : nullptr, ws.data_ptr(), wsb,
-                                stream()));
-}
 struct PreferenceBackward : public ObjectiveNode {
   std::string name() const override { return "PreferenceLoss"; }
   void fill(const Tensor& logits, const std::vector<Tensor>& s, const Tensor& upstream, bool only, Tensor& dz) override {
@@ -963,23 +927,31 @@ struct PreferenceBackward : public ObjectiveNode {
   }
 };
 // (loss [], rewards [B])
-std::tuple<Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& tokens, const OptTensor& ref_logprobs,
-                                           const OptTensor& mask, double beta, double label_smoothing, bool average,
+std::tuple<Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& tokens_, const OptTensor& ref_logprobs_,
+                                           const OptTensor& mask_, double beta, double label_smoothing, bool average,
                                            double out_scale) {
-  Tensor loss, rewards, stats;
-  preference_run(logits, tokens, ref_logprobs, mask, beta, label_smoothing, average, out_scale, &loss, &rewards, &stats, Tensor());
-  return {loss, rewards};
-}
-std::tuple<Tensor, Tensor> preference_loss_autograd(const Tensor& logits, const Tensor& tokens,
-                                                    const OptTensor& ref_logprobs, const OptTensor& mask, double beta,
-                                                    double label_smoothing, bool average, double out_scale) {
-  need_constant(ref_logprobs, "ref_logprobs");
+  need_constant(opt(ref_logprobs_), "ref_logprobs");
   const bool want = differentiated(logits);
-  Tensor loss, rewards, stats, dz;
+  Tensor tokens, loss, rewards, stats, dz;
   {
     at::AutoDispatchBelowADInplaceOrView below;
+    D3PM_GUARD(logits);
+    tokens = dense(tokens_);
+    const Tensor ref_logprobs = dense_f32(opt(ref_logprobs_)), mask = dense(opt(mask_));
+    auto v = logits_view(logits, tokens.sizes(), "tokens");
+    const int t_bytes = token_bytes(tokens, logits, "tokens");
+    const float* ref = ref_logprobs.defined() ? row_f32(ref_logprobs, tokens, logits, "ref_logprobs and tokens") : nullptr;
+    const uint8_t* m = mask_ptr(mask, tokens.sizes(), logits);
+    auto fo = logits.options().dtype(at::kFloat);
+    loss = at::empty({}, fo);
+    rewards = at::empty({v.desc.B}, fo);
+    stats = at::empty({tokens.numel(), 4}, fo);
     if (want) dz = grad_buffer(logits);
-    preference_run(logits, tokens, ref_logprobs, mask, beta, label_smoothing, average, out_scale, &loss, &rewards, &stats, dz);
+    const Tensor ws = objective_workspace(v.desc, logits);
+    check_rc(d3pm_preference_loss(&v.desc, tokens.data_ptr(), t_bytes, ref, m, (float)beta, (float)label_smoothing,
+                                  average, (float)out_scale, loss.data_ptr<float>(), rewards.data_ptr<float>(),
+                                  stats.data_ptr<float>(), want ? dz.data_ptr() : nullptr, ws.data_ptr(), ws.nbytes(),
+                                  stream()));
   }
   if (want) {
     auto node = new_node<PreferenceBackward>();
@@ -1076,8 +1048,8 @@ TORCH_LIBRARY_IMPL(d3pm_mi355x, CUDA, m) {
 
 // the fine-tuning objectives bring their own autograd nodes
 TORCH_LIBRARY_IMPL(d3pm_mi355x, AutogradCUDA, m) {
-  m.impl("token_logprobs", token_logprobs_autograd);
-  m.impl("topk_distill_loss", topk_distill_loss_autograd);
-  m.impl("policy_loss", policy_loss_autograd);
-  m.impl("preference_loss", preference_loss_autograd);
+  m.impl("token_logprobs", token_logprobs);
+  m.impl("topk_distill_loss", topk_distill_loss);
+  m.impl("policy_loss", policy_loss);
+  m.impl("preference_loss", preference_loss);
 }

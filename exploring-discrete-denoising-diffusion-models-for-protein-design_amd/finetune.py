@@ -27,29 +27,17 @@ from . import _lib
 from ._ops import ops
 
 
-def _tokens(x: torch.Tensor) -> torch.Tensor:
-    if x.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"tokens and classes must be int32 or int64, got {x.dtype}")
-    return x.contiguous()
-
-
-def _float32(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return None if x is None else x.to(torch.float32).contiguous()
-
-
-def _mask(mask: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    if mask is None:
-        return None
-    if mask.dtype != torch.bool:
-        raise TypeError(f"mask must be bool, got {mask.dtype}")
-    return mask.contiguous()
-
-
 def _temperature(x: float) -> float:
     x = float(x)
     if not 1e-6 <= x <= 1e6:
         raise ValueError(f"temperature must be in [1e-6, 1e6], got {x}")
     return x
+
+
+def _keep(module: torch.nn.Module, **values) -> None:
+    """Plain attributes of a module.  They are no parameters, and ``Module.__setattr__``'s search for them is a third of
+    the host time of a forward call."""
+    module.__dict__.update(values)
 
 
 def _finite(x: float, what: str) -> float:
@@ -64,8 +52,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, mask: Optional[to
     """``log_softmax(logits / temperature)`` at ``tokens`` (logits ``[..., V]``, tokens ``[...]``), float32 of the
     tokens' shape, 0 where ``mask`` is false; differentiable by the logits."""
     _lib.require_device(logits, tokens, mask)
-    tokens, mask, temperature = _tokens(tokens), _mask(mask), _temperature(temperature)
-    return ops.token_logprobs(logits, tokens, mask, temperature)
+    return ops.token_logprobs(logits, tokens, mask, _temperature(temperature))
 
 
 class TopKDistillLoss(torch.nn.Module):
@@ -79,13 +66,13 @@ class TopKDistillLoss(torch.nn.Module):
 
     def __init__(self, temperature: float = 1.0):
         super().__init__()
-        self.temperature = _temperature(temperature)
-        self.per_token = None
+        _keep(self, temperature=_temperature(temperature), per_token=None)
 
     def forward(self, logits, teacher_logits, teacher_index, mask=None, out_scale=1.0):
         _lib.require_device(logits, teacher_logits, teacher_index, mask)
-        loss, self.per_token = ops.topk_distill_loss(logits, teacher_logits.contiguous(), _tokens(teacher_index),
-                                                     _mask(mask), self.temperature, _finite(out_scale, "out_scale"))
+        loss, per_token = ops.topk_distill_loss(logits, teacher_logits, teacher_index, mask, self.temperature,
+                                                _finite(out_scale, "out_scale"))
+        _keep(self, per_token=per_token)
         return loss
 
 
@@ -100,20 +87,19 @@ class PolicyLoss(torch.nn.Module):
 
     def __init__(self, clip_low: float = 0.2, clip_high: float = 0.2, kl_coeff: float = 0.0, temperature: float = 1.0):
         super().__init__()
-        self.clip_low, self.clip_high = _finite(clip_low, "clip_low"), float(clip_high)
-        if not (0.0 <= self.clip_low <= 1.0 and self.clip_high >= 0.0):
+        clip_low, clip_high = _finite(clip_low, "clip_low"), float(clip_high)
+        if not (0.0 <= clip_low <= 1.0 and clip_high >= 0.0):
             raise ValueError(f"clip range [1 - {clip_low}, 1 + {clip_high}]: need 0 <= clip_low <= 1, clip_high >= 0")
-        self.kl_coeff = _finite(kl_coeff, "kl_coeff")
-        self.temperature = _temperature(temperature)
-        self.logprobs = None
+        _keep(self, clip_low=clip_low, clip_high=clip_high, kl_coeff=_finite(kl_coeff, "kl_coeff"),
+              temperature=_temperature(temperature), logprobs=None)
 
     def forward(self, logits, tokens, old_logprobs, advantages, ref_logprobs=None, mask=None, out_scale=1.0):
         _lib.require_device(logits, tokens, old_logprobs, advantages, ref_logprobs, mask)
         if self.kl_coeff != 0.0 and ref_logprobs is None:
             raise ValueError("kl_coeff needs ref_logprobs")
-        loss, self.logprobs = ops.policy_loss(logits, _tokens(tokens), _float32(old_logprobs), _float32(advantages),
-                                              _float32(ref_logprobs), _mask(mask), self.temperature, self.clip_low,
-                                              self.clip_high, self.kl_coeff, _finite(out_scale, "out_scale"))
+        loss, logprobs = ops.policy_loss(logits, tokens, old_logprobs, advantages, ref_logprobs, mask, self.temperature,
+                                         self.clip_low, self.clip_high, self.kl_coeff, _finite(out_scale, "out_scale"))
+        _keep(self, logprobs=logprobs)
         return loss
 
 
@@ -129,14 +115,14 @@ class PreferenceLoss(torch.nn.Module):
 
     def __init__(self, beta: float = 0.1, label_smoothing: float = 0.0, average: bool = False):
         super().__init__()
-        self.beta, self.label_smoothing = _finite(beta, "beta"), _finite(label_smoothing, "label_smoothing")
-        if not 0.0 <= self.label_smoothing <= 1.0:
+        beta, label_smoothing = _finite(beta, "beta"), _finite(label_smoothing, "label_smoothing")
+        if not 0.0 <= label_smoothing <= 1.0:
             raise ValueError(f"label_smoothing must be in [0, 1], got {label_smoothing}")
-        self.average = bool(average)
-        self.rewards = None
+        _keep(self, beta=beta, label_smoothing=label_smoothing, average=bool(average), rewards=None)
 
     def forward(self, logits, tokens, ref_logprobs=None, mask=None, out_scale=1.0):
         _lib.require_device(logits, tokens, ref_logprobs, mask)
-        loss, self.rewards = ops.preference_loss(logits, _tokens(tokens), _float32(ref_logprobs), _mask(mask), self.beta,
-                                                 self.label_smoothing, self.average, _finite(out_scale, "out_scale"))
+        loss, rewards = ops.preference_loss(logits, tokens, ref_logprobs, mask, self.beta, self.label_smoothing,
+                                            self.average, _finite(out_scale, "out_scale"))
+        _keep(self, rewards=rewards)
         return loss

@@ -441,8 +441,9 @@ int d3pm_token_grad(const d3pm_logits* z, const void* tokens, int tok_bytes, flo
  *   [B,L,k], 1 <= k <= 256
  *   per_token float32 [B,L]: temperature^2 KL (may be NULL)
  *   dlogits may be NULL (no gradient).  upstream (may be NULL) multiplies the
- *   gradient; loss == NULL: the call makes the gradient alone, and with
- *   only_if_rescaled leaves dlogits as it is if *upstream is 1. */
+ *   gradient; loss == NULL: the call makes the gradient alone (workspace: that
+ *   of the loss call, as it left it), and with only_if_rescaled leaves dlogits
+ *   as it is if *upstream is 1. */
 int d3pm_topk_distill_loss(const d3pm_logits* z, const void* teacher_logits, int teacher_dtype,
                            const void* teacher_index, int index_bytes, int k, const uint8_t* mask, float temperature,
                            float out_scale, const float* upstream, int only_if_rescaled, float* loss, float* per_token,
