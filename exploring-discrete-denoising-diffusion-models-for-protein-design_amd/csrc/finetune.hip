@@ -193,8 +193,8 @@ __device__ __forceinline__ TokenOut token_head(const RowArgs& a, int n, float zy
   return o;
 }
 // c (1 - p) of the token: S less its own exponential is exact where that is the row's largest
-__device__ __forceinline__ float token_grad(float c, float zy_m, float S, float inv_S, float c_hi, float c_lo) {
-  return c * (S - exp_d(zy_m, c_hi, c_lo)) * inv_S;
+__device__ __forceinline__ float token_grad(float c, float zy_m, float S, float c_hi, float c_lo) {
+  return c * ((S - exp_d(zy_m, c_hi, c_lo)) / S);
 }
 
 // ------------------------------------------------------------------------------------- one pass, rows in registers
@@ -207,6 +207,20 @@ struct Shape {
   static constexpr int ROWS = WG / G;
   static constexpr int GL = G < 64 ? G : 64;        // lanes that a teacher's list is spread over
 };
+
+// The pieces of a row as a buffer resource, for the shapes whose row is the same for a whole wave: an access beyond the
+// last piece reads 0 or writes nothing, so neither loads nor stores need a branch.  (The whole offset goes into the lane
+// offset: the range check compares that with the size less the scalar offset, which must not pass the size.)
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+__device__ __forceinline__ Rsrc pieces_of(const void* body, int full) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)body, 0, full * 16, 0x00027000);
+}
+__device__ __forceinline__ u32x4 load_piece(Rsrc r, int lane, int j, int G) {
+  return __builtin_amdgcn_raw_buffer_load_b128(r, (j * G + lane) * 16, 0, 0);
+}
+__device__ __forceinline__ void store_piece(Rsrc r, int lane, int j, int G, u32x4 v) {
+  __builtin_amdgcn_raw_buffer_store_b128(v, r, (j * G + lane) * 16, 0, 2 /* non-temporal */);
+}
 
 // Counted positions of a mask, by a whole workgroup of up to 1024: every thread gets the sum.
 __device__ __forceinline__ int count_mask(const uint8_t* mask, int N, int* lds) {
@@ -274,12 +288,23 @@ __device__ __forceinline__ void fresh(u32x4 (&v)[NV]) {
   for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(v[j]));
 }
 
-// m and S of the group's row from its lanes' values: a wave takes its exponentials against its own maximum, so a
-// row of several waves needs one exchange, not two.  The reference is kept off -inf (a wave that has only padding).
+// The places of v that hold no piece of the row hold -inf.
 template <typename T, int G, int NV>
-__device__ __forceinline__ void row_stats(u32x4 (&v)[NV], float edge, const RowArgs& a, float2* red, int wave,
-                                          float& m, float& S) {
-  constexpr int GL = Shape<G>::GL;
+__device__ __forceinline__ void mask_pieces(u32x4 (&v)[NV], int full, int g) {
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    if ((j + 1) * G > full) {
+      const bool in = j * G + g < full;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[j][i] = in ? v[j][i] : T::NEG_INF;
+    }
+}
+
+// m and S of the group's row from its lanes' values, in two steps: of the wave (a wave takes its exponentials against its
+// own maximum, so a row of several waves needs one exchange, not two; the reference is kept off -inf, for a wave that
+// has only padding), and of the row.  KEEP: the pieces are needed again, for the gradient.
+template <typename T, int GL, int NV, bool KEEP>
+__device__ __forceinline__ float2 wave_stats(u32x4 (&v)[NV], float edge, const RowArgs& a) {
   float f[T::E];
   float mx = edge;
 #pragma unroll
@@ -300,35 +325,54 @@ __device__ __forceinline__ void row_stats(u32x4 (&v)[NV], float edge, const RowA
       s1 += exp_d(f[e + 1] - mx, a.c_hi, a.c_lo);
     }
   }
-  fresh<NV>(v);
-  const float s = group_sum<GL>(s0 + s1);
-  if constexpr (G <= 64) {
-    m = mx;
-    S = s;
-  } else {
-    if ((threadIdx.x & 63) == 0) red[wave] = make_float2(mx, s);
-    __syncthreads();
-    m = -FLT_MAX;
+  if constexpr (KEEP) fresh<NV>(v);
+  return make_float2(mx, group_sum<GL>(s0 + s1));
+}
+template <int WAVES>
+__device__ __forceinline__ float2 join_stats(const float2* red, const RowArgs& a) {
+  float m = -FLT_MAX;
 #pragma unroll
-    for (int w = 0; w < G / 64; ++w) m = fmaxf(m, red[w].x);
-    double sum = 0.0;
+  for (int w = 0; w < WAVES; ++w) m = fmaxf(m, red[w].x);
+  double sum = 0.0;
 #pragma unroll
-    for (int w = 0; w < G / 64; ++w) sum += (double)(red[w].y * exp_d(red[w].x - m, a.c_hi, a.c_lo));
-    S = (float)sum;
-  }
+  for (int w = 0; w < WAVES; ++w) sum += (double)(red[w].y * exp_d(red[w].x - m, a.c_hi, a.c_lo));
+  return make_float2(m, (float)sum);
 }
 
-// The teacher's list of a row.  Loaded before the row's statistics are known: the kept entries' classes and
-// exponentials go to LDS (class -1: not kept), their sums stay with the lanes.
-struct List { int* idx; float* e; float St, A; int kept; };
-template <int GL>
+// The teacher's list of a row, spread over GL lanes of one wave: the kept entries' classes (-1: not kept), exponentials
+// and student logits go to LDS, padded to whole fours, the sums stay with the lanes.
+//
+// A class may be listed twice.  Every kept entry writes its number to its class' place in a table of bytes and looks what
+// is there afterwards: its own number everywhere means that no class is.  (In a table smaller than the alphabet two
+// classes may share a place; that costs the search of list_grad, no more.)  65536 rows of 100 float32 classes with 64
+// entries: 43 us, 82 with the search for every entry.  Rows of 16 pieces a lane have no registers left for it (8192 rows
+// of 131072 bf16 classes: 816 us without the table, 853 with it) and search.
+constexpr int TAGS = 16384;             // bytes of a workgroup's tables: every class of a row of up to 64 lanes has a place
+struct List {
+  int* idx; float* e; float* z; uint8_t* tag; int tag_mask;
+  float St, A; int kept, twice;
+};
+__host__ __device__ constexpr int list_pad(int k) { return (k + 3) & ~3; }
+constexpr size_t list_bytes(int rows, int k, bool tagged) { return (tagged ? TAGS : 0) + (size_t)rows * list_pad(k) * 12; }
+template <bool TAGGED>
+__device__ __forceinline__ List list_place(char* lds, int rows, int slot, int k) {
+  const int pad = list_pad(k);
+  float* at = (float*)(lds + (TAGGED ? TAGS : 0));
+  return List{(int*)at + slot * pad, at + (rows + slot) * pad, at + (2 * rows + slot) * pad,
+              (uint8_t*)lds + slot * (TAGS / rows), TAGS / rows - 1, 0.0f, 0.0f, 0, TAGGED ? 0 : 1};
+}
+template <int GL, bool TAGGED>
 __device__ __forceinline__ void list_load(const RowArgs& a, int n, int g, List& l) {
   const long at = (long)n * a.k;
   float mt = -INFINITY;
   int kept = 0;
-  for (int i = g; i < a.k; i += GL) {
-    const float t = get_any(a.t_logits, a.t_dtype, at + i);
-    int c = get_int(a.t_index, a.t_index_bytes, at + i);
+  for (int i = g; i < list_pad(a.k); i += GL) {
+    float t = -INFINITY;
+    int c = -1;
+    if (i < a.k) {
+      t = get_any(a.t_logits, a.t_dtype, at + i);
+      c = get_int(a.t_index, a.t_index_bytes, at + i);
+    }
     if (c < 0 || t == -INFINITY) c = -1;
     else {
       c = min(c, a.V - 1);
@@ -337,44 +381,61 @@ __device__ __forceinline__ void list_load(const RowArgs& a, int n, int g, List& 
     }
     l.idx[i] = c;
     l.e[i] = t;
+    if (TAGGED && c >= 0) l.tag[c & l.tag_mask] = (uint8_t)i;
   }
+  if constexpr (TAGGED) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   mt = fmaxf(group_max<GL>(mt), -FLT_MAX);          // a NaN entry alone leaves -inf here: its exponential is NaN
   l.kept = (int)group_max<GL>((float)kept);
   float St = 0.0f, A = 0.0f;
-  for (int i = g; i < a.k; i += GL) {
+  int twice = 0;
+  for (int i = g; i < list_pad(a.k); i += GL) {
     const float d = l.e[i] - mt;
-    const float e = l.idx[i] < 0 ? 0.0f : exp_d(d, a.c_hi, a.c_lo);
+    const int c = l.idx[i];
+    const float e = c < 0 ? 0.0f : exp_d(d, a.c_hi, a.c_lo);
+    if (TAGGED && c >= 0 && l.tag[c & l.tag_mask] != i) twice = 1;
     St += e;
     if (e != 0.0f) A = fmaf(e, d * a.inv_tau, A);
     l.e[i] = e;
   }
   l.St = group_sum<GL>(St);
   l.A = group_sum<GL>(A);
+  if constexpr (TAGGED) l.twice = (int)group_max<GL>((float)twice);
 }
 // tau^2 KL(teacher || student) of the row
 template <typename T, int GL>
 __device__ __forceinline__ float list_loss(const RowArgs& a, const char* row, int g, const List& l, float m, float S) {
   float Bs = 0.0f;
   for (int i = g; i < a.k; i += GL) {
-    const float e = l.e[i];
-    if (e != 0.0f) Bs = fmaf(e, (T::get(row, l.idx[i]) - m) * a.inv_tau, Bs);
+    const float e = l.e[i], z = T::get(row, max(l.idx[i], 0));
+    l.z[i] = z;
+    if (e != 0.0f) Bs = fmaf(e, (z - m) * a.inv_tau, Bs);
   }
   Bs = group_sum<GL>(Bs);
   const float tau = 1.0f / a.inv_tau;
   return l.kept ? tau * tau * ((l.A - Bs) / l.St - logf(l.St) + logf(S)) : 0.0f;
 }
-// gradient elements of the kept classes, c (q - p), over the -c p that the row's pieces hold there; a class listed
-// twice gets the sum of its entries, in the list's order, from each of them
-template <typename T, int GL>
-__device__ __forceinline__ void list_grad(const RowArgs& a, const char* row, char* out, int g, const List& l, float m,
-                                          float inv_S, float c) {
-  const float inv_St = 1.0f / l.St;
+// Gradient elements of the kept classes, c (q - p), over the -c p that the row's pieces hold there.  A class listed twice
+// gets the sum of its entries, in the list's order, from each of them.
+template <typename T, int GL, bool TAGGED>
+__device__ __forceinline__ void list_grad(const RowArgs& a, char* out, int g, const List& l, float m, float inv_S, float c) {
+  const float inv_St = rcp_acc(l.St);
   for (int i = g; i < a.k; i += GL) {
     const int cls = l.idx[i];
     if (cls < 0) continue;
-    float q = 0.0f;
-    for (int j = 0; j < a.k; ++j) q += l.idx[j] == cls ? l.e[j] : 0.0f;
-    const float p = exp_d(T::get(row, cls) - m, a.c_hi, a.c_lo) * inv_S;
+    float q = TAGGED ? l.e[i] : 0.0f;
+    if (!TAGGED || l.twice) {
+      q = 0.0f;
+#pragma unroll (TAGGED ? 1 : 4)
+      for (int j = 0; j < list_pad(a.k); j += 4) {
+        const int4 x = *(const int4*)(l.idx + j);
+        const float4 e = *(const float4*)(l.e + j);
+        q += x.x == cls ? e.x : 0.0f;
+        q += x.y == cls ? e.y : 0.0f;
+        q += x.z == cls ? e.z : 0.0f;
+        q += x.w == cls ? e.w : 0.0f;
+      }
+    }
+    const float p = exp_d(l.z[i] - m, a.c_hi, a.c_lo) * inv_S;
     T::put(out, cls, c * (q * inv_St - p));
   }
 }
@@ -389,19 +450,65 @@ __device__ __forceinline__ void zero_row(char* out, int V, int g, int G) {
   if (cut.has_edge(g)) T::put(out, cut.edge(g), 0.0f);
 }
 
-template <typename T, int G, int NV, bool DISTILL>
-__global__ __launch_bounds__(Shape<G>::WG) void k_rows(RowArgs a) {
+// scale exp((z - m) / tau) of a piece.  For the 16-bit types the scale goes into the exponent and the constant is one
+// float: 1e-6 of the value, against the 2^-12 and 2^-9 of their rounding, for 7.5 instructions instead of 9.5.
+struct Scale {
+  float scale, log2_abs;
+  uint32_t sign;                       // of both halves of a dword
+  __device__ __forceinline__ explicit Scale(float s)
+      : scale(s), log2_abs(__builtin_amdgcn_logf(fabsf(s))), sign(s < 0.0f ? 0x80008000u : 0u) {}
+};
+template <typename T, typename Args>
+__device__ __forceinline__ u32x4 grad_piece(u32x4 v, const Args& a, float m, const Scale& sc) {
+  float f[T::E];
+  T::unpack(v, f);
+  if constexpr (T::SIZE == 4) {
+#pragma unroll
+    for (int e = 0; e < T::E; ++e) f[e] = sc.scale * exp_d(f[e] - m, a.c_hi, a.c_lo);
+    return T::pack(f);
+  } else {
+#pragma unroll
+    for (int e = 0; e < T::E; ++e) f[e] = exp2_hw(fmaf(f[e] - m, a.c_hi, sc.log2_abs));
+    return T::pack(f) ^ sc.sign;
+  }
+}
+// The gradient pieces of a row from the pieces of its logits, and its end elements.
+template <typename T, int G, int NV, bool PEEL>
+__device__ __forceinline__ void grad_pieces(u32x4 (&v)[NV], float edge, const RowArgs& a, const Cut<T, PEEL>& cut,
+                                            char* out, int g, float m, float scale) {
+  char* body = out + cut.head * T::SIZE;
+  const Scale sc(scale);
+  if constexpr (G >= 64) {
+    const Rsrc to = pieces_of(body, cut.full);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) store_piece(to, g, j, G, grad_piece<T>(v[j], a, m, sc));
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (j * G + g < cut.full) store_piece<T>(body + j * (G * 16) + (uint32_t)g * 16u, grad_piece<T>(v[j], a, m, sc));
+  }
+  if (cut.has_edge(g)) T::put(out, cut.edge(g), scale * exp_d(edge - m, a.c_hi, a.c_lo));
+}
+
+// Waves of a SIMD that the registers are to leave room for: with 8 the small rows take 54 us instead of 57 (32 x 32 images,
+// 256 classes), the 8-piece ones gain 3 % with 6; the lists' registers would spill there (107 us with 4, 113 with 6).
+template <int G, int NV, bool DISTILL>
+constexpr int WAVES_PER_SIMD = G <= 64 ? (DISTILL ? 6 : 8) : NV == 8 && !DISTILL ? 6 : 4;
+template <typename T, int G, int NV, bool DISTILL, bool GRAD>
+__global__ __launch_bounds__(Shape<G>::WG)
+__attribute__((amdgpu_waves_per_eu(WAVES_PER_SIMD<G, NV, DISTILL>))) void k_rows(RowArgs a) {
   typedef Shape<G> Sh;
-  constexpr int E = T::E;
   constexpr bool PEEL = G >= 64;       // (a row of fewer lanes has no lane for every end element)
+  constexpr bool TAGGED = NV < 16;
   __shared__ float2 red[2][G > 64 ? G / 64 : 1];
   __shared__ int kept_flag[2];
+  __shared__ float list_sums[3];
   __shared__ double wg_sum[Sh::ROWS];
-  extern __shared__ char lists[];
+  __shared__ int counts[16];
+  extern __shared__ __align__(16) char lists[];
   if (a.only_if_rescaled && *a.upstream == 1.0f) return;
 
   const int g = threadIdx.x % G, slot = Sh::ROWS == 1 ? 0 : threadIdx.x / G, wave = threadIdx.x >> 6;
-  __shared__ int counts[16];
   const float w = row_weight(a, counts);
   double acc = 0.0;
   int phase = 0;
@@ -410,9 +517,9 @@ __global__ __launch_bounds__(Shape<G>::WG) void k_rows(RowArgs a) {
     int n = n0 + slot;
     if (Sh::ROWS > 1 && n >= a.N) break;
     if constexpr (G == 64) n = __builtin_amdgcn_readfirstlane(n);        // the row of a whole wave: scalar addresses
-    char* out = a.dz ? (char*)a.dz + (long)n * a.V * T::SIZE : nullptr;
+    char* out = GRAD ? (char*)a.dz + (long)n * a.V * T::SIZE : nullptr;
     if (a.mask && !a.mask[n]) {                      // not counted: nothing of its row is read
-      if (out) zero_row<T, PEEL>(out, a.V, g, G);
+      if constexpr (GRAD) zero_row<T, PEEL>(out, a.V, g, G);
       if (g == 0) {
         if (a.per_row) a.per_row[n] = 0.0f;
         if (a.stats) a.stats[n] = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
@@ -422,73 +529,84 @@ __global__ __launch_bounds__(Shape<G>::WG) void k_rows(RowArgs a) {
     const char* row = row_ptr(a, n, T::SIZE);
     const Cut<T, PEEL> cut(row, a.V);
     const char* body = row + cut.head * T::SIZE;
-    char* obody = out + cut.head * T::SIZE;
     u32x4 v[NV];
+    if constexpr (G >= 64) {
+      const Rsrc from = pieces_of(body, cut.full);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      v[j] = (u32x4){T::NEG_INF, T::NEG_INF, T::NEG_INF, T::NEG_INF};
-      if (j * G + g < cut.full) v[j] = *(const typename T::Raw*)(body + j * (G * 16) + (uint32_t)g * 16u);
+      for (int j = 0; j < NV; ++j) v[j] = load_piece(from, g, j, G);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        v[j] = (u32x4){T::NEG_INF, T::NEG_INF, T::NEG_INF, T::NEG_INF};
+        if (j * G + g < cut.full) v[j] = *(const typename T::Raw*)(body + j * (G * 16) + (uint32_t)g * 16u);
+      }
     }
     const float edge = cut.has_edge(g) ? T::get(row, cut.edge(g)) : -INFINITY;
-    float m, S;
+    // what the row's own arithmetic needs is on its way too
+    int y = 0;
+    float zy = 0.0f;
+    List l = list_place<TAGGED>(lists, Sh::ROWS, slot, a.k);
+    const bool lister = G <= 64 || wave == 0;        // a row of several waves: the first has the list
+    if constexpr (!DISTILL) {
+      y = min(max(get_int(a.tokens, a.tok_bytes, n), 0), a.V - 1);
+      zy = T::get(row, y);
+    } else if (lister) {
+      list_load<Sh::GL, TAGGED>(a, n, g, l);
+      if (G > 64 && g == 0) {
+        kept_flag[phase] = l.kept;
+        list_sums[0] = l.St;                          // (not carried in registers over the sweeps)
+        list_sums[1] = l.A;
+        if (TAGGED) list_sums[2] = (float)l.twice;
+      }
+    }
+    if constexpr (G >= 64) mask_pieces<T, G, NV>(v, cut.full, g);
+    float2 st = wave_stats<T, Sh::GL, NV, GRAD>(v, edge, a);
+    if constexpr (G > 64) {
+      if ((g & 63) == 0) red[phase][wave] = st;
+      __syncthreads();
+      st = join_stats<G / 64>(red[phase], a);
+    }
+    const float m = st.x, S = st.y;
 
     if constexpr (!DISTILL) {
-      const int y = min(max(get_int(a.tokens, a.tok_bytes, n), 0), a.V - 1);
-      const float zy = T::get(row, y);
-      row_stats<T, G, NV>(v, edge, a, red[phase], wave, m, S);
       const TokenOut o = token_head(a, n, zy - m, S);
       if (g == 0) {
         if (a.per_row) a.per_row[n] = o.lp;
-        if (a.stats) a.stats[n] = make_float4(m, S, a.head == HEAD_LOGPROB ? a.inv_tau : 0.0f, zy - m);
+        if (a.stats) a.stats[n] = make_float4(m, S, a.head == HEAD_LOGPROB ? a.inv_tau : 0.0f, zy);
         acc += (double)o.loss;
       }
-      if (out) {
-        const float c = w * o.c, inv_S = rcp_acc(S), scale = -c * inv_S;
-        float f[E];
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          T::unpack(v[j], f);
-#pragma unroll
-          for (int e = 0; e < E; ++e) f[e] = scale * exp_d(f[e] - m, a.c_hi, a.c_lo);
-          if (j * G + g < cut.full) store_piece<T>(obody + j * (G * 16) + (uint32_t)g * 16u, T::pack(f));
-        }
-        if (cut.has_edge(g)) T::put(out, cut.edge(g), scale * exp_d(edge - m, a.c_hi, a.c_lo));
+      if constexpr (GRAD) {
+        const float c = w * o.c, inv_S = rcp_acc(S);
+        grad_pieces<T, G, NV>(v, edge, a, cut, out, g, m, -c * inv_S);
         // the token's own element, c (1 - p), by the lane that wrote its place above
-        if (g == cut.lane_of(y, G)) T::put(out, y, token_grad(c, zy - m, S, inv_S, a.c_hi, a.c_lo));
+        if (g == cut.lane_of(y, G)) T::put(out, y, token_grad(c, zy - m, S, a.c_hi, a.c_lo));
       }
     } else {
-      List l;
-      l.idx = (int*)lists + slot * a.k;
-      l.e = (float*)lists + (Sh::ROWS + slot) * a.k;
-      const bool lister = G <= 64 || wave == 0;      // a row of several waves: the first has the list
-      if (lister) {
-        list_load<Sh::GL>(a, n, g, l);
-        if (G > 64 && g == 0) kept_flag[phase] = l.kept;
-      }
-      row_stats<T, G, NV>(v, edge, a, red[phase], wave, m, S);
       const int kept = G > 64 ? kept_flag[phase] : l.kept;
       if (lister) {
+        if constexpr (G > 64) {
+          l.St = list_sums[0];
+          l.A = list_sums[1];
+          l.kept = kept;
+        }
         const float loss = list_loss<T, Sh::GL>(a, row, g, l, m, S);
         if (g == 0) {
           if (a.per_row) a.per_row[n] = loss;
           acc += (double)loss;
         }
       }
-      if (out) {
-        const float inv_S = rcp_acc(S), c = kept ? -w : 0.0f, scale = kept ? w * inv_S : 0.0f;
-        float f[E];
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          T::unpack(v[j], f);
-#pragma unroll
-          for (int e = 0; e < E; ++e) f[e] = scale * exp_d(f[e] - m, a.c_hi, a.c_lo);
-          if (j * G + g < cut.full) store_piece<T>(obody + j * (G * 16) + (uint32_t)g * 16u, T::pack(f));
-        }
-        if (cut.has_edge(g)) T::put(out, cut.edge(g), scale * exp_d(edge - m, a.c_hi, a.c_lo));
-        // the listed classes' elements go over what the pieces' lanes have just written
+      if constexpr (GRAD) {
+        const float inv_S = rcp_acc(S);
+        grad_pieces<T, G, NV>(v, edge, a, cut, out, g, m, kept ? w * inv_S : 0.0f);
         if constexpr (G > 64) __syncthreads();
         else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (lister && kept) list_grad<T, Sh::GL>(a, row, out, g, l, m, inv_S, c);
+        if (lister && kept) {
+          if constexpr (G > 64) {
+            l.St = list_sums[0];
+            if (TAGGED) l.twice = list_sums[2] != 0.0f;
+          }
+          list_grad<T, Sh::GL, TAGGED>(a, out, g, l, m, inv_S, -w);
+        }
       }
     }
     phase ^= 1;
@@ -511,7 +629,7 @@ __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
   constexpr int E = T::E;
   __shared__ float2 red[2][WIDE / 64];
   __shared__ int kept_flag[2];
-  extern __shared__ char lists[];
+  extern __shared__ __align__(16) char lists[];
   if (a.only_if_rescaled && *a.upstream == 1.0f) return;
   const int g = threadIdx.x, wave = threadIdx.x >> 6;
   __shared__ int counts[16];
@@ -562,15 +680,13 @@ __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
     }
     int y = 0;
     float zy = 0.0f;
-    List l;
+    List l = list_place<false>(lists, 1, 0, a.k);
     if constexpr (!DISTILL) {
       y = min(max(get_int(a.tokens, a.tok_bytes, n), 0), a.V - 1);
       zy = T::get(row, y);
     } else {
-      l.idx = (int*)lists;
-      l.e = (float*)lists + a.k;
       if (wave == 0) {
-        list_load<64>(a, n, g, l);
+        list_load<64, false>(a, n, g, l);
         if (g == 0) kept_flag[phase] = l.kept;
       }
     }
@@ -591,7 +707,7 @@ __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
       const TokenOut o = token_head(a, n, zy - m, S);
       if (g == 0) {
         if (a.per_row) a.per_row[n] = o.lp;
-        if (a.stats) a.stats[n] = make_float4(m, S, a.head == HEAD_LOGPROB ? a.inv_tau : 0.0f, zy - m);
+        if (a.stats) a.stats[n] = make_float4(m, S, a.head == HEAD_LOGPROB ? a.inv_tau : 0.0f, zy);
         acc += (double)o.loss;
       }
       c = w * o.c;
@@ -609,19 +725,16 @@ __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
       scale = kept ? w * inv_S : 0.0f;
     }
     if (out) {
+      const Scale sc(scale);
 #pragma unroll 4
-      for (int j = g; j < cut.full; j += WIDE) {
-        T::unpack(*(const typename T::Raw*)(body + (uint32_t)j * 16u), f);
-#pragma unroll
-        for (int e = 0; e < E; ++e) f[e] = scale * exp_d(f[e] - m, a.c_hi, a.c_lo);
-        store_piece<T>(obody + (uint32_t)j * 16u, T::pack(f));
-      }
+      for (int j = g; j < cut.full; j += WIDE)
+        store_piece<T>(obody + (uint32_t)j * 16u, grad_piece<T>(*(const typename T::Raw*)(body + (uint32_t)j * 16u), a, m, sc));
       if (cut.has_edge(g)) T::put(out, cut.edge(g), scale * exp_d(edge - m, a.c_hi, a.c_lo));
       if constexpr (!DISTILL) {
-        if (g == cut.lane_of(y, WIDE)) T::put(out, y, token_grad(c, zy - m, S, inv_S, a.c_hi, a.c_lo));
+        if (g == cut.lane_of(y, WIDE)) T::put(out, y, token_grad(c, zy - m, S, a.c_hi, a.c_lo));
       } else {
         __syncthreads();
-        if (wave == 0 && kept) list_grad<T, 64>(a, row, out, g, l, m, inv_S, c);
+        if (wave == 0 && kept) list_grad<T, 64, false>(a, out, g, l, m, inv_S, c);
       }
     }
     phase ^= 1;
@@ -630,7 +743,7 @@ __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
 }
 
 // ------------------------------------------------------------------------------- gradient from the rows' statistics
-// dz = c u (1[v = y] - p): m, S and c from stats, u the upstream gradient of the row (u_stride 1) or of the whole (0).
+// dz = c u (1[v = y] - p): m, S, c and the token's logit from stats, u the upstream gradient of the row (u_stride 1) or of the whole (0).
 // A row's pieces are cut into chunks so that few long rows fill the chip too.
 struct GradArgs {
   const void* z; long sb, sl; int L, V, N; int dense;
@@ -675,14 +788,10 @@ __global__ __launch_bounds__(GRAD_WG) void k_token_grad(GradArgs a) {
     char* obody = out + cut.head * T::SIZE;
     const int lo = part * a.chunk, hi = min(cut.full, lo + a.chunk);
     const float m = st.x, inv_S = rcp_acc(st.y), scale = -c * inv_S;
-    float f[E];
+    const Scale sc(scale);
 #pragma unroll 4
-    for (int j = lo + g; j < hi; j += a.lanes) {
-      T::unpack(*(const typename T::Raw*)(body + (uint32_t)j * 16u), f);
-#pragma unroll
-      for (int e = 0; e < E; ++e) f[e] = scale * exp_d(f[e] - m, a.c_hi, a.c_lo);
-      store_piece<T>(obody + (uint32_t)j * 16u, T::pack(f));
-    }
+    for (int j = lo + g; j < hi; j += a.lanes)
+      store_piece<T>(obody + (uint32_t)j * 16u, grad_piece<T>(*(const typename T::Raw*)(body + (uint32_t)j * 16u), a, m, sc));
     if (last && cut.has_edge(g)) {
       const int i = cut.edge(g);
       T::put(out, i, scale * exp_d(T::get(row, i) - m, a.c_hi, a.c_lo));
@@ -691,7 +800,7 @@ __global__ __launch_bounds__(GRAD_WG) void k_token_grad(GradArgs a) {
     const int y = min(max(get_int(a.tokens, a.tok_bytes, n), 0), a.V - 1), in = y - cut.head;
     const bool piece = in >= 0 && in < cut.full * E;
     if (piece ? in / E >= lo && in / E < hi && ((in / E - lo) & (a.lanes - 1)) == g : last && cut.lane_of(y, 1) == g)
-      T::put(out, y, token_grad(c, st.w, st.y, inv_S, a.c_hi, a.c_lo));
+      T::put(out, y, token_grad(c, st.w - m, st.y, a.c_hi, a.c_lo));
   }
 }
 
@@ -727,6 +836,9 @@ struct PairArgs {
   float* rewards; double* pair_loss; float* loss;              // loss: of a single pair, written here
 };
 constexpr int PAIR_WG = 1024;
+// v_exp_f32 is low by 3.4e-9 of its value on average (over 6 M arguments in [-24, 0]; exact at 0, where the largest logit
+// is): nothing to one row, but a sequence's sum gathers it up (1537 tokens: 7e-6 of log-probability).
+constexpr double EXP2_LOW = 3.4e-9;
 // A pair's sums in 64 bits (a sequence's log-ratio is a long sum of small differences of large terms), its loss, and
 // the coefficient of its rows' gradients.
 __global__ __launch_bounds__(PAIR_WG) void k_pair(PairArgs a) {
@@ -740,7 +852,8 @@ __global__ __launch_bounds__(PAIR_WG) void k_pair(PairArgs a) {
     for (int l = threadIdx.x; l < a.L; l += PAIR_WG) {
       if (a.mask && !a.mask[n0 + l]) continue;
       const float4 st = a.stats[n0 + l];
-      s += (double)st.w - log((double)st.y) - (double)(a.ref ? a.ref[n0 + l] : 0.0f);
+      const double S = (double)st.y;
+      s += (double)st.w - (double)st.x - (log(S) + EXP2_LOW * (1.0 - 1.0 / S)) - (double)(a.ref ? a.ref[n0 + l] : 0.0f);
       c += 1.0;
     }
     D[h] = block_sum(s, lds);
@@ -816,10 +929,13 @@ template <typename T, int G, int NV, bool DISTILL>
 static int launch_rows(const RowArgs& a, int* grid, hipStream_t s) {
   typedef Shape<G> Sh;
   const int want = (a.N - 1) / Sh::ROWS + 1;
-  // parts of a wave: 8 workgroups of 256 a compute unit; whole workgroups: a row each as long as the partials allow
-  *grid = std::min(want, G <= 64 ? 2048 : MAX_PARTIALS);
-  const size_t lds = DISTILL ? (size_t)Sh::ROWS * a.k * 8 : 0;
-  hipLaunchKernelGGL((k_rows<T, G, NV, DISTILL>), dim3(*grid), dim3(Sh::WG), lds, s, a);
+  // Parts of a wave: as many workgroups as the 256 compute units hold, which walk over the rows.  A row to a workgroup:
+  // one each, as they come (5 to 10 % less than with walking ones), up to 1024 lanes, where a compute unit holds one
+  // and the next would wait for its last store (615 us against 684 at 6144 rows of 100003 bf16 classes).
+  *grid = std::min(want, G <= 64 ? 2048 : G < 1024 ? MAX_PARTIALS : 256);
+  const size_t lds = DISTILL ? list_bytes(Sh::ROWS, a.k, NV < 16) : 0;
+  if (a.dz) hipLaunchKernelGGL((k_rows<T, G, NV, DISTILL, true>), dim3(*grid), dim3(Sh::WG), lds, s, a);
+  else hipLaunchKernelGGL((k_rows<T, G, NV, DISTILL, false>), dim3(*grid), dim3(Sh::WG), lds, s, a);
   D3PM_LAUNCH_CHECK("k_rows");
   return D3PM_OK;
 }
@@ -839,7 +955,7 @@ static int dispatch_rows(const RowArgs& a, int* grid, hipStream_t s) {
   if (full <= 8192) return launch_rows<T, 512, 16, DISTILL>(a, grid, s);
   if (full <= 16384) return launch_rows<T, 1024, 16, DISTILL>(a, grid, s);
   *grid = std::min(a.N, MAX_PARTIALS);
-  hipLaunchKernelGGL((k_rows_wide<T, DISTILL>), dim3(*grid), dim3(WIDE), DISTILL ? (size_t)a.k * 8 : 0, s, a);
+  hipLaunchKernelGGL((k_rows_wide<T, DISTILL>), dim3(*grid), dim3(WIDE), DISTILL ? list_bytes(1, a.k, false) : 0, s, a);
   D3PM_LAUNCH_CHECK("k_rows_wide");
   return D3PM_OK;
 }
