@@ -801,3 +801,44 @@ def test_together(pkg):
             per = -torch.min(r * A, r.clamp(0.8, 1.2) * A) + 0.1 * (torch.exp(xx) - xx - 1)
             return (per * w).sum() / w.sum()
         step(lambda z: policy(z, y, old, adv, ref, mask=mask), policy64)
+
+
+@pytest.mark.parametrize("V,dtype", [(24, "f32"), (24, "bf16"), (60, "f32"), (100, "f16"), (250, "f32"), (255, "bf16"),
+                                     (500, "f32"), (1000, "f32"), (1001, "bf16"), (2047, "f16")])
+@pytest.mark.parametrize("B,L", [(2, 1), (4, 15), (6, 64), (2, 320), (4, 321)])
+def test_pairs_of_any_size(pkg, V, dtype, B, L):
+    """Preference pairs on both sides of what one workgroup takes."""
+    check(pkg, "preference", make(V + L, B, L, V, dtype, mask=B > 2))
+    check(pkg, "preference", make(V + L + 1, B, L, V, dtype, mask=False), average=True)
+
+
+def test_pair_without_slope(pkg):
+    """Smoothing 1/2 of an undecided pair: the slope is 0 and so is the gradient."""
+    for V in (24, 5000):
+        z = torch.randn(1, 7, V, device="cuda").repeat(2, 1, 1).requires_grad_(True)
+        y = torch.randint(0, V, (1, 7), device="cuda").repeat(2, 1)
+        loss = pkg.PreferenceLoss(beta=0.5, label_smoothing=0.5)(z, y)
+        loss.backward()
+        assert abs(float(loss.detach()) - math.log(2.0)) <= 2 * EPS and bool((z.grad == 0).all())
+
+
+@pytest.mark.parametrize("name", ["distill", "policy"])
+def test_masks_counted_by_the_row_launch_or_ahead_of_it(pkg, name):
+    """16384 positions are the row launch's own to count; a mask that starts at an odd address, bytes of any value."""
+    for N in (1, 15, 33, 16384, 16385, 20000):
+        d = to_dev(make(N, 1, N + 1, 20, "f32", mask=True))
+        d["mask"] = torch.rand(1, N + 1, device="cuda") < 0.5
+        d["mask"][0, 1] = True
+        cut = {k: (v[:, 1:].contiguous() if torch.is_tensor(v) else v) for k, v in d.items()}
+        odd = torch.empty(N + 1, dtype=torch.uint8, device="cuda")
+        odd[1:] = cut["mask"][0].to(torch.uint8) * 0x90
+        cut["mask"] = odd[1:].view(torch.bool).view(1, N)
+        keep = (odd[1:] != 0).view(1, N)
+        per = {k: v for k, v in cut.items()}
+        root, out = call(pkg, name, per, cut["logits"])
+        terms = call(pkg, name, {**cut, "mask": None}, cut["logits"])[1]
+        if name == "distill":
+            want = (terms["per"].double() * keep).sum() / keep.sum()
+            tol = N * EPS * float(terms["per"].abs().max()) / max(1, int(keep.sum())) + 4 * EPS * abs(float(want))
+            assert abs(float(out["loss"]) - float(want)) <= tol
+        assert torch.equal(out["per" if name == "distill" else "lp"], terms["per" if name == "distill" else "lp"] * keep)
