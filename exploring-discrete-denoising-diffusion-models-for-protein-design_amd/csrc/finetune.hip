@@ -221,8 +221,9 @@ typedef __amdgpu_buffer_rsrc_t Rsrc;
 __device__ __forceinline__ Rsrc pieces_of(const void* body, int full) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)body, 0, full * 16, 0x00027000);
 }
+template <bool NT>
 __device__ __forceinline__ u32x4 load_piece(Rsrc r, int lane, int j, int G) {
-  return __builtin_amdgcn_raw_buffer_load_b128(r, (j * G + lane) * 16, 0, 0);
+  return __builtin_amdgcn_raw_buffer_load_b128(r, (j * G + lane) * 16, 0, NT ? 2 /* non-temporal */ : 0);
 }
 __device__ __forceinline__ void store_piece(Rsrc r, int lane, int j, int G, u32x4 v) {
   __builtin_amdgcn_raw_buffer_store_b128(v, r, (j * G + lane) * 16, 0, 2 /* non-temporal */);
@@ -506,6 +507,10 @@ __attribute__((amdgpu_waves_per_eu(WAVES_PER_SIMD<G, NV, DISTILL>))) void k_rows
   typedef Shape<G> Sh;
   constexpr bool PEEL = G >= 64;       // (a row of fewer lanes has no lane for every end element)
   constexpr bool TAGGED = NV < 16;
+  // Logits that are read once, for the gradient too, pass the caches by: 3 to 10 % of 268 MB of them at 4096 classes and
+  // more.  (A statistics launch leaves them there for the gradient launch: 588 us against 606 for 4 pairs of 1537 x 49999
+  // float16; and walking workgroups of 1024 lose 3 %: 821 us against 844 at 8192 x 131072 bf16.)
+  constexpr bool NT_LOADS = GRAD && G < 1024;
   __shared__ float2 red[2][G > 64 ? G / 64 : 1];
   __shared__ int kept_flag[2];
   __shared__ float list_sums[3];
@@ -539,7 +544,7 @@ __attribute__((amdgpu_waves_per_eu(WAVES_PER_SIMD<G, NV, DISTILL>))) void k_rows
     if constexpr (G >= 64) {
       const Rsrc from = pieces_of(body, cut.full);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) v[j] = load_piece(from, g, j, G);
+      for (int j = 0; j < NV; ++j) v[j] = load_piece<NT_LOADS>(from, g, j, G);
     } else {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -749,64 +754,70 @@ __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
 }
 
 // ------------------------------------------------------------------------------- gradient from the rows' statistics
-// dz = c u (1[v = y] - p): m, S, c and the token's logit from stats, u the upstream gradient of the row (u_stride 1) or of the whole (0).
-// A row's pieces are cut into chunks so that few long rows fill the chip too.
+// dz = c u (1[v = y] - p): m, S, c and the token's logit from stats, u the upstream gradient of the row (u_stride 1) or
+// of the whole (0).  A group of `lanes` takes a row of up to GRAD_PIECES pieces a lane; of a longer one (SPLIT) a
+// workgroup takes SPLIT_PIECES a lane, so that few long rows fill the chip too.  All pieces are asked for before the
+// first is used, and the logits are not looked at again: non-temporal loads too.  8 x 1024 x 65536 bf16
+// log-probabilities, forward and backward: 500 us; 503 with 4 pieces a lane, 510 with 8, 538 with cached loads, 563 with
+// 8 pieces a lane in a loop of 4096 workgroups.
+constexpr int GRAD_WG = 256, GRAD_PIECES = 4, SPLIT_PIECES = 2;
 struct GradArgs {
-  const void* z; long sb, sl; int L, V, N; int dense;
-  const void* tokens; int tok_bytes;
-  float c_hi, c_lo, inv_tau;
-  const float4* stats; const float* upstream; int u_stride; int only_if_rescaled;
-  int lanes, chunk, chunks;          // lanes of a group; pieces of a chunk; chunks of a row
-  void* dz;
+  RowArgs r;                          // logits, tokens, stats, dz
+  const float* upstream; int u_stride; int only_if_rescaled;
+  int lanes, chunks;                  // chunks of a row
 };
-constexpr int GRAD_WG = 256;
-template <typename T, bool PEEL>
+template <typename T, bool SPLIT>
 __global__ __launch_bounds__(GRAD_WG) void k_token_grad(GradArgs a) {
-  constexpr int E = T::E;
+  constexpr int E = T::E, NV = SPLIT ? SPLIT_PIECES : GRAD_PIECES;
+  constexpr bool PEEL = SPLIT;
   if (a.only_if_rescaled && *a.upstream == 1.0f) return;
-  const int g = threadIdx.x & (a.lanes - 1), slot = threadIdx.x / a.lanes, groups = GRAD_WG / a.lanes;
-  const long jobs = (long)a.N * a.chunks;
-  for (long job = (long)blockIdx.x * groups + slot; job < jobs; job += (long)gridDim.x * groups) {
-    const int n = a.chunks == 1 ? (int)job : (int)(job / a.chunks);
-    const int part = a.chunks == 1 ? 0 : (int)(job - (long)n * a.chunks);
-    const bool last = part == a.chunks - 1;
-    const float4 st = a.stats[n];
+  const int lanes = SPLIT ? GRAD_WG : a.lanes;
+  const int g = threadIdx.x & (lanes - 1), slot = SPLIT ? 0 : threadIdx.x / lanes, groups = SPLIT ? 1 : GRAD_WG / lanes;
+  const unsigned jobs = (unsigned)a.r.N * (unsigned)a.chunks;
+  for (unsigned job = blockIdx.x * groups + slot; job < jobs; job += gridDim.x * groups) {
+    const int n = SPLIT ? (int)(job / (unsigned)a.chunks) : (int)job;
+    const int part = SPLIT ? (int)(job - (unsigned)n * (unsigned)a.chunks) : 0, lo = part * (NV * GRAD_WG);
+    const bool last = !SPLIT || part == a.chunks - 1;
+    const float4 st = a.r.stats[n];
     const float c = st.z * (a.upstream ? a.upstream[(long)n * a.u_stride] : 1.0f);
-    char* out = (char*)a.dz + (long)n * a.V * T::SIZE;
-    if (c == 0.0f) {                                  // a row that is not counted, or whose upstream gradient is 0
-      const Cut<T, PEEL> cut(out, a.V);
-      const u32x4 zero = {0, 0, 0, 0};
-      char* obody = out + cut.head * T::SIZE;
-      const int hi = min(cut.full, (part + 1) * a.chunk);
-      for (int j = part * a.chunk + g; j < hi; j += a.lanes) *(typename T::Raw*)(obody + (uint32_t)j * 16u) = zero;
-      if (last && cut.has_edge(g)) T::put(out, cut.edge(g), 0.0f);
-      continue;
-    }
-    long at;
-    if (a.dense) at = (long)n * a.sl;
-    else {
-      const unsigned b = (unsigned)n / (unsigned)a.L;
-      at = (long)b * a.sb + (long)((unsigned)n - b * (unsigned)a.L) * a.sl;
-    }
-    const char* row = (const char*)a.z + at * T::SIZE;
-    const Cut<T, PEEL> cut(row, a.V);
+    char* out = (char*)a.r.dz + (long)n * a.r.V * T::SIZE;
+    const bool zero = c == 0.0f;      // a row that is not counted, or whose upstream gradient is 0: its logits are not read
+    const char* row = zero ? out : row_ptr(a.r, n, T::SIZE);
+    const Cut<T, PEEL> cut(row, a.r.V);
     const char* body = row + cut.head * T::SIZE;
     char* obody = out + cut.head * T::SIZE;
-    const int lo = part * a.chunk, hi = min(cut.full, lo + a.chunk);
-    const float m = st.x, inv_S = rcp_acc(st.y), scale = -c * inv_S;
+    const float m = st.x, scale = zero ? 0.0f : -c * rcp_acc(st.y);
     const Scale sc(scale);
-#pragma unroll 4
-    for (int j = lo + g; j < hi; j += a.lanes)
-      store_piece<T>(obody + (uint32_t)j * 16u, grad_piece<T>(*(const typename T::Raw*)(body + (uint32_t)j * 16u), a, m, sc));
+    u32x4 v[NV];
+    if constexpr (SPLIT) {
+      const int some = max(0, min(cut.full - lo, NV * GRAD_WG));
+      const Rsrc from = pieces_of(body + (long)lo * 16, zero ? 0 : some), to = pieces_of(obody + (long)lo * 16, some);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) v[j] = load_piece<true>(from, g, j, GRAD_WG);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) store_piece(to, g, j, GRAD_WG, zero ? (u32x4){0, 0, 0, 0} : grad_piece<T>(v[j], a.r, m, sc));
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        v[j] = (u32x4){0, 0, 0, 0};
+        if (!zero && j * lanes + g < cut.full)
+          v[j] = __builtin_nontemporal_load((const typename T::Raw*)(body + (uint32_t)(j * lanes + g) * 16u));
+      }
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (j * lanes + g < cut.full)
+          store_piece<T>(obody + (uint32_t)(j * lanes + g) * 16u, zero ? (u32x4){0, 0, 0, 0} : grad_piece<T>(v[j], a.r, m, sc));
+    }
     if (last && cut.has_edge(g)) {
       const int i = cut.edge(g);
-      T::put(out, i, scale * exp_d(T::get(row, i) - m, a.c_hi, a.c_lo));
+      T::put(out, i, zero ? 0.0f : scale * exp_d(T::get(row, i) - m, a.r.c_hi, a.r.c_lo));
     }
+    if (zero) continue;
     // the token's own element, c (1 - p), by the lane that wrote its place above
-    const int y = min(max(get_int(a.tokens, a.tok_bytes, n), 0), a.V - 1), in = y - cut.head;
+    const int y = min(max(get_int(a.r.tokens, a.r.tok_bytes, n), 0), a.r.V - 1), in = y - cut.head;
     const bool piece = in >= 0 && in < cut.full * E;
-    if (piece ? in / E >= lo && in / E < hi && ((in / E - lo) & (a.lanes - 1)) == g : last && cut.lane_of(y, 1) == g)
-      T::put(out, y, token_grad(c, st.w - m, st.y, a.c_hi, a.c_lo));
+    if (piece ? in / E >= lo && in / E < lo + NV * lanes && ((in / E - lo) & (lanes - 1)) == g : last && cut.lane_of(y, 1) == g)
+      T::put(out, y, token_grad(c, st.w - m, st.y, a.r.c_hi, a.r.c_lo));
   }
 }
 
@@ -1090,13 +1101,6 @@ static int run_rows(const RowArgs& a, int dtype, int* grid, hipStream_t s) {
        : dtype == D3PM_F16 ? dispatch_rows<F16, DISTILL>(a, grid, s) : dispatch_rows<BF16, DISTILL>(a, grid, s);
 }
 
-template <typename T>
-static int launch_grad(const GradArgs& a, bool peel, int grid, hipStream_t s) {
-  if (peel) hipLaunchKernelGGL((k_token_grad<T, true>), dim3(grid), dim3(GRAD_WG), 0, s, a);
-  else hipLaunchKernelGGL((k_token_grad<T, false>), dim3(grid), dim3(GRAD_WG), 0, s, a);
-  D3PM_LAUNCH_CHECK("k_token_grad");
-  return D3PM_OK;
-}
 template <typename T, int G, int NV>
 static int launch_pairs(const PairArgs& a, hipStream_t s) {
   hipLaunchKernelGGL((k_pair_rows<T, G, NV>), dim3(a.P), dim3(PAIR_WG), (size_t)2 * a.r.L * sizeof(float4), s, a);
@@ -1115,25 +1119,30 @@ static int dispatch_pairs(const PairArgs& a, hipStream_t s) {
     default: return launch_pairs<T, 64, 4>(a, s);
   }
 }
+template <typename T>
+static int launch_grad(GradArgs& a, hipStream_t s) {
+  const int full = a.r.V / T::E;
+  a.lanes = 8;
+  while (a.lanes < 64 && a.lanes * GRAD_PIECES < full) a.lanes <<= 1;
+  const bool split = a.lanes * GRAD_PIECES < full;
+  a.chunks = split ? (full + GRAD_WG * SPLIT_PIECES - 1) / (GRAD_WG * SPLIT_PIECES) : 1;
+  const long jobs = (long)a.r.N * a.chunks, per = split ? 1 : GRAD_WG / a.lanes;
+  D3PM_CHECK_ARG(jobs < INT_MAX, "token gradient: %d rows of %d classes", a.r.N, a.r.V);
+  // (the call that mostly finds nothing to do is not to cost the dispatch of all that would do it)
+  const int grid = (int)std::min<long>((jobs + per - 1) / per, a.only_if_rescaled ? 2048 : 1 << 20);
+  if (split) hipLaunchKernelGGL((k_token_grad<T, true>), dim3(grid), dim3(GRAD_WG), 0, s, a);
+  else hipLaunchKernelGGL((k_token_grad<T, false>), dim3(grid), dim3(GRAD_WG), 0, s, a);
+  D3PM_LAUNCH_CHECK("k_token_grad");
+  return D3PM_OK;
+}
 static int run_grad(const d3pm_logits* z, const void* tokens, int tok_bytes, float tau, const float* stats,
                     const float* upstream, int per_row, int only_if_rescaled, void* dz, hipStream_t s) {
   GradArgs a{};
-  a.z = z->data; a.sb = z->stride_b; a.sl = z->stride_l;
-  a.L = (int)z->L; a.V = z->V; a.N = (int)(z->B * z->L); a.dense = is_dense(z) ? 1 : 0;
-  a.tokens = tokens; a.tok_bytes = tok_bytes;
-  set_temperature(tau, &a.c_hi, &a.c_lo, &a.inv_tau);
-  a.stats = (const float4*)stats; a.upstream = upstream; a.u_stride = per_row; a.only_if_rescaled = only_if_rescaled;
-  a.dz = dz;
-  const int full = a.V / (z->dtype == D3PM_F32 ? 4 : 8);
-  a.lanes = 8;
-  while (a.lanes < 256 && a.lanes < full) a.lanes <<= 1;
-  a.chunk = a.lanes * 8;
-  a.chunks = std::max(1, (full + a.chunk - 1) / a.chunk);
-  const long jobs = (long)a.N * a.chunks, per = GRAD_WG / a.lanes;
-  const int grid = (int)std::min<long>((jobs + per - 1) / per, 4096);
-  const bool peel = a.lanes >= 64;                   // a lane for every end element
-  if (z->dtype == D3PM_F32) return launch_grad<F32>(a, peel, grid, s);
-  return z->dtype == D3PM_F16 ? launch_grad<F16>(a, peel, grid, s) : launch_grad<BF16>(a, peel, grid, s);
+  a.r = row_args(z, tau);
+  a.r.tokens = tokens; a.r.tok_bytes = tok_bytes;
+  a.r.stats = (float4*)stats; a.r.dz = dz;
+  a.upstream = upstream; a.u_stride = per_row; a.only_if_rescaled = only_if_rescaled;
+  return z->dtype == D3PM_F32 ? launch_grad<F32>(a, s) : z->dtype == D3PM_F16 ? launch_grad<F16>(a, s) : launch_grad<BF16>(a, s);
 }
 
 // The count of the mask (first 8 bytes of the workspace, where a later call for the gradient alone finds it) and the
