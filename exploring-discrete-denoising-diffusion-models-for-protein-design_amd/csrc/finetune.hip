@@ -505,7 +505,7 @@ template <typename T, int G, int NV, bool DISTILL, bool GRAD>
 __global__ __launch_bounds__(Shape<G>::WG)
 __attribute__((amdgpu_waves_per_eu(WAVES_PER_SIMD<G, NV, DISTILL>))) void k_rows(RowArgs a) {
   typedef Shape<G> Sh;
-  constexpr bool PEEL = G >= 64;       // (a row of fewer lanes has no lane for every end element)
+  constexpr bool PEEL = G >= 2 * T::E; // (a row of fewer lanes has no lane for every end element)
   constexpr bool TAGGED = NV < 16;
   // Logits that are read once, for the gradient too, pass the caches by: 3 to 10 % of 268 MB of them at 4096 classes and
   // more.  (A statistics launch leaves them there for the gradient launch: 588 us against 606 for 4 pairs of 1537 x 49999

@@ -223,7 +223,7 @@ def test_more_rows_than_workgroups(pkg, V, dtype):
     fn = pkg.PolicyLoss()
     loss = fn(zz, y, old, torch.ones(rows, device="cuda"))
     loss.backward()
-    assert abs(float(loss) + math.exp(0.05)) < 4 * TOL
+    assert abs(float(loss.detach()) + math.exp(0.05)) < 4 * TOL
     for sl in (slice(0, 3), slice(rows // 2, rows // 2 + 3), slice(rows - 3, rows)):
         lp64 = torch.log_softmax(z[sl].double(), -1)
         lp = lp64.gather(1, y[sl][:, None])
@@ -842,3 +842,69 @@ def test_masks_counted_by_the_row_launch_or_ahead_of_it(pkg, name):
             tol = N * EPS * float(terms["per"].abs().max()) / max(1, int(keep.sum())) + 4 * EPS * abs(float(want))
             assert abs(float(out["loss"]) - float(want)) <= tol
         assert torch.equal(out["per" if name == "distill" else "lp"], terms["per" if name == "distill" else "lp"] * keep)
+
+
+def test_classes_that_share_a_place_of_the_table(pkg):
+    """Classes a multiple of 16384 apart (the table's size), listed once and twice."""
+    V, k = 60000, 12
+    d = make(101, 2, 3, V, "bf16", k=k, mask=False)
+    base = torch.randint(0, 5000, (2, 3, k // 3))
+    d["index"] = torch.cat([base, base + 16384, base + 32768], -1)
+    check(pkg, "distill", d)
+    d["index"][0, :, 1] = d["index"][0, :, 0]
+    check(pkg, "distill", d)
+
+
+@pytest.mark.parametrize("name", OBJECTIVES)
+def test_second_derivative_is_refused(pkg, name):
+    d = make(103, 4, 3, 20, "f32", mask=False)
+    c = to_dev(d)
+    z = c["logits"].requires_grad_(True)
+    root, _ = call(pkg, name, c, z)
+    g = torch.autograd.grad(root, z, torch.ones_like(root), create_graph=True)[0]
+    assert bool(torch.isfinite(g).all())
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    root, _ = call(pkg, name, c, z)
+    root.backward(torch.ones_like(root))
+    with pytest.raises(RuntimeError):                            # the graph is gone
+        root.backward(torch.ones_like(root))
+
+
+@pytest.mark.parametrize("name", OBJECTIVES)
+def test_modes_without_a_gradient(pkg, name):
+    d = to_dev(make(105, 4, 3, 20, "f32"))
+    want = call(pkg, name, d, d["logits"])[1]
+    with torch.inference_mode():
+        got = call(pkg, name, {k: (v.clone() if torch.is_tensor(v) else v) for k, v in d.items()}, d["logits"].clone())[1]
+        assert all(torch.equal(want[k], got[k]) for k in want)
+    for k in ("ref", "old", "adv"):                              # constants may require a gradient where none is recorded
+        d[k].requires_grad_(True)
+    with torch.no_grad():
+        got = call(pkg, name, d, d["logits"].requires_grad_(True))[1]
+    assert all(torch.equal(want[k], got[k]) for k in want)
+
+
+def test_row_shapes_at_their_edges(pkg):
+    """Widths around what each shape of the row kernel holds, for rows that start at every alignment."""
+    for dtype, E in (("f32", 4), ("bf16", 8)):
+        for pieces in (8, 16, 32, 64, 128, 256, 512, 1024, 2048, 4096):
+            for V in (pieces * E - 1, pieces * E, pieces * E + E - 1, pieces * E + E):
+                rows = 9
+                g = torch.Generator(device="cuda").manual_seed(V)
+                z = torch.randn(rows, V, generator=g, device="cuda").to(DTYPES[dtype]).requires_grad_(True)
+                y = torch.randint(0, V, (rows,), generator=g, device="cuda")
+                y[:3] = torch.tensor([0, V - 1, V // 2], device="cuda")
+                lp64 = torch.log_softmax(z.detach().double(), -1)
+                p, lp = lp64.exp(), lp64.gather(1, y[:, None])[:, 0]
+                onehot = torch.zeros_like(p).scatter_(1, y[:, None], 1.0)
+                c = torch.rand(rows, device="cuda") + 0.5
+                got = pkg.token_logprobs(z, y)
+                assert bool(((got.detach().double() - lp).abs() <= TOL + 4 * EPS * lp.abs()).all()), V
+                got.backward(c)
+                want, bound = c.double()[:, None] * (onehot - p), c.double()[:, None] * 2 * TOL * (p + onehot)
+                check_grad(z.grad, want.cpu(), bound.cpu(), z.dtype)
+                z.grad = None
+                loss = pkg.PolicyLoss(clip_low=1.0, clip_high=1e6)(z, y, lp.float(), c)       # r = 1: the same gradient, over rows
+                loss.backward()
+                check_grad(z.grad, (-want / rows).cpu(), (2 * bound / rows).cpu(), z.dtype)
