@@ -26,7 +26,7 @@ namespace ft {
 constexpr int MAX_K = 256;              // entries of a teacher's list
 constexpr int MAX_PARTIALS = 8192;      // workgroups of a loss launch: one partial sum each
 
-enum Head { HEAD_LOGPROB = 0, HEAD_PREFERENCE = 1, HEAD_POLICY = 2, HEAD_DISTILL = 3 };
+enum Head { HEAD_LOGPROB = 0, HEAD_PREFERENCE = 1, HEAD_POLICY = 2 };
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -893,7 +893,8 @@ __device__ __forceinline__ float2 pair_finish(const PairArgs& a, int p, double D
     const double z = exp(-fabs(margin)), soft = log1p(z), top = 1.0 / (1.0 + z);
     const double sig = margin >= 0.0 ? top : z * top, gis = margin >= 0.0 ? z * top : top;  // sigma(margin), sigma(-margin)
     const double neg = margin < 0.0 ? -margin : 0.0, pos = margin > 0.0 ? margin : 0.0;
-    const double loss = (1.0 - e) * (soft + neg) + e * (soft + pos);
+    // a term of weight 0 is not there (a token that the model rules out makes the other one infinite)
+    const double loss = (e < 1.0 ? (1.0 - e) * (soft + neg) : 0.0) + (e > 0.0 ? e * (soft + pos) : 0.0);
     const double slope = -(double)a.out_scale * (double)a.beta / (double)a.P * ((1.0 - e) * gis - e * sig);
     if (lane == 0) {
       a.rewards[p] = (float)((double)a.beta * D0);
@@ -1248,7 +1249,6 @@ extern "C" int d3pm_topk_distill_loss(const d3pm_logits* z, const void* teacher_
   D3PM_CHECK_ARG(z->B * z->L == 0 || (teacher_logits && teacher_index), "%s: null teacher", who);
   D3PM_CHECK_ARG(std::isfinite(out_scale), "%s: out_scale is not finite", who);
   RowArgs a = row_args(z, temperature);
-  a.head = HEAD_DISTILL;
   a.mask = mask;
   a.t_logits = teacher_logits; a.t_dtype = teacher_dtype;
   a.t_index = teacher_index; a.t_index_bytes = index_bytes; a.k = k;

@@ -3,8 +3,8 @@
 // A thin shim: every operator checks its tensors, allocates its outputs (and workspace) with torch's
 // allocator, and calls the C ABI of libd3pm_hip.so (include/d3pm_hip.h) on torch's current HIP stream.  No
 // arithmetic happens here.  The operators carry the reference function they stand for in their schema comment;
-// autograd nodes live in the Python facade, which calls these operators (those of the fine-tuning objectives live here).  Status codes of the library become
-// the exceptions the reference raises: D3PM_EINVAL -> ValueError, D3PM_EUNSUPPORTED -> NotImplementedError,
+// autograd nodes live in the Python facade, which calls these operators; those of the fine-tuning objectives live
+// here.  Status codes of the library become the exceptions the reference raises: D3PM_EINVAL -> ValueError, D3PM_EUNSUPPORTED -> NotImplementedError,
 // D3PM_EHIP -> RuntimeError.  Every operator makes the device of its first tensor current for the call and checks
 // every tensor's element count against the batch it describes before a pointer reaches the library: a mis-shaped
 // call raises, it does not read or write out of bounds.
@@ -714,12 +714,13 @@ struct ObjectiveNode : public torch::autograd::Node {
     TORCH_CHECK(!released_, torch::autograd::ERR_BACKWARD_TWICE);
     if (!grads[0].defined() || !task_should_compute_output(0)) return variable_list(1);
     const bool twice = at::GradMode::is_enabled();
+    // (with autograd still in place: a checkpoint computes its part of the model again here)
+    const Tensor logits = logits_.unpack(getptr());
+    std::vector<Tensor> saved;
+    for (const auto& v : saved_) saved.push_back(v.unpack(getptr()));
     Tensor dz;
     {
       at::AutoDispatchBelowADInplaceOrView below;
-      const Tensor logits = logits_.unpack(getptr());
-      std::vector<Tensor> saved;
-      for (const auto& v : saved_) saved.push_back(v.unpack(getptr()));
       const Tensor upstream = grads[0].contiguous();
       const bool first = dz_.defined();
       dz = first ? std::move(dz_) : at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));

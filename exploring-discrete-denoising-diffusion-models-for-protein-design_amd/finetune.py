@@ -111,7 +111,7 @@ class PreferenceLoss(torch.nn.Module):
     model (``token_logprobs``; None: 0).  With ``D`` a sequence's sum of ``lp - ref_logprobs`` over its counted
     positions (their mean with ``average``) and ``m = beta * (D_preferred - D_other)``, ``forward`` returns the mean
     over the pairs of ``-(1 - label_smoothing) * log sigmoid(m) - label_smoothing * log sigmoid(-m)``, times
-    ``out_scale``.  ``rewards`` holds ``beta * D`` ``[2 P]`` of the last call."""
+    ``out_scale`` (a term of weight 0 is left out, also where its logarithm is infinite).  ``rewards`` holds ``beta * D`` ``[2 P]`` of the last call."""
 
     def __init__(self, beta: float = 0.1, label_smoothing: float = 0.0, average: bool = False):
         super().__init__()

@@ -908,3 +908,45 @@ def test_row_shapes_at_their_edges(pkg):
                 loss = pkg.PolicyLoss(clip_low=1.0, clip_high=1e6)(z, y, lp.float(), c)       # r = 1: the same gradient, over rows
                 loss.backward()
                 check_grad(z.grad, (-want / rows).cpu(), (2 * bound / rows).cpu(), z.dtype)
+
+
+@pytest.mark.parametrize("name", OBJECTIVES)
+def test_checkpointed_and_offloaded(pkg, name):
+    """The head and its loss under a checkpoint (backward computes them again), or with saved tensors moved to the host:
+    the gradients of the ordinary call, bit for bit."""
+    from torch.utils.checkpoint import checkpoint
+    d = to_dev(make(107, 4, 5, 40, "f32"))
+    h = torch.randn(4 * 5, 16, generator=torch.Generator().manual_seed(1)).cuda().requires_grad_(True)
+    w = torch.randn(16, 40, generator=torch.Generator().manual_seed(2)).cuda().requires_grad_(True)
+
+    def part(h, w):
+        return call(pkg, name, d, (h @ w).view(4, 5, 40))[0]
+
+    def grads(run):
+        root = run()
+        return torch.autograd.grad(root, (h, w), 1.5 * torch.ones_like(root))
+
+    want = grads(lambda: part(h, w))
+    again = grads(lambda: checkpoint(part, h, w, use_reentrant=False))
+
+    def offloaded():
+        with torch.autograd.graph.save_on_cpu():
+            return part(h, w)
+
+    for got in (again, grads(offloaded)):
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("L,V", [(4, 24), (700, 24), (3, 9000)])
+def test_pair_whose_other_sequence_is_impossible(pkg, L, V):
+    """-log sigmoid(inf) = 0 and its slope is 0: without label smoothing the infinite other term is not there."""
+    d = to_dev(make(109, 2, L, V, "f32", mask=False))
+    for side in (1, 0):
+        z = d["logits"].clone()
+        z[side, 1, int(d["tokens"][side, 1])] = -math.inf
+        z.requires_grad_(True)
+        fn = pkg.PreferenceLoss(beta=0.5, label_smoothing=1.0 - side)      # smoothing of 1: the other way round
+        loss = fn(z, d["tokens"])
+        loss.backward()
+        assert float(loss) == 0.0 and int((z.grad != 0).sum()) == 0
+        assert float(fn.rewards[side]) == -math.inf and math.isfinite(float(fn.rewards[1 - side]))
