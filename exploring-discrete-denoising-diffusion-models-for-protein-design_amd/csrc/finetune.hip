@@ -127,6 +127,7 @@ struct RowArgs {
   const void* z; long sb, sl; int L, V, N; int dense;         // dense: row n lies at n * sl
   const void* tokens; int tok_bytes; const uint8_t* mask;
   float c_hi, c_lo, inv_tau;                                  // log2(e) / tau in two floats; 1 / tau
+  float d_min;                                                // z - m from which on exp((z - m) / tau) is 0
   int head;
   const float* old_lp; const float* ref_lp; const float* adv; int adv_per_seq; float clip_lo, clip_hi, kl_coeff;
   const void* t_logits; int t_dtype; const void* t_index; int t_index_bytes; int k;
@@ -173,25 +174,42 @@ __device__ __forceinline__ float exp_rest(float x) {
   return fabsf(x) < 0.35f ? x * x * q : exp_any(x) - 1.0f - x;
 }
 
+// (z - m) / tau - log S as hi + lo, to about 4e-8 whatever its size (of -8, float32 keeps 2.4e-7): with S = 2^e f, e ln 2 is
+// taken off in one exact step and a second for its rest, and what rounds there is kept.
+struct LogProb { float hi, lo; };
+__device__ __forceinline__ LogProb log_prob(float zy_m, float inv_tau, float S) {
+#pragma clang fp contract(off)
+  const float e = (float)__builtin_amdgcn_frexp_expf(S);
+  const float K = e * 0.693145752f;                                      // ln 2 to 16 bits: exact
+  const float k = fmaf(e, 1.42860677e-6f, logf(__builtin_amdgcn_frexp_mantf(S)));
+  const float p = zy_m * inv_tau, p_lo = fmaf(zy_m, inv_tau, -p);
+  const float s = p - K, b = s - p;
+  const float s_lo = (p - (s - b)) - (K + b);
+  return LogProb{s, fabsf(s) < INFINITY ? s_lo + p_lo - k : -k};         // (a token ruled out: -inf)
+}
+
 // What a row's token gives once m and S are known: its log-probability, its share of the loss and the coefficient
 // c of its gradient (without the weight).  Comparisons are written so that a NaN stays one.  Every lane of the row
-// computes this: at 32 classes its instructions are most of the launch, hence the short forms above.
+// computes this: at 32 classes its instructions are most of the launch, hence the short forms above.  Differences of
+// log-probabilities are taken from both parts: a mean over advantages of both signs is small against its terms, and an
+// error of 2.4e-7 in each of them showed in it.
 struct TokenOut { float lp, loss, c; };
 __device__ __forceinline__ TokenOut token_head(const RowArgs& a, int n, float zy_m, float S) {
   TokenOut o;
-  o.lp = zy_m * a.inv_tau - logf(S);
+  const LogProb lp = log_prob(zy_m, a.inv_tau, S);
+  o.lp = lp.hi + lp.lo;
   o.loss = 0.0f;
   o.c = 1.0f;
   if (a.head == HEAD_POLICY) {
     const float A = a.adv[a.adv_per_seq ? (unsigned)n / (unsigned)a.L : (unsigned)n];
-    const float r = exp_any(o.lp - a.old_lp[n]);
+    const float r = exp_any((lp.hi - a.old_lp[n]) + lp.lo);
     const float held_r = r < a.clip_lo ? a.clip_lo : r > a.clip_hi ? a.clip_hi : r;
     const float free_s = r * A, held_s = held_r * A;
     const bool clipped = free_s > held_s;
     o.loss = clipped ? -held_s : -free_s;
     o.c = clipped ? 0.0f : -free_s;
     if (a.ref_lp) {
-      const float x = a.ref_lp[n] - o.lp, q = exp_rest(x);
+      const float x = (a.ref_lp[n] - lp.hi) - lp.lo, q = exp_rest(x);
       o.loss = fmaf(a.kl_coeff, q, o.loss);
       o.c = fmaf(-a.kl_coeff, x + q, o.c);
     }
@@ -288,11 +306,15 @@ struct Cut {
 };
 
 // Keeps the compiler from carrying the unpacked values of one sweep over a row into the next: they take twice the
-// registers of the 16-bit pieces that they are unpacked from (220 instead of 64 + 36 at 16 pieces a lane).
-template <int NV>
+// registers of the 16-bit pieces that they are unpacked from (220 instead of 64 + 36 at 16 pieces a lane).  WAY: of two
+// sweeps in the two ways of a branch each has a text of its own, or their unpacking would be moved up before the branch.
+template <int NV, bool WAY = false>
 __device__ __forceinline__ void fresh(u32x4 (&v)[NV]) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(v[j]));
+  for (int j = 0; j < NV; ++j) {
+    if constexpr (WAY) asm volatile("; sweep" : "+v"(v[j]));
+    else asm volatile("" : "+v"(v[j]));
+  }
 }
 
 // The places of v that hold no piece of the row hold -inf.
@@ -310,8 +332,26 @@ __device__ __forceinline__ void mask_pieces(u32x4 (&v)[NV], int full, int g) {
 // m and S of the group's row from its lanes' values, in two steps: of the wave (a wave takes its exponentials against its
 // own maximum, so a row of several waves needs one exchange, not two; the reference is kept off -inf, for a wave that
 // has only padding), and of the row.  KEEP: the pieces are needed again, for the gradient.
-template <typename T, int GL, int NV, bool KEEP>
-__device__ __forceinline__ float2 wave_stats(u32x4 (&v)[NV], float edge, const RowArgs& a) {
+// EXACT: S in 64 bits, as hi + lo.  A preference loss sums a sequence's log-ratios, which may nearly cancel, and a policy
+// loss means over advantages of both signs.  With EXACT in a row of up to one wave the rounding of each exponent x is kept
+// as x_lo, and exp2(x + x_lo) = exp2(x) (1 + ln 2 x_lo); over the many terms of longer rows it averages out.
+struct RowSum { float m, hi, lo; };
+constexpr double LN2 = 0.69314718055994530942;
+// v_exp_f32 is low by 3.4e-9 of its value on average (over 6 M arguments in [-24, 0]; exact at 0, where the largest logit
+// is): nothing to one row, but a sequence's sum gathers it up (1537 tokens: 7e-6 of log-probability).
+constexpr double EXP2_LOW = 3.4e-9;
+__device__ __forceinline__ float exp_parts(float d, const RowArgs& a, float& low) {
+  d = __builtin_elementwise_maximum(d, a.d_min);     // (of a class ruled out, x_lo is no number; a NaN stays one)
+  const float x = d * a.c_hi, e = exp2_hw(x);
+  low = fmaf(e, fmaf(d, a.c_lo, fmaf(d, a.c_hi, -x)), low);
+  return e;
+}
+__device__ __forceinline__ RowSum in_parts(float m, double S) {
+  const float hi = (float)S;
+  return RowSum{m, hi, (float)(S - (double)hi)};
+}
+template <typename T, int G, int NV>
+__device__ __forceinline__ float wave_max(const u32x4 (&v)[NV], float edge) {
   float f[T::E];
   float mx = edge;
 #pragma unroll
@@ -320,30 +360,71 @@ __device__ __forceinline__ float2 wave_stats(u32x4 (&v)[NV], float edge, const R
 #pragma unroll
     for (int e = 0; e < T::E; ++e) mx = fmaxf(mx, f[e]);
   }
-  mx = fmaxf(group_max<GL>(mx), -FLT_MAX);
-  fresh<NV>(v);
-  float s0 = exp_d(edge - mx, a.c_hi, a.c_lo), s1 = 0.0f;
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    T::unpack(v[j], f);
-#pragma unroll
-    for (int e = 0; e < T::E; e += 2) {
-      s0 += exp_d(f[e] - mx, a.c_hi, a.c_lo);
-      s1 += exp_d(f[e + 1] - mx, a.c_hi, a.c_lo);
-    }
-  }
-  if constexpr (KEEP) fresh<NV>(v);
-  return make_float2(mx, group_sum<GL>(s0 + s1));
+  return fmaxf(group_max<(G < 64 ? G : 64)>(mx), -FLT_MAX);
 }
-template <int WAVES>
-__device__ __forceinline__ float2 join_stats(const float2* red, const RowArgs& a) {
+template <typename T, int G, int NV, bool KEEP, bool EXACT>
+__device__ __forceinline__ RowSum wave_sum(u32x4 (&v)[NV], float edge, float mx, const RowArgs& a) {
+  constexpr int GL = G < 64 ? G : 64;
+  float f[T::E];
+  fresh<NV, EXACT>(v);
+  if constexpr (EXACT && G <= 64) {
+    float low = 0.0f;
+    double s = (double)exp_parts(edge - mx, a, low);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      T::unpack(v[j], f);
+#pragma unroll
+      for (int e = 0; e < T::E; ++e) s += (double)exp_parts(f[e] - mx, a, low);
+    }
+    if constexpr (KEEP) fresh<NV>(v);
+    return in_parts(mx, group_sum<GL>(fma((double)low, LN2, s)));
+  } else {
+    float s0 = exp_d(edge - mx, a.c_hi, a.c_lo), s1 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      T::unpack(v[j], f);
+#pragma unroll
+      for (int e = 0; e < T::E; e += 2) {
+        s0 += exp_d(f[e] - mx, a.c_hi, a.c_lo);
+        s1 += exp_d(f[e + 1] - mx, a.c_hi, a.c_lo);
+      }
+    }
+    if constexpr (KEEP) fresh<NV>(v);
+    if constexpr (EXACT) return in_parts(mx, group_sum<GL>((double)s0 + (double)s1));
+    return RowSum{mx, group_sum<GL>(s0 + s1), 0.0f};
+  }
+}
+template <int WAVES, bool EXACT>
+__device__ __forceinline__ RowSum join_stats(const float2* red, const float* red_lo, const RowArgs& a) {
   float m = -FLT_MAX;
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) m = fmaxf(m, red[w].x);
   double sum = 0.0;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) sum += (double)(red[w].y * exp_d(red[w].x - m, a.c_hi, a.c_lo));
-  return make_float2(m, (float)sum);
+  for (int w = 0; w < WAVES; ++w) {
+    if constexpr (!EXACT) {
+      sum += (double)(red[w].y * exp_d(red[w].x - m, a.c_hi, a.c_lo));
+      continue;
+    }
+    float low = 0.0f;
+    const float e = exp_parts(red[w].x - m, a, low);
+    // (EXP2_LOW: of this exponential; a wave that holds the maximum has 1)
+    sum += ((double)red[w].y + (double)red_lo[w]) * (e == 1.0f ? 1.0 : fma((double)low, LN2, (double)e) * (1.0 + EXP2_LOW));
+  }
+  return in_parts(m, sum);
+}
+
+template <typename T, int G, int NV, bool KEEP, bool EXACT>
+__device__ __forceinline__ RowSum row_sum(u32x4 (&v)[NV], float edge, float mx, const RowArgs& a, float2* red,
+                                          float* red_lo) {
+  const RowSum st = wave_sum<T, G, NV, KEEP, EXACT>(v, edge, mx, a);
+  if constexpr (G <= 64) return st;
+  if ((threadIdx.x & 63) == 0) {
+    red[threadIdx.x >> 6] = make_float2(st.m, st.hi);
+    if (EXACT) red_lo[threadIdx.x >> 6] = st.lo;
+  }
+  __syncthreads();
+  return join_stats<G / 64, EXACT>(red, red_lo, a);
 }
 
 // The teacher's list of a row, spread over GL lanes of one wave: the kept entries' classes (-1: not kept), exponentials
@@ -512,6 +593,7 @@ __attribute__((amdgpu_waves_per_eu(WAVES_PER_SIMD<G, NV, DISTILL>))) void k_rows
   // float16; and walking workgroups of 1024 lose 3 %: 821 us against 844 at 8192 x 131072 bf16.)
   constexpr bool NT_LOADS = GRAD && G < 1024;
   __shared__ float2 red[2][G > 64 ? G / 64 : 1];
+  __shared__ float red_lo[2][G > 64 ? G / 64 : 1];
   __shared__ int kept_flag[2];
   __shared__ float list_sums[3];
   __shared__ double wg_sum[Sh::ROWS];
@@ -571,19 +653,20 @@ __attribute__((amdgpu_waves_per_eu(WAVES_PER_SIMD<G, NV, DISTILL>))) void k_rows
       }
     }
     if constexpr (G >= 64) mask_pieces<T, G, NV>(v, cut.full, g);
-    float2 st = wave_stats<T, Sh::GL, NV, GRAD>(v, edge, a);
-    if constexpr (G > 64) {
-      if ((g & 63) == 0) red[phase][wave] = st;
-      __syncthreads();
-      st = join_stats<G / 64>(red[phase], a);
-    }
-    const float m = st.x, S = st.y;
+    const float mx = wave_max<T, G, NV>(v, edge);
+    RowSum st;
+    if constexpr (DISTILL || GRAD)                   // (no registers for EXACT in rows of several waves with their gradient)
+      st = row_sum<T, G, NV, GRAD, !DISTILL && G <= 64>(v, edge, mx, a, red[phase], red_lo[phase]);
+    else if (a.head == HEAD_PREFERENCE || (G <= 64 && a.head == HEAD_POLICY))
+      st = row_sum<T, G, NV, false, true>(v, edge, mx, a, red[phase], red_lo[phase]);
+    else st = row_sum<T, G, NV, false, false>(v, edge, mx, a, red[phase], red_lo[phase]);
+    const float m = st.m, S = st.hi;
 
     if constexpr (!DISTILL) {
       const TokenOut o = token_head(a, n, zy - m, S);
       if (g == 0) {
         if (a.per_row) a.per_row[n] = o.lp;
-        if (a.stats) a.stats[n] = make_float4(m, S, a.head == HEAD_LOGPROB ? a.inv_tau : 0.0f, zy);
+        if (a.stats) a.stats[n] = make_float4(m, S, a.head == HEAD_LOGPROB ? a.inv_tau : st.lo, zy);
         acc += (double)o.loss;
       }
       if constexpr (GRAD) {
@@ -855,12 +938,10 @@ struct PairArgs {
   float* rewards; double* pair_loss; float* loss;             // loss: of a single pair, written here
 };
 constexpr int PAIR_WG = 1024;
-// v_exp_f32 is low by 3.4e-9 of its value on average (over 6 M arguments in [-24, 0]; exact at 0, where the largest logit
-// is): nothing to one row, but a sequence's sum gathers it up (1537 tokens: 7e-6 of log-probability).
-constexpr double EXP2_LOW = 3.4e-9;
-// A row's log-ratio in 64 bits: a sequence's is a long sum of small differences of large terms.
+// A row's log-ratio in 64 bits: a sequence's is a long sum of small differences of large terms.  (S = y + z: the place of
+// c holds the rest of S until the pair's sums are known.)
 __device__ __forceinline__ double row_ratio(const PairArgs& a, float4 st, long n) {
-  const double S = (double)st.y;
+  const double S = (double)st.y + (double)st.z;
   return (double)st.w - (double)st.x - (log(S) + EXP2_LOW * (1.0 - 1.0 / S)) - (double)(a.ref ? a.ref[n] : 0.0f);
 }
 // Sums and counts of a pair's two sequences over the workgroup; then, by the first wave alone (every wave with its share
@@ -953,7 +1034,7 @@ __global__ __launch_bounds__(PAIR_WG) void k_pair_rows(PairArgs a) {
   for (int i = slot; i < 2 * L; i += ROWS) {
     const int n = (int)row_of(i);
     if (a.r.mask && !a.r.mask[n]) {
-      if (g == 0) stats[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);             // S = 0: not counted
+      if (g == 0) stats[i] = make_float4(0.0f, -1.0f, 0.0f, 0.0f);            // S = -1: not counted
       continue;
     }
     const char* row = row_ptr(a.r, n, T::SIZE);
@@ -967,15 +1048,15 @@ __global__ __launch_bounds__(PAIR_WG) void k_pair_rows(PairArgs a) {
     const float edge = cut.has_edge(g) ? T::get(row, cut.edge(g)) : -INFINITY;
     const int y = min(max(get_int(a.r.tokens, a.r.tok_bytes, n), 0), a.r.V - 1);
     const float zy = T::get(row, y);
-    const float2 st = wave_stats<T, G, NV, false>(v, edge, a.r);
-    if (g == 0) stats[i] = make_float4(st.x, st.y, 1.0f, zy);
+    const RowSum st = wave_sum<T, G, NV, false, true>(v, edge, wave_max<T, G, NV>(v, edge), a.r);
+    if (g == 0) stats[i] = make_float4(st.m, st.hi, st.lo, zy);
   }
   __syncthreads();
   double D[2] = {0.0, 0.0};
   int cnt[2] = {0, 0};
   for (int i = threadIdx.x; i < 2 * L; i += PAIR_WG) {
     const float4 st = stats[i];
-    if (st.z == 0.0f) continue;
+    if (st.y < 0.0f) continue;
     const double r = row_ratio(a, st, row_of(i));
     D[0] += i < L ? r : 0.0;
     D[1] += i < L ? 0.0 : r;
@@ -985,7 +1066,7 @@ __global__ __launch_bounds__(PAIR_WG) void k_pair_rows(PairArgs a) {
   const float2 c = pair_finish(a, p, D[0], D[1], cnt[0], cnt[1], sh);
   for (int i = threadIdx.x; i < 2 * L; i += PAIR_WG) {
     float4 st = stats[i];
-    if (st.z == 0.0f) st.y = 1.0f;
+    if (st.y < 0.0f) st.y = 1.0f;
     else st.z = i < L ? c.x : c.y;
     stats[i] = st;
     a.r.stats[row_of(i)] = st;
@@ -1054,6 +1135,7 @@ static RowArgs row_args(const d3pm_logits* z, float tau) {
   a.z = z->data; a.sb = z->stride_b; a.sl = z->stride_l;
   a.L = (int)z->L; a.V = z->V; a.N = (int)(z->B * z->L); a.dense = is_dense(z) ? 1 : 0;
   set_temperature(tau, &a.c_hi, &a.c_lo, &a.inv_tau);
+  a.d_min = -200.0f * tau;                                    // (exp2 of -288)
   a.inv_count = 1.0f;
   return a;
 }
