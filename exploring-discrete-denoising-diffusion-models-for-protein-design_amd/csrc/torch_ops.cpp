@@ -690,20 +690,37 @@ Tensor grad_buffer(const Tensor& z) { return at::empty(z.sizes(), z.options().me
 // node and its saved tensors took 45 us of a 92 us forward and backward.  A node keeps what its gradient needs, and
 // the gradient buffer that the loss launch filled for an upstream gradient of 1; backward hands that buffer over
 // after a launch that does it again only if the upstream gradient is another number, and a second backward
-// (retain_graph) fills a buffer of its own.
+// (retain_graph) fills a buffer of its own.  So does a backward that is captured into another graph than its forward, or
+// captured without it: a replay would find the buffer as the last one left it, not as the forward fills it.
 using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
+
+// the capture that the current stream is in, 0 if none
+unsigned long long capture_id() {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo((hipStream_t)stream(), &status, &id) != hipSuccess) {
+    (void)hipGetLastError();
+    return 0;
+  }
+  return status == hipStreamCaptureStatusActive ? id + 1 : 0;
+}
 
 struct ObjectiveNode : public torch::autograd::Node {
   SavedVariable logits_;
   std::vector<SavedVariable> saved_;
   Tensor dz_;
+  unsigned long long capture_ = 0;       // that the loss launch was in
   bool released_ = false;
 
   void save(const Tensor& logits, std::initializer_list<Tensor> others) {
     logits_ = SavedVariable(logits, false);
     for (const Tensor& t : others) saved_.emplace_back(t, false);
     set_next_edges(torch::autograd::collect_next_edges(logits));
+  }
+  void keep_gradient(Tensor&& dz) {
+    dz_ = std::move(dz);
+    capture_ = capture_id();
   }
   // the gradient for `upstream` into dz; only_if_rescaled: dz holds that for an upstream gradient of 1
   virtual void fill(const Tensor& logits, const std::vector<Tensor>& saved, const Tensor& upstream,
@@ -722,7 +739,7 @@ struct ObjectiveNode : public torch::autograd::Node {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       const Tensor upstream = grads[0].contiguous();
-      const bool first = dz_.defined();
+      const bool first = dz_.defined() && capture_ == capture_id();
       dz = first ? std::move(dz_) : at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
       dz_.reset();
       fill(logits, saved, upstream, first, dz);
@@ -849,7 +866,7 @@ std::tuple<Tensor, Tensor> topk_distill_loss(const Tensor& logits, const Tensor&
   if (want) {
     auto node = new_node<DistillBackward>();
     node->save(logits, {teacher_logits, teacher_index, mask, ws});
-    node->dz_ = std::move(dz);
+    node->keep_gradient(std::move(dz));
     node->args = args;
     torch::autograd::set_history(loss, node);
   }
@@ -913,7 +930,7 @@ std::tuple<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& token
   if (want) {
     auto node = new_node<PolicyBackward>();
     node->save(logits, {tokens, old_logprobs, advantages, ref_logprobs, mask, ws});
-    node->dz_ = std::move(dz);
+    node->keep_gradient(std::move(dz));
     node->args = args;
     torch::autograd::set_history(loss, node);
   }
@@ -957,7 +974,7 @@ std::tuple<Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& t
   if (want) {
     auto node = new_node<PreferenceBackward>();
     node->save(logits, {tokens, stats});
-    node->dz_ = std::move(dz);
+    node->keep_gradient(std::move(dz));
     torch::autograd::set_history(loss, node);
   }
   return {loss, rewards};

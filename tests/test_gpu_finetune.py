@@ -950,3 +950,42 @@ def test_pair_whose_other_sequence_is_impossible(pkg, L, V):
         loss.backward()
         assert float(loss) == 0.0 and int((z.grad != 0).sum()) == 0
         assert float(fn.rewards[side]) == -math.inf and math.isfinite(float(fn.rewards[1 - side]))
+
+
+@pytest.mark.parametrize("name", OBJECTIVES)
+@pytest.mark.parametrize("V", [24, 3000])
+def test_backward_in_a_graph_of_its_own(pkg, name, V):
+    """Forward and backward captured apart: the backward replayed again for other upstream gradients, with its result
+    overwritten between, and for new logits after the forward's replay."""
+    c = to_dev(make(111, 4, 6, V, "bf16"))
+    z = c["logits"].clone().requires_grad_(True)
+
+    def loss():
+        return call(pkg, name, c, z)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        root = loss()
+        u = torch.ones_like(root)
+        torch.autograd.grad(root, z, u)
+    torch.cuda.current_stream().wait_stream(side)
+    del root
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first):
+        root = loss()
+    with torch.cuda.graph(second, pool=first.pool()):
+        grad, = torch.autograd.grad(root, z, u)
+    for seed in (1, 2):
+        with torch.no_grad():
+            z.copy_(torch.randn(z.shape, generator=torch.Generator().manual_seed(seed)).cuda())
+        first.replay()
+        for factor in (2.0, 1.0, 1.0, -0.5):
+            u.fill_(factor)
+            grad.zero_()
+            second.replay()
+            torch.cuda.synchronize()
+            fresh = call(pkg, name, c, z.detach().clone().requires_grad_(True))[0]
+            zz = z.detach().clone().requires_grad_(True)
+            want, = torch.autograd.grad(call(pkg, name, c, zz)[0], zz, u)
+            assert torch.equal(grad, want) and torch.equal(root, fresh)
