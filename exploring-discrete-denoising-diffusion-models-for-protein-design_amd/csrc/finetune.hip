@@ -396,24 +396,18 @@ __device__ __forceinline__ RowSum wave_sum(u32x4 (&v)[NV], float edge, float mx,
     return RowSum{mx, group_sum<GL>(s0 + s1), 0.0f};
   }
 }
+// (Lane l of a wave takes the entry of wave l % WAVES, and the lanes add up among themselves.)
 template <int WAVES, bool EXACT>
 __device__ __forceinline__ RowSum join_stats(const float2* red, const float* red_lo, const RowArgs& a) {
-  float m = -FLT_MAX;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) m = fmaxf(m, red[w].x);
-  double sum = 0.0;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    if constexpr (!EXACT) {
-      sum += (double)(red[w].y * exp_d(red[w].x - m, a.c_hi, a.c_lo));
-      continue;
-    }
-    float low = 0.0f;
-    const float e = exp_parts(red[w].x - m, a, low);
-    // (EXP2_LOW: of this exponential; a wave that holds the maximum has 1)
-    sum += ((double)red[w].y + (double)red_lo[w]) * (e == 1.0f ? 1.0 : fma((double)low, LN2, (double)e) * (1.0 + EXP2_LOW));
-  }
-  return in_parts(m, sum);
+  const int w = threadIdx.x % WAVES;
+  const float2 r = red[w];
+  const float m = fmaxf(group_max<WAVES>(r.x), -FLT_MAX);
+  if constexpr (!EXACT) return in_parts(m, group_sum<WAVES>((double)(r.y * exp_d(r.x - m, a.c_hi, a.c_lo))));
+  float low = 0.0f;
+  const float e = exp_parts(r.x - m, a, low);
+  // (EXP2_LOW: of this exponential; a wave that holds the maximum has 1)
+  const double share = e == 1.0f ? 1.0 : fma((double)low, LN2, (double)e) * (1.0 + EXP2_LOW);
+  return in_parts(m, group_sum<WAVES>(((double)r.y + (double)red_lo[w]) * share));
 }
 
 template <typename T, int G, int NV, bool KEEP, bool EXACT>
@@ -657,9 +651,9 @@ __attribute__((amdgpu_waves_per_eu(WAVES_PER_SIMD<G, NV, DISTILL>))) void k_rows
     if constexpr (G >= 64) mask_pieces<T, G, NV>(v, cut.full, g);
     const float mx = wave_max<T, G, NV>(v, edge);
     RowSum st;
-    if constexpr (DISTILL || GRAD)                   // (no registers for EXACT in rows of several waves with their gradient)
-      st = row_sum<T, G, NV, GRAD, !DISTILL && G <= 64>(v, edge, mx, a, red[phase], red_lo[phase]);
-    else if (a.head == HEAD_PREFERENCE || (G <= 64 && a.head == HEAD_POLICY))
+    if constexpr (DISTILL || GRAD)
+      st = row_sum<T, G, NV, GRAD, !DISTILL>(v, edge, mx, a, red[phase], red_lo[phase]);
+    else if (a.head != HEAD_LOGPROB)
       st = row_sum<T, G, NV, false, true>(v, edge, mx, a, red[phase], red_lo[phase]);
     else st = row_sum<T, G, NV, false, false>(v, edge, mx, a, red[phase], red_lo[phase]);
     const float m = st.m, S = st.hi;
@@ -1153,7 +1147,7 @@ static int launch_rows(const RowArgs& a, int* grid, hipStream_t s) {
   // Parts of a wave: as many workgroups as the 256 compute units hold, which walk over the rows.  A row to a workgroup:
   // one each, as they come (5 to 10 % less than with walking ones), up to 1024 lanes, where a compute unit holds one
   // and the next would wait for its last store (615 us against 684 at 6144 rows of 100003 bf16 classes).
-  *grid = std::min(want, G <= 64 ? 2048 : G < 1024 ? MAX_PARTIALS : 256);
+  *grid = std::min(want, G <= 64 ? 2048 : G < 1024 || DISTILL ? MAX_PARTIALS : 256);
   const size_t lds = DISTILL ? list_bytes(Sh::ROWS, a.k, NV < 16) : 0;
   if (a.dz) hipLaunchKernelGGL((k_rows<T, G, NV, DISTILL, true>), dim3(*grid), dim3(Sh::WG), lds, s, a);
   else hipLaunchKernelGGL((k_rows<T, G, NV, DISTILL, false>), dim3(*grid), dim3(Sh::WG), lds, s, a);
