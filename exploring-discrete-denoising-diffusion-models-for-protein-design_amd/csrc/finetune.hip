@@ -119,9 +119,10 @@ __device__ __forceinline__ int get_int(const void* p, int bytes, long i) {
 
 // A piece of a gradient row: nothing in the launch reads it again, and the caches are better kept for the logits
 // (2 % of a launch at 32 k classes and more).
-template <typename T>
+template <typename T, bool NT = true>
 __device__ __forceinline__ void store_piece(char* p, u32x4 v) {
-  __builtin_nontemporal_store((typename T::Raw)v, (typename T::Raw*)p);
+  if constexpr (NT) __builtin_nontemporal_store((typename T::Raw)v, (typename T::Raw*)p);
+  else *(typename T::Raw*)p = (typename T::Raw)v;
 }
 
 // ------------------------------------------------------------------------------------------------------ arguments
@@ -245,8 +246,9 @@ template <bool NT>
 __device__ __forceinline__ u32x4 load_piece(Rsrc r, int lane, int j, int G) {
   return __builtin_amdgcn_raw_buffer_load_b128(r, (j * G + lane) * 16, 0, NT ? 2 /* non-temporal */ : 0);
 }
+template <bool NT>
 __device__ __forceinline__ void store_piece(Rsrc r, int lane, int j, int G, u32x4 v) {
-  __builtin_amdgcn_raw_buffer_store_b128(v, r, (j * G + lane) * 16, 0, 2 /* non-temporal */);
+  __builtin_amdgcn_raw_buffer_store_b128(v, r, (j * G + lane) * 16, 0, NT ? 2 /* non-temporal */ : 0);
 }
 
 // Counted positions of a mask, by a whole workgroup of up to 1024: every thread gets the sum.
@@ -319,6 +321,12 @@ __device__ __forceinline__ void fresh(u32x4 (&v)[NV]) {
   }
 }
 
+// Whether the j-th pieces of a row's lanes may hold any of its `full` pieces: those of rows of several waves, where the
+// answer is one branch, are passed over if not (a row fills at least half of its shape's pieces).  12288 rows of 70001
+// bf16 classes: 900 -> 751 us.  (Rows of one wave have no registers left for it: 99 -> 106 us at 2000 classes.)
+template <int G, int NV>
+__device__ __forceinline__ bool holds(int j, int full) { return G <= 64 || j < NV / 2 || j * G < full; }
+
 // The places of v that hold no piece of the row hold -inf.
 template <typename T, int G, int NV>
 __device__ __forceinline__ void mask_pieces(u32x4 (&v)[NV], int full, int g) {
@@ -353,11 +361,12 @@ __device__ __forceinline__ RowSum in_parts(float m, double S) {
   return RowSum{m, hi, (float)(S - (double)hi)};
 }
 template <typename T, int G, int NV>
-__device__ __forceinline__ float wave_max(const u32x4 (&v)[NV], float edge) {
+__device__ __forceinline__ float wave_max(const u32x4 (&v)[NV], float edge, int full) {
   float f[T::E];
   float mx = edge;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
+    if (!holds<G, NV>(j, full)) break;
     T::unpack(v[j], f);
 #pragma unroll
     for (int e = 0; e < T::E; ++e) mx = fmaxf(mx, f[e]);
@@ -365,7 +374,7 @@ __device__ __forceinline__ float wave_max(const u32x4 (&v)[NV], float edge) {
   return fmaxf(group_max<(G < 64 ? G : 64)>(mx), -FLT_MAX);
 }
 template <typename T, int G, int NV, bool KEEP, bool EXACT>
-__device__ __forceinline__ RowSum wave_sum(u32x4 (&v)[NV], float edge, float mx, const RowArgs& a) {
+__device__ __forceinline__ RowSum wave_sum(u32x4 (&v)[NV], float edge, float mx, int full, const RowArgs& a) {
   constexpr int GL = G < 64 ? G : 64;
   float f[T::E];
   fresh<NV, EXACT>(v);
@@ -374,6 +383,7 @@ __device__ __forceinline__ RowSum wave_sum(u32x4 (&v)[NV], float edge, float mx,
     double s = (double)exp_parts(edge - mx, a, low);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
+      if (!holds<G, NV>(j, full)) break;
       T::unpack(v[j], f);
 #pragma unroll
       for (int e = 0; e < T::E; ++e) s += (double)exp_parts(f[e] - mx, a, low);
@@ -384,6 +394,7 @@ __device__ __forceinline__ RowSum wave_sum(u32x4 (&v)[NV], float edge, float mx,
     float s0 = exp_d(edge - mx, a.c_hi, a.c_lo), s1 = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
+      if (!holds<G, NV>(j, full)) break;
       T::unpack(v[j], f);
 #pragma unroll
       for (int e = 0; e < T::E; e += 2) {
@@ -411,9 +422,9 @@ __device__ __forceinline__ RowSum join_stats(const float2* red, const float* red
 }
 
 template <typename T, int G, int NV, bool KEEP, bool EXACT>
-__device__ __forceinline__ RowSum row_sum(u32x4 (&v)[NV], float edge, float mx, const RowArgs& a, float2* red,
+__device__ __forceinline__ RowSum row_sum(u32x4 (&v)[NV], float edge, float mx, int full, const RowArgs& a, float2* red,
                                           float* red_lo) {
-  const RowSum st = wave_sum<T, G, NV, KEEP, EXACT>(v, edge, mx, a);
+  const RowSum st = wave_sum<T, G, NV, KEEP, EXACT>(v, edge, mx, full, a);
   if constexpr (G <= 64) return st;
   if ((threadIdx.x & 63) == 0) {
     red[threadIdx.x >> 6] = make_float2(st.m, st.hi);
@@ -557,7 +568,7 @@ __device__ __forceinline__ u32x4 grad_piece(u32x4 v, const Args& a, float m, con
   }
 }
 // The gradient pieces of a row from the pieces of its logits, and its end elements.
-template <typename T, int G, int NV, bool PEEL>
+template <typename T, int G, int NV, bool NT, bool PEEL>
 __device__ __forceinline__ void grad_pieces(u32x4 (&v)[NV], float edge, const RowArgs& a, const Cut<T, PEEL>& cut,
                                             char* out, int g, float m, float scale) {
   char* body = out + cut.head * T::SIZE;
@@ -565,11 +576,14 @@ __device__ __forceinline__ void grad_pieces(u32x4 (&v)[NV], float edge, const Ro
   if constexpr (G >= 64) {
     const Rsrc to = pieces_of(body, cut.full);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) store_piece(to, g, j, G, grad_piece<T>(v[j], a, m, sc));
+    for (int j = 0; j < NV; ++j) {
+      if (!holds<G, NV>(j, cut.full)) break;
+      store_piece<NT>(to, g, j, G, grad_piece<T>(v[j], a, m, sc));
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-      if (j * G + g < cut.full) store_piece<T>(body + j * (G * 16) + (uint32_t)g * 16u, grad_piece<T>(v[j], a, m, sc));
+      if (j * G + g < cut.full) store_piece<T, NT>(body + j * (G * 16) + (uint32_t)g * 16u, grad_piece<T>(v[j], a, m, sc));
   }
   if (cut.has_edge(g)) T::put(out, cut.edge(g), scale * exp_d(edge - m, a.c_hi, a.c_lo));
 }
@@ -588,6 +602,10 @@ __attribute__((amdgpu_waves_per_eu(WAVES_PER_SIMD<G, NV, DISTILL>))) void k_rows
   // more.  (A statistics launch leaves them there for the gradient launch: 588 us against 606 for 4 pairs of 1537 x 49999
   // float16; and walking workgroups of 1024 lose 3 %: 821 us against 844 at 8192 x 131072 bf16.)
   constexpr bool NT_LOADS = GRAD && G < 1024;
+  // A list's gradient goes over elements of pieces just written: in rows of up to four pieces a lane it hits much of them,
+  // which have to be in the caches still (64 entries: 65536 rows of 2000 bf16 classes 186 -> 150 us, 32768 of 8000 322 ->
+  // 272; at 4000 rows of 32003 103 -> 110).
+  constexpr bool NT_STORES = !DISTILL || NV > 4;
   __shared__ float2 red[2][G > 64 ? G / 64 : 1];
   __shared__ float red_lo[2][G > 64 ? G / 64 : 1];
   __shared__ int kept_flag[2];
@@ -649,13 +667,13 @@ __attribute__((amdgpu_waves_per_eu(WAVES_PER_SIMD<G, NV, DISTILL>))) void k_rows
       }
     }
     if constexpr (G >= 64) mask_pieces<T, G, NV>(v, cut.full, g);
-    const float mx = wave_max<T, G, NV>(v, edge);
+    const float mx = wave_max<T, G, NV>(v, edge, cut.full);
     RowSum st;
     if constexpr (DISTILL || GRAD)
-      st = row_sum<T, G, NV, GRAD, !DISTILL>(v, edge, mx, a, red[phase], red_lo[phase]);
+      st = row_sum<T, G, NV, GRAD, !DISTILL>(v, edge, mx, cut.full, a, red[phase], red_lo[phase]);
     else if (a.head != HEAD_LOGPROB)
-      st = row_sum<T, G, NV, false, true>(v, edge, mx, a, red[phase], red_lo[phase]);
-    else st = row_sum<T, G, NV, false, false>(v, edge, mx, a, red[phase], red_lo[phase]);
+      st = row_sum<T, G, NV, false, true>(v, edge, mx, cut.full, a, red[phase], red_lo[phase]);
+    else st = row_sum<T, G, NV, false, false>(v, edge, mx, cut.full, a, red[phase], red_lo[phase]);
     const float m = st.m, S = st.hi;
 
     if constexpr (!DISTILL) {
@@ -667,7 +685,7 @@ __attribute__((amdgpu_waves_per_eu(WAVES_PER_SIMD<G, NV, DISTILL>))) void k_rows
       }
       if constexpr (GRAD) {
         const float c = w * o.c, inv_S = rcp_acc(S);
-        grad_pieces<T, G, NV>(v, edge, a, cut, out, g, m, -c * inv_S);
+        grad_pieces<T, G, NV, true>(v, edge, a, cut, out, g, m, -c * inv_S);
         // the token's own element, c (1 - p), by the lane that wrote its place above
         if (g == cut.lane_of(y, G)) T::put(out, y, token_grad(c, zy - m, S, a.c_hi, a.c_lo));
       }
@@ -687,7 +705,7 @@ __attribute__((amdgpu_waves_per_eu(WAVES_PER_SIMD<G, NV, DISTILL>))) void k_rows
       }
       if constexpr (GRAD) {
         const float inv_S = rcp_acc(S);
-        grad_pieces<T, G, NV>(v, edge, a, cut, out, g, m, kept ? w * inv_S : 0.0f);
+        grad_pieces<T, G, NV, NT_STORES>(v, edge, a, cut, out, g, m, kept ? w * inv_S : 0.0f);
         if constexpr (G > 64) __syncthreads();
         else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (lister && kept) {
@@ -874,7 +892,7 @@ __global__ __launch_bounds__(GRAD_WG) void k_token_grad(GradArgs a) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) v[j] = load_piece<true>(from, g, j, GRAD_WG);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) store_piece(to, g, j, GRAD_WG, zero ? (u32x4){0, 0, 0, 0} : grad_piece<T>(v[j], a.r, m, sc));
+      for (int j = 0; j < NV; ++j) store_piece<true>(to, g, j, GRAD_WG, zero ? (u32x4){0, 0, 0, 0} : grad_piece<T>(v[j], a.r, m, sc));
     } else {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -1044,7 +1062,7 @@ __global__ __launch_bounds__(PAIR_WG) void k_pair_rows(PairArgs a) {
     const float edge = cut.has_edge(g) ? T::get(row, cut.edge(g)) : -INFINITY;
     const int y = min(max(get_int(a.r.tokens, a.r.tok_bytes, n), 0), a.r.V - 1);
     const float zy = T::get(row, y);
-    const RowSum st = wave_sum<T, G, NV, false, true>(v, edge, wave_max<T, G, NV>(v, edge), a.r);
+    const RowSum st = wave_sum<T, G, NV, false, true>(v, edge, wave_max<T, G, NV>(v, edge, NV * G), NV * G, a.r);
     if (g == 0) stats[i] = make_float4(st.m, st.hi, st.lo, zy);
   }
   __syncthreads();
