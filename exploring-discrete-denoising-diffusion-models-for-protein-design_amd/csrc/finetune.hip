@@ -604,8 +604,9 @@ __attribute__((amdgpu_waves_per_eu(WAVES_PER_SIMD<G, NV, DISTILL>))) void k_rows
   constexpr bool NT_LOADS = GRAD && G < 1024;
   // A list's gradient goes over elements of pieces just written: in rows of up to four pieces a lane it hits much of them,
   // which have to be in the caches still (64 entries: 65536 rows of 2000 bf16 classes 186 -> 150 us, 32768 of 8000 322 ->
-  // 272; at 4000 rows of 32003 103 -> 110).
-  constexpr bool NT_STORES = !DISTILL || NV > 4;
+  // 272; at 4000 rows of 32003 103 -> 110).  So does a token's element in short float32 rows (2 M rows of 32 classes 159 ->
+  // 147; of 1 M rows of 24 bf16 classes 80 -> 84).
+  constexpr bool NT_STORES = DISTILL ? NV > 4 : G > 8 || T::SIZE == 2;
   __shared__ float2 red[2][G > 64 ? G / 64 : 1];
   __shared__ float red_lo[2][G > 64 ? G / 64 : 1];
   __shared__ int kept_flag[2];
@@ -685,7 +686,7 @@ __attribute__((amdgpu_waves_per_eu(WAVES_PER_SIMD<G, NV, DISTILL>))) void k_rows
       }
       if constexpr (GRAD) {
         const float c = w * o.c, inv_S = rcp_acc(S);
-        grad_pieces<T, G, NV, true>(v, edge, a, cut, out, g, m, -c * inv_S);
+        grad_pieces<T, G, NV, NT_STORES>(v, edge, a, cut, out, g, m, -c * inv_S);
         // the token's own element, c (1 - p), by the lane that wrote its place above
         if (g == cut.lane_of(y, G)) T::put(out, y, token_grad(c, zy - m, S, a.c_hi, a.c_lo));
       }
