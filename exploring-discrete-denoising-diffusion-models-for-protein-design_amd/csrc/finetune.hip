@@ -242,13 +242,20 @@ typedef __amdgpu_buffer_rsrc_t Rsrc;
 __device__ __forceinline__ Rsrc pieces_of(const void* body, int full) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)body, 0, full * 16, 0x00027000);
 }
-template <bool NT>
-__device__ __forceinline__ u32x4 load_piece(Rsrc r, int lane, int j, int G) {
-  return __builtin_amdgcn_raw_buffer_load_b128(r, (j * G + lane) * 16, 0, NT ? 2 /* non-temporal */ : 0);
+// A lane's byte offset in the first pieces.  It is made again for every sweep: kept over the loop of the rows, the offsets
+// of 16 pieces would take 16 registers.
+__device__ __forceinline__ int lane_offset(int g) {
+  int at = g * 16;
+  asm volatile("" : "+v"(at));
+  return at;
 }
 template <bool NT>
-__device__ __forceinline__ void store_piece(Rsrc r, int lane, int j, int G, u32x4 v) {
-  __builtin_amdgcn_raw_buffer_store_b128(v, r, (j * G + lane) * 16, 0, NT ? 2 /* non-temporal */ : 0);
+__device__ __forceinline__ u32x4 load_piece(Rsrc r, int lane16, int j, int G) {
+  return __builtin_amdgcn_raw_buffer_load_b128(r, lane16 + j * (G * 16), 0, NT ? 2 /* non-temporal */ : 0);
+}
+template <bool NT>
+__device__ __forceinline__ void store_piece(Rsrc r, int lane16, int j, int G, u32x4 v) {
+  __builtin_amdgcn_raw_buffer_store_b128(v, r, lane16 + j * (G * 16), 0, NT ? 2 /* non-temporal */ : 0);
 }
 
 // Counted positions of a mask, by a whole workgroup of up to 1024: every thread gets the sum.
@@ -440,8 +447,8 @@ __device__ __forceinline__ RowSum row_sum(u32x4 (&v)[NV], float edge, float mx, 
 // A class may be listed twice.  Every kept entry writes its number to its class' place in a table of bytes and looks what
 // is there afterwards: its own number everywhere means that no class is.  (In a table smaller than the alphabet two
 // classes may share a place; that costs the search of list_grad, no more.)  65536 rows of 100 float32 classes with 64
-// entries: 43 us, 82 with the search for every entry.  Rows of 16 pieces a lane have no registers left for it (8192 rows
-// of 131072 bf16 classes: 816 us without the table, 853 with it) and search.
+// entries: 43 us, 82 with the search for every entry.  Rows of 16 pieces a lane search (8192 rows of 131072 bf16 classes:
+// 813 us without the table, 835 with it).
 constexpr int TAGS = 16384;             // bytes of a workgroup's tables: every class of a row of up to 64 lanes has a place
 struct List {
   int* idx; float* e; float* z; uint8_t* tag; int tag_mask;
@@ -575,10 +582,11 @@ __device__ __forceinline__ void grad_pieces(u32x4 (&v)[NV], float edge, const Ro
   const Scale sc(scale);
   if constexpr (G >= 64) {
     const Rsrc to = pieces_of(body, cut.full);
+    const int at = lane_offset(g);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (!holds<G, NV>(j, cut.full)) break;
-      store_piece<NT>(to, g, j, G, grad_piece<T>(v[j], a, m, sc));
+      store_piece<NT>(to, at, j, G, grad_piece<T>(v[j], a, m, sc));
     }
   } else {
 #pragma unroll
@@ -640,8 +648,9 @@ __attribute__((amdgpu_waves_per_eu(WAVES_PER_SIMD<G, NV, DISTILL>))) void k_rows
     u32x4 v[NV];
     if constexpr (G >= 64) {
       const Rsrc from = pieces_of(body, cut.full);
+      const int at = lane_offset(g);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) v[j] = load_piece<NT_LOADS>(from, g, j, G);
+      for (int j = 0; j < NV; ++j) v[j] = load_piece<NT_LOADS>(from, at, j, G);
     } else {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -891,9 +900,9 @@ __global__ __launch_bounds__(GRAD_WG) void k_token_grad(GradArgs a) {
       const int some = max(0, min(cut.full - lo, NV * GRAD_WG));
       const Rsrc from = pieces_of(body + (long)lo * 16, zero ? 0 : some), to = pieces_of(obody + (long)lo * 16, some);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) v[j] = load_piece<true>(from, g, j, GRAD_WG);
+      for (int j = 0; j < NV; ++j) v[j] = load_piece<true>(from, g * 16, j, GRAD_WG);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) store_piece<true>(to, g, j, GRAD_WG, zero ? (u32x4){0, 0, 0, 0} : grad_piece<T>(v[j], a.r, m, sc));
+      for (int j = 0; j < NV; ++j) store_piece<true>(to, g * 16, j, GRAD_WG, zero ? (u32x4){0, 0, 0, 0} : grad_piece<T>(v[j], a.r, m, sc));
     } else {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -1165,8 +1174,8 @@ static int launch_rows(const RowArgs& a, int* grid, hipStream_t s) {
   const int want = (a.N - 1) / Sh::ROWS + 1;
   // Parts of a wave: as many workgroups as the 256 compute units hold, which walk over the rows.  A row to a workgroup:
   // one each, as they come (5 to 10 % less than with walking ones), up to 1024 lanes, where a compute unit holds one
-  // and the next would wait for its last store (615 us against 684 at 6144 rows of 100003 bf16 classes).
-  *grid = std::min(want, G <= 64 ? 2048 : G < 1024 || DISTILL ? MAX_PARTIALS : 256);
+  // and the next would wait for its last store (581 us against 631 at 4 x 2048 ragged rows of 100003 bf16 classes).
+  *grid = std::min(want, G <= 64 ? 2048 : G < 1024 ? MAX_PARTIALS : 256);
   const size_t lds = DISTILL ? list_bytes(Sh::ROWS, a.k, NV < 16) : 0;
   if (a.dz) hipLaunchKernelGGL((k_rows<T, G, NV, DISTILL, true>), dim3(*grid), dim3(Sh::WG), lds, s, a);
   else hipLaunchKernelGGL((k_rows<T, G, NV, DISTILL, false>), dim3(*grid), dim3(Sh::WG), lds, s, a);
