@@ -13,8 +13,8 @@
 //
 // A row with its gradient is read once and written once, and takes 14 vector instructions per 16-bit logit (statistics
 // alone: 9; one of them per sweep an exponential, at a quarter of the rate).  The memory system bounds it: 8192 x 131072
-// bf16 with the gradient 820 us, 5.2 TB/s, vector units busy 0.60 of the time (a copy of that size: 4.8 TB/s); statistics
-// of 8192 x 65536 bf16 188 us, 5.7 TB/s, vector units busy 0.86.
+// bf16 with the gradient 811 us, 5.3 TB/s, vector units busy 0.59 of the time (a copy of that size: 4.8 TB/s); statistics
+// of 8192 x 65536 bf16 180 us, 6.0 TB/s, vector units busy 0.83.
 #include "d3pm_device.h"
 
 #include <algorithm>
