@@ -138,9 +138,11 @@ struct RowArgs {
   int* count; int count_here; float inv_count;                // ... over *count, which the launch finds itself with
                                                               // count_here (NULL: inv_count, every row counts)
   const float* upstream; int only_if_rescaled;                // gradient only: times *upstream; nothing to do at 1
-  float4* stats; float* per_row; double* partial; void* dz;
+  float4* stats;                                              // m, S, c, the token's logit; S = -1: not counted
+  float* per_row; double* partial; void* dz;
   float* loss; float out_scale;                               // a loss of one workgroup is written by it
 };
+__device__ __forceinline__ float4 not_counted() { return make_float4(0.0f, -1.0f, 0.0f, 0.0f); }
 // The sum of one workgroup's rows: a partial sum, or the loss.
 __device__ __forceinline__ void put_sum(const RowArgs& a, double s) {
   if (gridDim.x > 1) a.partial[blockIdx.x] = s;
@@ -638,7 +640,7 @@ __attribute__((amdgpu_waves_per_eu(WAVES_PER_SIMD<G, NV, DISTILL>))) void k_rows
       if constexpr (GRAD) zero_row<T, PEEL>(out, a.V, g, G);
       if (g == 0) {
         if (a.per_row) a.per_row[n] = 0.0f;
-        if (a.stats) a.stats[n] = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
+        if (a.stats) a.stats[n] = not_counted();
       }
       continue;
     }
@@ -760,7 +762,7 @@ __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
       if (out) zero_row<T, true>(out, a.V, g, WIDE);
       if (g == 0) {
         if (a.per_row) a.per_row[n] = 0.0f;
-        if (a.stats) a.stats[n] = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
+        if (a.stats) a.stats[n] = not_counted();
       }
       continue;
     }
@@ -886,9 +888,11 @@ __global__ __launch_bounds__(GRAD_WG) void k_token_grad(GradArgs a) {
     const int part = SPLIT ? (int)(job - (unsigned)n * (unsigned)a.chunks) : 0, lo = part * (NV * GRAD_WG);
     const bool last = !SPLIT || part == a.chunks - 1;
     const float4 st = a.r.stats[n];
-    const float c = st.z * (a.upstream ? a.upstream[(long)n * a.u_stride] : 1.0f);
+    // A row that is not counted, whatever its upstream gradient (a NaN or inf there is common: 0 times it is none), or
+    // one whose coefficient is 0: its logits are not read.
+    const float c = st.y < 0.0f ? 0.0f : st.z * (a.upstream ? a.upstream[(long)n * a.u_stride] : 1.0f);
     char* out = (char*)a.r.dz + (long)n * a.r.V * T::SIZE;
-    const bool zero = c == 0.0f;      // a row that is not counted, or whose upstream gradient is 0: its logits are not read
+    const bool zero = c == 0.0f;
     const char* row = zero ? out : row_ptr(a.r, n, T::SIZE);
     const Cut<T, PEEL> cut(row, a.r.V);
     const char* body = row + cut.head * T::SIZE;
@@ -1058,7 +1062,7 @@ __global__ __launch_bounds__(PAIR_WG) void k_pair_rows(PairArgs a) {
   for (int i = slot; i < 2 * L; i += ROWS) {
     const int n = (int)row_of(i);
     if (a.r.mask && !a.r.mask[n]) {
-      if (g == 0) stats[i] = make_float4(0.0f, -1.0f, 0.0f, 0.0f);            // S = -1: not counted
+      if (g == 0) stats[i] = not_counted();
       continue;
     }
     const char* row = row_ptr(a.r, n, T::SIZE);
@@ -1090,8 +1094,7 @@ __global__ __launch_bounds__(PAIR_WG) void k_pair_rows(PairArgs a) {
   const float2 c = pair_finish(a, p, D[0], D[1], cnt[0], cnt[1], sh);
   for (int i = threadIdx.x; i < 2 * L; i += PAIR_WG) {
     float4 st = stats[i];
-    if (st.y < 0.0f) st.y = 1.0f;
-    else st.z = i < L ? c.x : c.y;
+    if (!(st.y < 0.0f)) st.z = i < L ? c.x : c.y;
     stats[i] = st;
     a.r.stats[row_of(i)] = st;
   }
@@ -1101,7 +1104,7 @@ __global__ __launch_bounds__(PAIR_WG) void k_pair_rows(PairArgs a) {
     const int n = (int)row_of(i);
     const float4 st = stats[i];
     char* out = (char*)a.r.dz + (long)n * a.r.V * T::SIZE;
-    if (st.z == 0.0f) {
+    if (st.z == 0.0f) {                  // (of a row that is not counted too)
       zero_row<T, false>(out, a.r.V, g, G);
       continue;
     }

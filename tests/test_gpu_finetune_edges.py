@@ -1,0 +1,52 @@
+"""The fine-tuning objectives where a call is allowed but unusual: upstream gradients that are no numbers at places that
+are not counted, derivatives that these losses do not have, far log-probabilities, long sums, rows that start anywhere,
+dispatch modes and transforms.  Inputs, definitions and tolerances as in test_gpu_finetune.py unless stated."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_finetune import call, make, to_dev
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def pkg():
+    import d3pm_amd
+    return d3pm_amd
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [24, 300, 3000, 70001, 140001])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_upstream_of_a_place_that_is_not_counted(pkg, V, dtype, bad):
+    """exp(lp - old) with a NaN at a pad, or a mean over no position, sends such an upstream gradient: the gradient there
+    is 0 all the same, and the row is not looked at."""
+    d = make(V, 4, 6, V, dtype)
+    off = ~d["mask"]
+    d["logits"][off] = math.nan
+    d["tokens"][off] = -100
+    c = to_dev(d)
+    z = c["logits"].requires_grad_(True)
+    want, = torch.autograd.grad(pkg.token_logprobs(z, c["tokens"], mask=c["mask"]), z, c["up"] * c["mask"])
+    got, = torch.autograd.grad(pkg.token_logprobs(z, c["tokens"], mask=c["mask"]), z,
+                               torch.where(c["mask"], c["up"], torch.full((), bad, device="cuda")))
+    assert bool((got[off.cuda()] == 0).all())
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("name", ["distill", "preference", "policy"])
+@pytest.mark.parametrize("L,V", [(6, 24), (700, 24), (6, 3000), (6, 70001)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_loss_scale_that_is_no_number(pkg, name, L, V, bad):
+    """An upstream gradient of inf or NaN is for the counted positions only."""
+    d = make(V + L, 4, L, V, "f32")
+    off = ~d["mask"]
+    d["logits"][off] = math.nan
+    c = to_dev(d)
+    z = c["logits"].requires_grad_(True)
+    g, = torch.autograd.grad(call(pkg, name, c, z)[0], z, torch.full((), bad, device="cuda"))
+    assert bool((g[off.cuda()] == 0).all())
+    if math.isnan(bad):
+        assert bool(torch.isnan(g[c["mask"]]).all())
