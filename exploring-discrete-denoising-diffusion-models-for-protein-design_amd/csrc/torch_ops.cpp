@@ -745,9 +745,14 @@ struct ObjectiveNode : public torch::autograd::Node {
       fill(logits, saved, upstream, first, dz);
     }
     if (!twice) return {std::move(dz)};
-    // create_graph: the gradient is a value; differentiating it is an error, not a zero
-    auto error = std::make_shared<torch::autograd::DelayedError>("d3pm_mi355x: the gradient of " + name() + " cannot be differentiated", 1);
-    return (*error)({std::move(dz)});
+    // create_graph: the gradient is a value that depends on the logits and on the upstream gradient; differentiating it
+    // by either is an error, not a zero, also where it is one term of a sum
+    auto edges = torch::autograd::collect_next_edges(grads[0]);
+    edges.insert(edges.end(), next_edges().begin(), next_edges().end());
+    using torch::autograd::Error;
+    torch::autograd::set_history(dz, std::shared_ptr<Error>(new Error("d3pm_mi355x: the gradient of " + name() +
+        " cannot be differentiated", std::move(edges)), torch::autograd::deleteNode));
+    return {std::move(dz)};
   }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);

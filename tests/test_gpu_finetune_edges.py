@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_finetune import call, make, to_dev
+from test_gpu_finetune import OBJECTIVES, call, make, to_dev
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,24 @@ def test_loss_scale_that_is_no_number(pkg, name, L, V, bad):
     assert bool((g[off.cuda()] == 0).all())
     if math.isnan(bad):
         assert bool(torch.isnan(g[c["mask"]]).all())
+
+
+@pytest.mark.parametrize("name", OBJECTIVES)
+def test_the_gradient_of_a_gradient_is_an_error(pkg, name):
+    """Also where it is one term of a sum that has a gradient: not a silent zero."""
+    c = to_dev(make(103, 4, 3, 20, "f32", mask=False))
+    z = c["logits"].requires_grad_(True)
+
+    def gradient():
+        root, _ = call(pkg, name, c, z)
+        return torch.autograd.grad(root, z, torch.ones_like(root), create_graph=True)[0]
+
+    g = gradient()
+    assert g.requires_grad and bool(torch.isfinite(g).all())
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        g.sum().backward()
+    g = gradient()
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        (z.square().sum() + g.square().sum()).backward()
+    plain, = torch.autograd.grad(call(pkg, name, c, z)[0], z, None if name != "logprobs" else torch.ones(4, 3, device="cuda"))
+    assert torch.equal(plain, gradient().detach())
