@@ -765,7 +765,13 @@ struct ObjectiveNode : public torch::autograd::Node {
 template <typename N>
 std::shared_ptr<N> new_node() { return std::shared_ptr<N>(new N(), torch::autograd::deleteNode); }
 bool differentiated(const Tensor& logits) { return at::GradMode::is_enabled() && logits.requires_grad(); }
+// these losses have no forward-mode derivative: a tangent is refused, not dropped
+void need_no_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(t.defined() && t._fw_grad(0).defined()), "d3pm_mi355x: ", what,
+                              " carries a forward-mode tangent, and this loss has no forward-mode derivative");
+}
 void need_constant(const Tensor& t, const char* what) {
+  need_no_tangent(t, what);
   TORCH_CHECK_VALUE(!(t.defined() && at::GradMode::is_enabled() && t.requires_grad()), "d3pm_mi355x: ", what, " is a constant of this loss and must not require a gradient (detach it)");
 }
 
@@ -799,6 +805,7 @@ struct TokenLogprobsBackward : public ObjectiveNode {
   }
 };
 Tensor token_logprobs(const Tensor& logits, const Tensor& tokens_, const OptTensor& mask_, double temperature) {
+  need_no_tangent(logits, "logits");
   const bool want = differentiated(logits);
   Tensor tokens, lp, stats;
   {
@@ -858,6 +865,7 @@ struct DistillBackward : public ObjectiveNode {
 std::tuple<Tensor, Tensor> topk_distill_loss(const Tensor& logits, const Tensor& teacher_logits_,
                                              const Tensor& teacher_index_, const OptTensor& mask_, double temperature,
                                              double out_scale) {
+  need_no_tangent(logits, "logits");
   need_constant(teacher_logits_, "teacher_logits");
   const bool want = differentiated(logits);
   const DistillArgs args{temperature, out_scale};
@@ -919,6 +927,7 @@ std::tuple<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& token
                                        const Tensor& advantages_, const OptTensor& ref_logprobs_, const OptTensor& mask_,
                                        double temperature, double clip_low, double clip_high, double kl_coeff,
                                        double out_scale) {
+  need_no_tangent(logits, "logits");
   need_constant(old_logprobs_, "old_logprobs");
   need_constant(advantages_, "advantages");
   need_constant(opt(ref_logprobs_), "ref_logprobs");
@@ -953,6 +962,7 @@ struct PreferenceBackward : public ObjectiveNode {
 std::tuple<Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& tokens_, const OptTensor& ref_logprobs_,
                                            const OptTensor& mask_, double beta, double label_smoothing, bool average,
                                            double out_scale) {
+  need_no_tangent(logits, "logits");
   need_constant(opt(ref_logprobs_), "ref_logprobs");
   const bool want = differentiated(logits);
   Tensor tokens, loss, rewards, stats, dz;

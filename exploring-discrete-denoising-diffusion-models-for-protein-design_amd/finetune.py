@@ -10,8 +10,9 @@ Logits are float32, float16 or bfloat16 ``[..., V]`` on the GPU with any strides
 (sums over rows and sequences in float64) and the gradient is rounded once, to the logits' type.  ``mask`` (bool, the
 tokens' shape) says which positions count: the others' logits and labels are not looked at (they may hold NaN, or
 tokens that are none), their outputs and gradients are 0.  Tokens and classes outside ``[0, V)`` are clamped into it
-(a negative ``teacher_index`` marks an entry that is not there).  Only the logits are differentiated; any other
-floating input that requires a gradient is refused.
+(a negative ``teacher_index`` marks an entry that is not there).  Only the logits are differentiated, in reverse mode and
+once: any other floating input that requires a gradient, a forward-mode tangent and the gradient of a gradient are
+refused.
 
 ``out_scale=`` multiplies a loss and its gradient.  The gradient of the launch is that for an upstream gradient of 1,
 so a constant factor (a loss scaler's, 1 / accumulated batches) costs nothing there, while any other upstream gradient

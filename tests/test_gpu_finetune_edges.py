@@ -71,3 +71,19 @@ def test_the_gradient_of_a_gradient_is_an_error(pkg, name):
         (z.square().sum() + g.square().sum()).backward()
     plain, = torch.autograd.grad(call(pkg, name, c, z)[0], z, None if name != "logprobs" else torch.ones(4, 3, device="cuda"))
     assert torch.equal(plain, gradient().detach())
+
+
+@pytest.mark.parametrize("name", OBJECTIVES)
+def test_forward_mode_is_refused(pkg, name):
+    """No tangent comes out, so none is taken: of the logits, and of the inputs that are constants."""
+    import torch.autograd.forward_ad as fwd
+    c = to_dev(make(113, 4, 3, 20, "f32", mask=False))
+    floats = {"logprobs": [], "distill": ["teacher"], "preference": ["ref"], "policy": ["old", "ref", "adv"]}[name]
+    for key in ["logits"] + floats:
+        with fwd.dual_level():
+            d = {**c, key: fwd.make_dual(c[key], torch.ones_like(c[key]))}
+            with pytest.raises(NotImplementedError, match="forward"):
+                call(pkg, name, d, d["logits"])
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward"):
+                call(pkg, name, d, d["logits"])
+            call(pkg, name, c, c["logits"])                       # an ordinary call inside the level
