@@ -240,7 +240,13 @@ struct Shape {
 // The pieces of a row as a buffer resource, for the shapes whose row is the same for a whole wave: an access beyond the
 // last piece reads 0 or writes nothing, so neither loads nor stores need a branch.  (The whole offset goes into the lane
 // offset: the range check compares that with the size less the scalar offset, which must not pass the size.)
+// Its base is a multiple of 4: of the logits' pieces always (of 16, by PEEL), of the gradient's where `in_dwords` says so.
+// The gradient's rows begin elsewhere than the logits' where these are strided, in 16-bit rows of odd widths at any
+// multiple of 2: those take global stores, each behind a branch (policy loss of 2048 rows of 32003 bf16 classes: 57 us
+// where they are cut out of rows of 32004, 56 where they are dense).
 typedef __amdgpu_buffer_rsrc_t Rsrc;
+template <typename T>
+__device__ __forceinline__ bool in_dwords(const char* p) { return T::SIZE == 4 || ((uintptr_t)p & 3) == 0; }
 __device__ __forceinline__ Rsrc pieces_of(const void* body, int full) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)body, 0, full * 16, 0x00027000);
 }
@@ -582,7 +588,7 @@ __device__ __forceinline__ void grad_pieces(u32x4 (&v)[NV], float edge, const Ro
                                             char* out, int g, float m, float scale) {
   char* body = out + cut.head * T::SIZE;
   const Scale sc(scale);
-  if constexpr (G >= 64) {
+  if (G >= 64 && in_dwords<T>(body)) {
     const Rsrc to = pieces_of(body, cut.full);
     const int at = lane_offset(g);
 #pragma unroll
@@ -590,7 +596,7 @@ __device__ __forceinline__ void grad_pieces(u32x4 (&v)[NV], float edge, const Ro
       if (!holds<G, NV>(j, cut.full)) break;
       store_piece<NT>(to, at, j, G, grad_piece<T>(v[j], a, m, sc));
     }
-  } else {
+  } else if (G < 64 || T::SIZE < 4) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       if (j * G + g < cut.full) store_piece<T, NT>(body + j * (G * 16) + (uint32_t)g * 16u, grad_piece<T>(v[j], a, m, sc));
@@ -902,11 +908,19 @@ __global__ __launch_bounds__(GRAD_WG) void k_token_grad(GradArgs a) {
     u32x4 v[NV];
     if constexpr (SPLIT) {
       const int some = max(0, min(cut.full - lo, NV * GRAD_WG));
-      const Rsrc from = pieces_of(body + (long)lo * 16, zero ? 0 : some), to = pieces_of(obody + (long)lo * 16, some);
+      const Rsrc from = pieces_of(body + (long)lo * 16, zero ? 0 : some);
+      char* to = obody + (long)lo * 16;
 #pragma unroll
       for (int j = 0; j < NV; ++j) v[j] = load_piece<true>(from, g * 16, j, GRAD_WG);
+      auto piece = [&](int j) { return zero ? (u32x4){0, 0, 0, 0} : grad_piece<T>(v[j], a.r, m, sc); };
+      if (in_dwords<T>(to)) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) store_piece<true>(to, g * 16, j, GRAD_WG, zero ? (u32x4){0, 0, 0, 0} : grad_piece<T>(v[j], a.r, m, sc));
+        for (int j = 0; j < NV; ++j) store_piece<true>(pieces_of(to, some), g * 16, j, GRAD_WG, piece(j));
+      } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          if (j * GRAD_WG + g < some) store_piece<T>(to + (uint32_t)(j * GRAD_WG + g) * 16u, piece(j));
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {

@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_finetune import OBJECTIVES, call, make, to_dev
+from test_gpu_finetune import DTYPES, EPS, OBJECTIVES, call, check_grad, make, reference, to_dev
 
 pytestmark = pytest.mark.gpu
 
@@ -50,6 +50,34 @@ def test_loss_scale_that_is_no_number(pkg, name, L, V, bad):
     assert bool((g[off.cuda()] == 0).all())
     if math.isnan(bad):
         assert bool(torch.isnan(g[c["mask"]]).all())
+
+
+@pytest.mark.parametrize("V,dtype", [(1001, "bf16"), (2001, "bf16"), (4099, "f16"), (9001, "bf16"), (16411, "bf16"),
+                                     (32003, "bf16"), (65001, "f16"), (100003, "bf16"), (131077, "bf16"), (2051, "f32"),
+                                     (33001, "f32"), (65543, "f32")])
+@pytest.mark.parametrize("kind", ["shift", "padded"])
+@pytest.mark.parametrize("name", OBJECTIVES)
+def test_gradient_rows_that_start_elsewhere(pkg, name, kind, V, dtype):
+    """Odd widths out of strided rows: a row of the gradient lies at another alignment than the logits' row."""
+    B, L = 4, 3
+    dt = DTYPES[dtype]
+    d = make(V, B, L, V, dtype, k=16)
+    base = torch.randn((B, L + 1, V) if kind == "shift" else (B, L, V + 2), generator=torch.Generator().manual_seed(V)).to(dt)
+    view = (lambda t: t[:, :-1]) if kind == "shift" else (lambda t: t[..., 1:V + 1])
+    d["logits"] = view(base).contiguous()
+    out, grad, bound = reference(name, d)
+    c = to_dev(d)
+    z = view(base.cuda()).requires_grad_(True)
+    assert not z.is_contiguous()
+    root, got = call(pkg, name, c, z)
+    g, = torch.autograd.grad(root, z, c["up"] * c["mask"] if name == "logprobs" else None)
+    assert g.is_contiguous()
+    check_grad(g, grad, bound, dt)
+    # (not bit for bit a contiguous call's: the pieces begin elsewhere in the row, so its terms are added in another order)
+    for k in ("lp", "rewards", "loss"):
+        if k in out:
+            diff = (got[k].detach().cpu().double() - out[k]).abs()
+            assert bool((diff <= out[k + "_tol"] + EPS * out[k].abs()).all())
 
 
 @pytest.mark.parametrize("name", OBJECTIVES)
