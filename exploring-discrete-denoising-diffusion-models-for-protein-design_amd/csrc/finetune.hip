@@ -896,7 +896,8 @@ __global__ __launch_bounds__(GRAD_WG) void k_token_grad(GradArgs a) {
     const float4 st = a.r.stats[n];
     // A row that is not counted, whatever its upstream gradient (a NaN or inf there is common: 0 times it is none), or
     // one whose coefficient is 0: its logits are not read.
-    const float c = st.y < 0.0f ? 0.0f : st.z * (a.upstream ? a.upstream[(long)n * a.u_stride] : 1.0f);
+    const float u = a.upstream ? a.upstream[(long)n * a.u_stride] : 1.0f;      // (asked for with the statistics)
+    const float c = st.y < 0.0f ? 0.0f : st.z * u;
     char* out = (char*)a.r.dz + (long)n * a.r.V * T::SIZE;
     const bool zero = c == 0.0f;
     const char* row = zero ? out : row_ptr(a.r, n, T::SIZE);
