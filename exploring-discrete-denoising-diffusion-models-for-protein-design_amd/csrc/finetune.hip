@@ -422,6 +422,13 @@ __device__ __forceinline__ RowSum wave_sum(u32x4 (&v)[NV], float edge, float mx,
     return RowSum{mx, group_sum<GL>(s0 + s1), 0.0f};
   }
 }
+// What a sum taken against a maximum counts for against one that is higher by -d.  (EXP2_LOW: of this exponential; at
+// d = 0 there is none)
+__device__ __forceinline__ double share_of(float d, const RowArgs& a) {
+  float low = 0.0f;
+  const float e = exp_parts(d, a, low);
+  return e == 1.0f ? 1.0 : fma((double)low, LN2, (double)e) * (1.0 + EXP2_LOW);
+}
 // (Lane l of a wave takes the entry of wave l % WAVES, and the lanes add up among themselves.)
 template <int WAVES, bool EXACT>
 __device__ __forceinline__ RowSum join_stats(const float2* red, const float* red_lo, const RowArgs& a) {
@@ -429,11 +436,7 @@ __device__ __forceinline__ RowSum join_stats(const float2* red, const float* red
   const float2 r = red[w];
   const float m = fmaxf(group_max<WAVES>(r.x), -FLT_MAX);
   if constexpr (!EXACT) return in_parts(m, group_sum<WAVES>((double)(r.y * exp_d(r.x - m, a.c_hi, a.c_lo))));
-  float low = 0.0f;
-  const float e = exp_parts(r.x - m, a, low);
-  // (EXP2_LOW: of this exponential; a wave that holds the maximum has 1)
-  const double share = e == 1.0f ? 1.0 : fma((double)low, LN2, (double)e) * (1.0 + EXP2_LOW);
-  return in_parts(m, group_sum<WAVES>(((double)r.y + (double)red_lo[w]) * share));
+  return in_parts(m, group_sum<WAVES>(((double)r.y + (double)red_lo[w]) * share_of(r.x - m, a)));
 }
 
 template <typename T, int G, int NV, bool KEEP, bool EXACT>
@@ -754,6 +757,7 @@ template <typename T, bool DISTILL>
 __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
   constexpr int E = T::E;
   __shared__ float2 red[2][WIDE / 64];
+  __shared__ float red_lo[2][WIDE / 64];
   __shared__ int kept_flag[2];
   extern __shared__ __align__(16) char lists[];
   if (a.only_if_rescaled && *a.upstream == 1.0f) return;
@@ -777,9 +781,11 @@ __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
     const char* body = row + cut.head * T::SIZE;
     char* obody = out + cut.head * T::SIZE;
     const float edge = cut.has_edge(g) ? T::get(row, cut.edge(g)) : -INFINITY;
-    // the lane's running maximum and sum
+    // The lane's running maximum and sum.  The sum is held in 64 bits: a lane of the widest rows adds 131072 terms, and
+    // what a float32 addition of equal terms rounds away is the same every time (6e-5 of S at 4 M classes).  Two chains
+    // of at most 16 additions stay in float32.
     float mx = fmaxf(edge, -FLT_MAX);
-    float s = exp_d(edge - mx, a.c_hi, a.c_lo);
+    double s = (double)exp_d(edge - mx, a.c_hi, a.c_lo);
     float f[E];
     for (int j = g; j < cut.full; j += 4 * WIDE) {       // four pieces on their way at a time
       u32x4 v[4];
@@ -795,14 +801,19 @@ __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
 #pragma unroll
         for (int e = 0; e < E; ++e) top = fmaxf(top, f[e]);
       }
-      s *= exp_d(mx - top, a.c_hi, a.c_lo);
+      if (top > mx) s *= share_of(mx - top, a);
       mx = top;
+      float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         T::unpack(v[u], f);
 #pragma unroll
-        for (int e = 0; e < E; ++e) s += exp_d(f[e] - mx, a.c_hi, a.c_lo);
+        for (int e = 0; e < E; e += 2) {
+          s0 += exp_d(f[e] - mx, a.c_hi, a.c_lo);
+          s1 += exp_d(f[e + 1] - mx, a.c_hi, a.c_lo);
+        }
       }
+      s += (double)s0 + (double)s1;
     }
     int y = 0;
     float zy = 0.0f;
@@ -817,14 +828,14 @@ __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
       }
     }
     const float mw = group_max<64>(mx);
-    s = group_sum<64>(s * exp_d(mx - mw, a.c_hi, a.c_lo));
-    if ((g & 63) == 0) red[phase][wave] = make_float2(mw, s);
+    const RowSum part = in_parts(mw, group_sum<64>(s * share_of(mx - mw, a)));
+    if ((g & 63) == 0) {
+      red[phase][wave] = make_float2(mw, part.hi);
+      red_lo[phase][wave] = part.lo;
+    }
     __syncthreads();
-    float m = -FLT_MAX;
-    for (int i = 0; i < WIDE / 64; ++i) m = fmaxf(m, red[phase][i].x);
-    double sum = 0.0;
-    for (int i = 0; i < WIDE / 64; ++i) sum += (double)(red[phase][i].y * exp_d(red[phase][i].x - m, a.c_hi, a.c_lo));
-    const float S = (float)sum;
+    const RowSum st = join_stats<WIDE / 64, true>(red[phase], red_lo[phase], a);
+    const float m = st.m, S = st.hi;
 
     float c, scale;
     const float inv_S = rcp_acc(S);
@@ -833,7 +844,7 @@ __global__ __launch_bounds__(WIDE) void k_rows_wide(RowArgs a) {
       const TokenOut o = token_head(a, n, zy - m, S);
       if (g == 0) {
         if (a.per_row) a.per_row[n] = o.lp;
-        if (a.stats) a.stats[n] = make_float4(m, S, a.head == HEAD_LOGPROB ? a.inv_tau : 0.0f, zy);
+        if (a.stats) a.stats[n] = make_float4(m, S, a.head == HEAD_LOGPROB ? a.inv_tau : st.lo, zy);
         acc += (double)o.loss;
       }
       c = w * o.c;

@@ -115,3 +115,43 @@ def test_forward_mode_is_refused(pkg, name):
             with torch.no_grad(), pytest.raises(NotImplementedError, match="forward"):
                 call(pkg, name, d, d["logits"])
             call(pkg, name, c, c["logits"])                       # an ordinary call inside the level
+
+
+@pytest.mark.parametrize("V,dtype", [(1 << 18, "f32"), ((1 << 20) + 5, "bf16"), ((1 << 22) + 3, "f32"), ((1 << 22) + 3, "bf16")])
+def test_sums_of_long_rows(pkg, V, dtype):
+    """Rows of equal classes behind M higher ones, which every lane meets first: every later term of the sum is the same
+    number, so what the additions lose adds up (4096 float32 additions of exp(-87/128): 1010 eps).  S = M + (V - M) e,
+    e = exp(-87/128): the exponent's rounding and the instruction's ulp make 1.5 + 2 eps of e, a lane's float32 additions
+    (16 of them at most, the rest in 64 bits) 16 eps: 20 eps of log S, and |lp| eps for the output's rounding (the type's)."""
+    M = 8208
+    z = torch.full((2, 3, V), -87.0 / 128.0, dtype=DTYPES[dtype])     # (a number of all types)
+    z[..., :M] = 0.0
+    y = torch.tensor([[0, M // 2, M - 1], [1, 7, M - 2]])
+    lp = -math.log(M + (V - M) * math.exp(-87.0 / 128.0))
+    z, y = z.cuda(), y.cuda()
+    assert float((pkg.token_logprobs(z, y).double() - lp).abs().max()) <= (20 + abs(lp)) * EPS
+    fn = pkg.PreferenceLoss(beta=1.0)
+    ref = torch.full((2, 3), lp, dtype=torch.float32, device="cuda")
+    fn(z, y, ref)
+    want = 3 * (lp - float(ref[0, 0]))
+    assert float((fn.rewards.double() - want).abs().max()) <= 3 * 20 * EPS
+    fn = pkg.PolicyLoss(clip_low=1.0, clip_high=1e6)
+    loss = fn(z, y, ref, torch.ones(2, 3, device="cuda"))
+    # the ratio: exp of a small number (2 eps), the mean's rounding; S and its logarithm as float32 (4 eps)
+    assert abs(float(loss) + math.exp(lp - float(ref[0, 0]))) <= (20 + 8) * EPS
+
+
+@pytest.mark.parametrize("L,V,dtype", [(263, 24, "f32"), (263, 24, "bf16"), (300, 60, "f32")])
+def test_rewards_of_long_sequences(pkg, L, V, dtype):
+    """A reward is a long sum of small differences of large terms.  Per row the instruction's error (within one ulp,
+    2 eps, either way: at most 1 eps in the root mean square) is what is left of S in 64 bits, whatever its sign, and its
+    mean is taken off: sqrt(L) eps over a sequence, in the root mean square over the sequences, + the reward's rounding."""
+    d = make(L + V, 64, L, V, dtype, mask=False)
+    d["ref"] = torch.log_softmax(d["logits"].double(), -1).gather(-1, d["tokens"][..., None])[..., 0].float()
+    lp = torch.log_softmax(d["logits"].double(), -1).gather(-1, d["tokens"][..., None])[..., 0]
+    want = (lp - d["ref"].double()).sum(1)
+    c = to_dev(d)
+    fn = pkg.PreferenceLoss(beta=1.0)
+    fn(c["logits"], c["tokens"], c["ref"])
+    err = fn.rewards.cpu().double() - want
+    assert float(err.square().mean().sqrt()) <= math.sqrt(L) * EPS + EPS * float(want.abs().max())
