@@ -129,7 +129,7 @@ __device__ __forceinline__ void store_piece(char* p, u32x4 v) {
 struct RowArgs {
   const void* z; long sb, sl; int L, V, N; int dense;         // dense: row n lies at n * sl
   const void* tokens; int tok_bytes; const uint8_t* mask;
-  float c_hi, c_lo, inv_tau;                                  // log2(e) / tau in two floats; 1 / tau
+  float c_hi, c_lo, inv_tau, inv_tau_lo;                      // log2(e) / tau and 1 / tau, each in two floats
   float d_min;                                                // z - m from which on exp((z - m) / tau) is 0
   int head;
   const float* old_lp; const float* ref_lp; const float* adv; int adv_per_seq; float clip_lo, clip_hi, kl_coeff;
@@ -179,15 +179,16 @@ __device__ __forceinline__ float exp_rest(float x) {
   return fabsf(x) < 0.35f ? x * x * q : exp_any(x) - 1.0f - x;
 }
 
-// (z - m) / tau - log S as hi + lo, to about 4e-8 whatever its size (of -8, float32 keeps 2.4e-7): with S = 2^e f, e ln 2 is
-// taken off in one exact step and a second for its rest, and what rounds there is kept.
+// (z - m) / tau - log S as hi + lo, to about 4e-8 whatever its size (of -8, float32 keeps 2.4e-7): 1 / tau is there in two
+// floats (of one, -60 would be 2e-6 off at tau = 1.7, in every row the same way), with S = 2^e f, e ln 2 is taken off in
+// one exact step and a second for its rest, and what rounds there is kept.
 struct LogProb { float hi, lo; };
-__device__ __forceinline__ LogProb log_prob(float zy_m, float inv_tau, float S) {
+__device__ __forceinline__ LogProb log_prob(float zy_m, float inv_tau, float inv_tau_lo, float S) {
 #pragma clang fp contract(off)
   const float e = (float)__builtin_amdgcn_frexp_expf(S);
   const float K = e * 0.693145752f;                                      // ln 2 to 16 bits: exact
   const float k = fmaf(e, 1.42860677e-6f, logf(__builtin_amdgcn_frexp_mantf(S)));
-  const float p = zy_m * inv_tau, p_lo = fmaf(zy_m, inv_tau, -p);
+  const float p = zy_m * inv_tau, p_lo = fmaf(zy_m, inv_tau_lo, fmaf(zy_m, inv_tau, -p));
   const float s = p - K, b = s - p;
   const float s_lo = (p - (s - b)) - (K + b);
   return LogProb{s, fabsf(s) < INFINITY ? s_lo + p_lo - k : -k};         // (a token ruled out: -inf)
@@ -201,7 +202,7 @@ __device__ __forceinline__ LogProb log_prob(float zy_m, float inv_tau, float S) 
 struct TokenOut { float lp, loss, c; };
 __device__ __forceinline__ TokenOut token_head(const RowArgs& a, int n, float zy_m, float S) {
   TokenOut o;
-  const LogProb lp = log_prob(zy_m, a.inv_tau, S);
+  const LogProb lp = log_prob(zy_m, a.inv_tau, a.inv_tau_lo, S);
   o.lp = lp.hi + lp.lo;
   o.loss = 0.0f;
   o.c = 1.0f;
@@ -1173,13 +1174,15 @@ static int check_int_bytes(int b, const char* what, const char* who) {
   return D3PM_OK;
 }
 
-// log2(e) / tau in two floats, the second above 0: a class ruled out with -inf stays -inf in both products of exp_d
-static void set_temperature(float tau, float* c_hi, float* c_lo, float* inv_tau) {
+// log2(e) / tau and 1 / tau, each in two floats.  The second of log2(e) / tau is above 0: a class ruled out with -inf
+// stays -inf in both products of exp_d.
+static void set_temperature(float tau, float* c_hi, float* c_lo, float* inv_tau, float* inv_tau_lo) {
   const double c = 1.44269504088896340736 / (double)tau;
   *c_hi = (float)c;
   if ((double)*c_hi >= c) *c_hi = std::nextafterf(*c_hi, 0.0f);
   *c_lo = (float)(c - (double)*c_hi);
   *inv_tau = (float)(1.0 / (double)tau);
+  *inv_tau_lo = (float)(1.0 / (double)tau - (double)*inv_tau);
 }
 static bool is_dense(const d3pm_logits* z) { return z->B <= 1 || z->stride_b == z->L * z->stride_l; }
 
@@ -1187,7 +1190,7 @@ static RowArgs row_args(const d3pm_logits* z, float tau) {
   RowArgs a{};
   a.z = z->data; a.sb = z->stride_b; a.sl = z->stride_l;
   a.L = (int)z->L; a.V = z->V; a.N = (int)(z->B * z->L); a.dense = is_dense(z) ? 1 : 0;
-  set_temperature(tau, &a.c_hi, &a.c_lo, &a.inv_tau);
+  set_temperature(tau, &a.c_hi, &a.c_lo, &a.inv_tau, &a.inv_tau_lo);
   a.d_min = -200.0f * tau;                                    // (exp2 of -288)
   a.inv_count = 1.0f;
   return a;

@@ -155,3 +155,23 @@ def test_rewards_of_long_sequences(pkg, L, V, dtype):
     fn(c["logits"], c["tokens"], c["ref"])
     err = fn.rewards.cpu().double() - want
     assert float(err.square().mean().sqrt()) <= math.sqrt(L) * EPS + EPS * float(want.abs().max())
+
+
+@pytest.mark.parametrize("V", [24, 2000, 70001])
+@pytest.mark.parametrize("tau", [0.3, 1.3, 1.7, 3.0])
+def test_ratios_of_improbable_tokens(pkg, V, tau):
+    """The log-probability's two parts hold (z - m) / tau whatever its size.  With old = lp rounded to float32 the ratio
+    is exp of a difference of at most half a step of lp: its error is that of lp, log S (4 eps: the exponentials' ulp, the
+    sum's rounding to float32, the logarithm's ulp) and 2 eps of the parts' own last additions, plus 2 eps of the
+    exponential and 1 eps of the mean's rounding; a row's float32 additions (V > 256) add up to 35 eps."""
+    g = torch.Generator().manual_seed(V)
+    z = torch.randn(4, 8, V, generator=g)
+    z[..., 0] = 30.0
+    y = torch.randint(1, V, (4, 8), generator=g)
+    t32 = float(torch.tensor(tau, dtype=torch.float32))           # tau as the library takes it
+    lp = torch.log_softmax(z.double() / t32, -1).gather(-1, y[..., None])[..., 0]
+    old = lp.float()
+    fn = pkg.PolicyLoss(clip_low=1.0, clip_high=1e6, temperature=tau)
+    loss = fn(z.cuda(), y.cuda(), old.cuda(), torch.ones(4, 8, device="cuda"))
+    want = -torch.exp(lp - old.double()).mean()
+    assert abs(float(loss) - float(want)) <= (9 + (35 if V > 256 else 0)) * EPS * float(want.abs())
