@@ -623,29 +623,42 @@ int float_dtype(const Tensor& t, const char* what) {
 void need_same_device(const Tensor& t, const Tensor& z, const char* what) {
   TORCH_CHECK(t.device() == z.device(), "d3pm_mi355x: ", what, " is on ", t.device(), ", the logits on ", z.device());
 }
-// The library's view of logits [B, ..., V]: `rows` keeps the tensor that it points into (a copy where the middle
-// dimensions cannot be walked with one stride, or the classes do not lie side by side).
+// Whether logits [B, ..., V] are rows as the library walks them: classes side by side, the middle dimensions with one
+// stride (`inner`; -1: there is one position to a sequence).
+bool in_rows(const Tensor& z, int64_t* inner) {
+  *inner = -1;
+  if (z.dim() < 2) return false;
+  bool walk = z.size(-1) == 1 || z.stride(-1) == 1;
+  int64_t next = 0;                             // what the next middle dimension's stride must be
+  for (int64_t i = z.dim() - 2; i >= 1 && walk; --i) {
+    if (z.size(i) == 1) continue;
+    if (*inner < 0) *inner = z.stride(i);
+    else walk = z.stride(i) == next;
+    next = z.stride(i) * z.size(i);
+  }
+  return walk;
+}
+// Logits as such rows: themselves, or a copy.  A loss makes it once and keeps it for its gradient.
+Tensor as_rows(const Tensor& z) {
+  int64_t inner;
+  return z.dim() < 2 || in_rows(z, &inner) ? z : z.contiguous();
+}
+// The library's view of them: `rows` keeps the tensor that it points into.
 struct LogitsView { Tensor rows; d3pm_logits desc; };
 LogitsView logits_view(const Tensor& z, at::IntArrayRef per_row, const char* per_row_name) {
   TORCH_CHECK(z.is_cuda(), "d3pm_mi355x: logits must live on an MI355X (device='cuda'); there is no CPU path");
   TORCH_CHECK_VALUE(z.dim() >= 2 && z.sizes().slice(0, z.dim() - 1) == per_row,
                     "d3pm_mi355x: logits must have the shape of ", per_row_name, " and a trailing class dimension, got ",
                     z.sizes(), " and ", per_row);
-  const int64_t nd = z.dim(), V = z.size(-1);
+  const int64_t V = z.size(-1);
   TORCH_CHECK_VALUE(V >= 1 && V <= (1 << 27), "d3pm_mi355x: logits have ", V, " classes, need 1 .. 2^27");
   LogitsView v{z, {}};
   v.desc.dtype = float_dtype(z, "logits");
   v.desc.V = (int)V;
   v.desc.B = z.size(0);
   v.desc.L = v.desc.B ? z.numel() / V / v.desc.B : 0;
-  bool walk = V == 1 || z.stride(-1) == 1;
-  int64_t inner = -1, next = 0;                 // stride of the innermost middle dimension; what the next one must be
-  for (int64_t i = nd - 2; i >= 1 && walk; --i) {
-    if (z.size(i) == 1) continue;
-    if (inner < 0) inner = z.stride(i);
-    else walk = z.stride(i) == next;
-    next = z.stride(i) * z.size(i);
-  }
+  int64_t inner;
+  const bool walk = in_rows(z, &inner);
   if (!walk) v.rows = z.contiguous();
   v.desc.stride_b = walk ? z.stride(0) : v.desc.L * V;
   v.desc.stride_l = !walk ? V : inner >= 0 ? inner : v.desc.stride_b;
@@ -713,8 +726,9 @@ struct ObjectiveNode : public torch::autograd::Node {
   unsigned long long capture_ = 0;       // that the loss launch was in
   bool released_ = false;
 
-  void save(const Tensor& logits, std::initializer_list<Tensor> others) {
-    logits_ = SavedVariable(logits, false);
+  // rows: the logits, or their copy
+  void save(const Tensor& logits, const Tensor& rows, std::initializer_list<Tensor> others) {
+    logits_ = SavedVariable(rows, false);
     for (const Tensor& t : others) saved_.emplace_back(t, false);
     set_next_edges(torch::autograd::collect_next_edges(logits));
   }
@@ -807,15 +821,16 @@ struct TokenLogprobsBackward : public ObjectiveNode {
 Tensor token_logprobs(const Tensor& logits, const Tensor& tokens_, const OptTensor& mask_, double temperature) {
   need_no_tangent(logits, "logits");
   const bool want = differentiated(logits);
-  Tensor tokens, lp, stats;
+  Tensor rows, tokens, lp, stats;
   {
     at::AutoDispatchBelowADInplaceOrView below;
+    rows = as_rows(logits);
     tokens = dense(tokens_);
-    std::tie(lp, stats) = token_logprobs_run(logits, tokens, dense(opt(mask_)), temperature, want);
+    std::tie(lp, stats) = token_logprobs_run(rows, tokens, dense(opt(mask_)), temperature, want);
   }
   if (want) {
     auto node = new_node<TokenLogprobsBackward>();
-    node->save(logits, {tokens, stats});
+    node->save(logits, rows, {tokens, stats});
     node->temperature = temperature;
     torch::autograd::set_history(lp, node);
   }
@@ -869,16 +884,17 @@ std::tuple<Tensor, Tensor> topk_distill_loss(const Tensor& logits, const Tensor&
   need_constant(teacher_logits_, "teacher_logits");
   const bool want = differentiated(logits);
   const DistillArgs args{temperature, out_scale};
-  Tensor teacher_logits, teacher_index, mask, loss, per, dz, ws;
+  Tensor rows, teacher_logits, teacher_index, mask, loss, per, dz, ws;
   {
     at::AutoDispatchBelowADInplaceOrView below;
+    rows = as_rows(logits);
     teacher_logits = dense(teacher_logits_); teacher_index = dense(teacher_index_); mask = dense(opt(mask_));
     if (want) dz = grad_buffer(logits);
-    distill_run(logits, teacher_logits, teacher_index, mask, args, nullptr, false, &loss, &per, dz, ws);
+    distill_run(rows, teacher_logits, teacher_index, mask, args, nullptr, false, &loss, &per, dz, ws);
   }
   if (want) {
     auto node = new_node<DistillBackward>();
-    node->save(logits, {teacher_logits, teacher_index, mask, ws});
+    node->save(logits, rows, {teacher_logits, teacher_index, mask, ws});
     node->keep_gradient(std::move(dz));
     node->args = args;
     torch::autograd::set_history(loss, node);
@@ -933,17 +949,18 @@ std::tuple<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& token
   need_constant(opt(ref_logprobs_), "ref_logprobs");
   const bool want = differentiated(logits);
   const PolicyArgs args{temperature, clip_low, clip_high, kl_coeff, out_scale};
-  Tensor tokens, old_logprobs, advantages, ref_logprobs, mask, loss, lp, dz, ws;
+  Tensor rows, tokens, old_logprobs, advantages, ref_logprobs, mask, loss, lp, dz, ws;
   {
     at::AutoDispatchBelowADInplaceOrView below;
+    rows = as_rows(logits);
     tokens = dense(tokens_); old_logprobs = dense_f32(old_logprobs_); advantages = dense_f32(advantages_);
     ref_logprobs = dense_f32(opt(ref_logprobs_)); mask = dense(opt(mask_));
     if (want) dz = grad_buffer(logits);
-    policy_run(logits, tokens, old_logprobs, advantages, ref_logprobs, mask, args, nullptr, false, &loss, &lp, dz, ws);
+    policy_run(rows, tokens, old_logprobs, advantages, ref_logprobs, mask, args, nullptr, false, &loss, &lp, dz, ws);
   }
   if (want) {
     auto node = new_node<PolicyBackward>();
-    node->save(logits, {tokens, old_logprobs, advantages, ref_logprobs, mask, ws});
+    node->save(logits, rows, {tokens, old_logprobs, advantages, ref_logprobs, mask, ws});
     node->keep_gradient(std::move(dz));
     node->args = args;
     torch::autograd::set_history(loss, node);
@@ -965,13 +982,14 @@ std::tuple<Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& t
   need_no_tangent(logits, "logits");
   need_constant(opt(ref_logprobs_), "ref_logprobs");
   const bool want = differentiated(logits);
-  Tensor tokens, loss, rewards, stats, dz;
+  Tensor rows, tokens, loss, rewards, stats, dz;
   {
     at::AutoDispatchBelowADInplaceOrView below;
     D3PM_GUARD(logits);
     tokens = dense(tokens_);
     const Tensor ref_logprobs = dense_f32(opt(ref_logprobs_)), mask = dense(opt(mask_));
-    auto v = logits_view(logits, tokens.sizes(), "tokens");
+    rows = as_rows(logits);
+    auto v = logits_view(rows, tokens.sizes(), "tokens");
     const int t_bytes = token_bytes(tokens, logits, "tokens");
     const float* ref = ref_logprobs.defined() ? row_f32(ref_logprobs, tokens, logits, "ref_logprobs and tokens") : nullptr;
     const uint8_t* m = mask_ptr(mask, tokens.sizes(), logits);
@@ -988,7 +1006,7 @@ std::tuple<Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& t
   }
   if (want) {
     auto node = new_node<PreferenceBackward>();
-    node->save(logits, {tokens, stats});
+    node->save(logits, rows, {tokens, stats});
     node->keep_gradient(std::move(dz));
     torch::autograd::set_history(loss, node);
   }

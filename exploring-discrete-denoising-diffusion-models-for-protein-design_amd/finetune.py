@@ -6,7 +6,9 @@ package: the gradient at the logits comes out of the launch that computes the lo
   PreferenceLoss    pairs of sequences, the first of each preferred: -log sigmoid of the difference of log-ratios
   PolicyLoss        clipped ratio of new to old probabilities times an advantage, with a KL term
 
-Logits are float32, float16 or bfloat16 ``[..., V]`` on the GPU with any strides; everything is computed in float32
+Logits are float32, float16 or bfloat16 ``[..., V]`` on the GPU with any strides (where the classes do not lie side by
+side, or the positions of a sequence do not follow each other with one stride, they are copied into rows once, and the
+copy is kept for the gradient in their place); everything is computed in float32
 (sums over rows and sequences in float64) and the gradient is rounded once, to the logits' type.  ``mask`` (bool, the
 tokens' shape) says which positions count: the others' logits and labels are not looked at (they may hold NaN, or
 tokens that are none), their outputs and gradients are 0.  Tokens and classes outside ``[0, V)`` are clamped into it

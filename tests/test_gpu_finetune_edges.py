@@ -175,3 +175,30 @@ def test_ratios_of_improbable_tokens(pkg, V, tau):
     loss = fn(z.cuda(), y.cuda(), old.cuda(), torch.ones(4, 8, device="cuda"))
     want = -torch.exp(lp - old.double()).mean()
     assert abs(float(loss) - float(want)) <= (9 + (35 if V > 256 else 0)) * EPS * float(want.abs())
+
+
+@pytest.mark.parametrize("name", OBJECTIVES)
+@pytest.mark.parametrize("kind", ["classes_apart", "odd_middle"])
+def test_backward_makes_no_second_copy(pkg, name, kind):
+    """Logits that are copied into rows are copied once, in the forward call."""
+    B, L, V = 4, 32, 4096
+    d = make(115, B, L, V, "f32", mask=False)
+    c = to_dev(d)
+    if kind == "classes_apart":
+        z = c["logits"].transpose(1, 2).contiguous().transpose(1, 2)
+    else:                                                     # [B, L / 4, 4, V] whose middle dimensions are swapped
+        c = {k: (v.reshape((B, L // 4, 4) + v.shape[2:]) if torch.is_tensor(v) else v) for k, v in c.items()}
+        z = c["logits"].transpose(1, 2).contiguous().transpose(1, 2)
+    z = z.detach().requires_grad_(True)
+    size = z.numel() * z.element_size()
+    up = c["up"] if name == "logprobs" else torch.ones((), device="cuda")
+    flat = z.detach().contiguous().requires_grad_(True)
+    want, = torch.autograd.grad(call(pkg, name, c, flat)[0], flat, up)
+    root, _ = call(pkg, name, c, z)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got, = torch.autograd.grad(root, z, up)
+    grown = torch.cuda.max_memory_allocated() - before
+    assert torch.equal(got, want)
+    assert grown < (1.5 if name == "logprobs" else 0.5) * size      # (a log-probability's gradient is made in backward)
