@@ -11,6 +11,8 @@
 #include <ATen/ATen.h>
 #include <ATen/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <ATen/core/dispatch/Dispatcher.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -678,6 +680,7 @@ const uint8_t* mask_ptr(const Tensor& m, at::IntArrayRef per_row, const Tensor& 
 Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
 Tensor dense_f32(const Tensor& t) { return t.defined() ? (t.scalar_type() == at::kFloat ? t : t.to(at::kFloat)).contiguous() : t; }
 Tensor opt(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+OptTensor as_opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 const float* row_f32(const Tensor& t, const Tensor& per_row, const Tensor& z, const char* what) {
   need_same_device(t, z, what);
   need_same_shape(t, per_row, what);
@@ -694,8 +697,25 @@ const float* upstream_ptr(const Tensor& u, const Tensor& z) {
   need_numel(u, 1, "upstream");
   return f32(u, "upstream");
 }
-Tensor objective_workspace(const d3pm_logits& d, const Tensor& z) {
-  return at::empty({(int64_t)(d3pm_objective_workspace(d.B, d.L) / 8 + 1)}, z.options().dtype(at::kDouble));
+int64_t workspace_doubles(const Tensor& z) {
+  const long B = z.dim() ? z.size(0) : 0, L = z.dim() > 1 && z.numel() ? z.numel() / z.size(-1) / B : 0;
+  return (int64_t)(d3pm_objective_workspace(B, L) / 8 + 1);
+}
+Tensor objective_workspace(const Tensor& z) { return at::empty({workspace_doubles(z)}, z.options().dtype(at::kDouble)); }
+// the workspace of a loss call, for its gradient alone
+Tensor need_workspace(const Tensor& ws, const Tensor& z) {
+  need_device(ws, "workspace");
+  need_same_device(ws, z, "workspace");
+  TORCH_CHECK(ws.scalar_type() == at::kDouble, "d3pm_mi355x: workspace must be float64");
+  need_numel(ws, workspace_doubles(z), "workspace");
+  return ws;
+}
+void* grad_ptr(const Tensor& dz, const Tensor& z) {
+  need_device(dz, "dlogits");
+  need_same_device(dz, z, "dlogits");
+  need_same_shape(dz, z, "dlogits and logits");
+  TORCH_CHECK(dz.scalar_type() == z.scalar_type(), "d3pm_mi355x: dlogits must have the logits' type");
+  return dz.data_ptr();
 }
 Tensor grad_buffer(const Tensor& z) { return at::empty(z.sizes(), z.options().memory_format(at::MemoryFormat::Contiguous)); }
 
@@ -705,11 +725,27 @@ Tensor grad_buffer(const Tensor& z) { return at::empty(z.sizes(), z.options().me
 // after a launch that does it again only if the upstream gradient is another number, and a second backward
 // (retain_graph) fills a buffer of its own.  So does a backward that is captured into another graph than its forward, or
 // captured without it: a replay would find the buffer as the last one left it, not as the forward fills it.
+//
+// The autograd kernel of an operator calls, through the dispatcher, the operator itself (no gradient wanted) or one of
+// underscored name that returns what the node keeps too; backward calls one that fills the gradient.  So dispatch modes
+// and transforms see what runs.  Those operators are not differentiable themselves: their derivative is an error.
 using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
-// the capture that the current stream is in, 0 if none
-unsigned long long capture_id() {
+template <typename F>
+c10::TypedOperatorHandle<F> op_handle(const char* name, F*) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+// the operator that `run` is the device kernel of
+#define D3PM_CALL(name, run, ...)                                            \
+  ([&] {                                                                     \
+    static const auto op_ = op_handle("d3pm_mi355x::" name, &run);           \
+    return op_.call(__VA_ARGS__);                                            \
+  }())
+
+// the capture that the current stream of the tensor's device is in, 0 if none
+unsigned long long capture_id(const Tensor& on) {
+  D3PM_GUARD(on);
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   unsigned long long id = 0;
   if (hipStreamGetCaptureInfo((hipStream_t)stream(), &status, &id) != hipSuccess) {
@@ -718,6 +754,9 @@ unsigned long long capture_id() {
   }
   return status == hipStreamCaptureStatusActive ? id + 1 : 0;
 }
+
+// a gradient, as a function of the logits and the upstream gradient without a derivative
+Tensor once_differentiable(const Tensor& grad, const Tensor&, const Tensor&) { return grad.clone(); }
 
 struct ObjectiveNode : public torch::autograd::Node {
   SavedVariable logits_;
@@ -734,7 +773,7 @@ struct ObjectiveNode : public torch::autograd::Node {
   }
   void keep_gradient(Tensor&& dz) {
     dz_ = std::move(dz);
-    capture_ = capture_id();
+    capture_ = capture_id(dz_);
   }
   // the gradient for `upstream` into dz; only_if_rescaled: dz holds that for an upstream gradient of 1
   virtual void fill(const Tensor& logits, const std::vector<Tensor>& saved, const Tensor& upstream,
@@ -753,7 +792,7 @@ struct ObjectiveNode : public torch::autograd::Node {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       const Tensor upstream = grads[0].contiguous();
-      const bool first = dz_.defined() && capture_ == capture_id();
+      const bool first = dz_.defined() && capture_ == capture_id(logits);
       dz = first ? std::move(dz_) : at::empty(logits.sizes(), logits.options().memory_format(at::MemoryFormat::Contiguous));
       dz_.reset();
       fill(logits, saved, upstream, first, dz);
@@ -761,6 +800,8 @@ struct ObjectiveNode : public torch::autograd::Node {
     if (!twice) return {std::move(dz)};
     // create_graph: the gradient is a value that depends on the logits and on the upstream gradient; differentiating it
     // by either is an error, not a zero, also where it is one term of a sum
+    if (dz.key_set().has(c10::DispatchKey::FuncTorchGradWrapper))      // nested transforms: in the graph of each of them
+      dz = D3PM_CALL("_once_differentiable", once_differentiable, dz, logits, grads[0]);
     auto edges = torch::autograd::collect_next_edges(grads[0]);
     edges.insert(edges.end(), next_edges().begin(), next_edges().end());
     using torch::autograd::Error;
@@ -790,60 +831,68 @@ void need_constant(const Tensor& t, const char* what) {
 }
 
 // ---- log_softmax(logits / temperature) at the tokens, float32; stats [.., 4]: what its gradient is made from
-std::tuple<Tensor, Tensor> token_logprobs_run(const Tensor& logits, const Tensor& tokens, const Tensor& mask,
-                                              double temperature, bool want_stats) {
+std::tuple<Tensor, Tensor> logprobs_run(const Tensor& logits, const Tensor& tokens_, const Tensor& mask,
+                                        double temperature, bool want_stats) {
   D3PM_GUARD(logits);
+  const Tensor tokens = dense(tokens_), m = dense(mask);
   auto v = logits_view(logits, tokens.sizes(), "tokens");
   auto fo = logits.options().dtype(at::kFloat);
   Tensor lp = at::empty(tokens.sizes(), fo), stats;
   if (want_stats) stats = at::empty({tokens.numel(), 4}, fo);
   check_rc(d3pm_token_logprobs(&v.desc, tokens.data_ptr(), token_bytes(tokens, logits, "tokens"),
-                               mask_ptr(mask, tokens.sizes(), logits), (float)temperature, lp.data_ptr<float>(),
+                               mask_ptr(m, tokens.sizes(), logits), (float)temperature, lp.data_ptr<float>(),
                                want_stats ? stats.data_ptr<float>() : nullptr, stream()));
   return {lp, stats};
 }
+Tensor token_logprobs(const Tensor& logits, const Tensor& tokens, const OptTensor& mask, double temperature) {
+  return std::get<0>(logprobs_run(logits, tokens, opt(mask), temperature, false));
+}
+std::tuple<Tensor, Tensor> token_logprobs_stats(const Tensor& logits, const Tensor& tokens, const OptTensor& mask,
+                                                double temperature) {
+  return logprobs_run(logits, tokens, opt(mask), temperature, true);
+}
 // the gradient at the logits from the rows' statistics
-void token_grad_run(const Tensor& logits, const Tensor& tokens, double temperature, const Tensor& stats,
-                    const Tensor& upstream, bool per_row, bool only_if_rescaled, Tensor& dz) {
+Tensor& token_grad_(Tensor& dz, const Tensor& logits, const Tensor& tokens, double temperature, const Tensor& stats,
+                    const Tensor& upstream, bool per_row, bool only_if_rescaled) {
   D3PM_GUARD(logits);
   auto v = logits_view(logits, tokens.sizes(), "tokens");
+  need_numel(stats, tokens.numel() * 4, "stats");
   const float* u = per_row ? row_f32(upstream, tokens, logits, "upstream and tokens") : upstream_ptr(upstream, logits);
   check_rc(d3pm_token_grad(&v.desc, tokens.data_ptr(), token_bytes(tokens, logits, "tokens"), (float)temperature,
-                           f32(stats, "stats"), u, per_row, only_if_rescaled, dz.data_ptr(), stream()));
+                           f32(stats, "stats"), u, per_row, only_if_rescaled, grad_ptr(dz, logits), stream()));
+  return dz;
 }
 struct TokenLogprobsBackward : public ObjectiveNode {
   double temperature;
   std::string name() const override { return "TokenLogprobs"; }
   void fill(const Tensor& logits, const std::vector<Tensor>& s, const Tensor& upstream, bool, Tensor& dz) override {
-    token_grad_run(logits, s[0], temperature, s[1], upstream, true, false, dz);
+    D3PM_CALL("_token_grad_", token_grad_, dz, logits, s[0], temperature, s[1], upstream, true, false);
   }
 };
-Tensor token_logprobs(const Tensor& logits, const Tensor& tokens_, const OptTensor& mask_, double temperature) {
+Tensor token_logprobs_autograd(const Tensor& logits, const Tensor& tokens_, const OptTensor& mask, double temperature) {
   need_no_tangent(logits, "logits");
   const bool want = differentiated(logits);
   Tensor rows, tokens, lp, stats;
   {
     at::AutoDispatchBelowADInplaceOrView below;
+    if (!want) return D3PM_CALL("token_logprobs", token_logprobs, logits, tokens_, mask, temperature);
     rows = as_rows(logits);
     tokens = dense(tokens_);
-    std::tie(lp, stats) = token_logprobs_run(rows, tokens, dense(opt(mask_)), temperature, want);
+    std::tie(lp, stats) = D3PM_CALL("_token_logprobs", token_logprobs_stats, rows, tokens, mask, temperature);
   }
-  if (want) {
-    auto node = new_node<TokenLogprobsBackward>();
-    node->save(logits, rows, {tokens, stats});
-    node->temperature = temperature;
-    torch::autograd::set_history(lp, node);
-  }
+  auto node = new_node<TokenLogprobsBackward>();
+  node->save(logits, rows, {tokens, stats});
+  node->temperature = temperature;
+  torch::autograd::set_history(lp, node);
   return lp;
 }
 
 // ---- distillation from a teacher's top logits
-struct DistillArgs { double temperature, out_scale; };
-// loss and per may be null (the gradient alone, times upstream), dz too (no gradient); ws: the loss call's workspace
-void distill_run(const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_index, const Tensor& mask,
-                 const DistillArgs& args, const float* upstream, bool only_if_rescaled, Tensor* loss, Tensor* per,
-                 const Tensor& dz, Tensor& ws) {
-  D3PM_GUARD(logits);
+// loss and per may be null (the gradient alone, times upstream), dz undefined (no gradient); ws: the loss call's workspace
+void distill_run(const Tensor& logits, const Tensor& teacher_logits_, const Tensor& teacher_index_, const Tensor& mask_,
+                 double temperature, double out_scale, const float* upstream, bool only_if_rescaled, Tensor* loss,
+                 Tensor* per, const Tensor& dz, Tensor ws) {
+  const Tensor teacher_logits = dense(teacher_logits_), teacher_index = dense(teacher_index_), mask = dense(mask_);
   const auto rows = logits.sizes().slice(0, std::max<int64_t>(logits.dim(), 1) - 1);
   auto v = logits_view(logits, rows, "the teacher's positions");
   need_device(teacher_logits, "teacher_logits");
@@ -861,53 +910,80 @@ void distill_run(const Tensor& logits, const Tensor& teacher_logits, const Tenso
     auto fo = logits.options().dtype(at::kFloat);
     *loss = at::empty({}, fo);
     *per = at::empty(rows, fo);
-    ws = objective_workspace(v.desc, logits);
   }
   check_rc(d3pm_topk_distill_loss(&v.desc, teacher_logits.data_ptr(), t_dtype, teacher_index.data_ptr(), i_bytes, (int)k,
-                                  m, (float)args.temperature, (float)args.out_scale, upstream, only_if_rescaled,
+                                  m, (float)temperature, (float)out_scale, upstream, only_if_rescaled,
                                   loss ? loss->data_ptr<float>() : nullptr, per ? per->data_ptr<float>() : nullptr,
-                                  dz.defined() ? dz.data_ptr() : nullptr, ws.data_ptr(), ws.nbytes(), stream()));
+                                  dz.defined() ? grad_ptr(dz, logits) : nullptr, ws.data_ptr(), ws.nbytes(), stream()));
+}
+// (loss [], per_token)
+std::tuple<Tensor, Tensor> topk_distill_loss(const Tensor& logits, const Tensor& teacher_logits,
+                                             const Tensor& teacher_index, const OptTensor& mask, double temperature,
+                                             double out_scale) {
+  D3PM_GUARD(logits);
+  Tensor loss, per;
+  distill_run(logits, teacher_logits, teacher_index, opt(mask), temperature, out_scale, nullptr, false, &loss, &per,
+              Tensor(), objective_workspace(logits));
+  return {loss, per};
+}
+// (loss, per_token, gradient, workspace)
+std::tuple<Tensor, Tensor, Tensor, Tensor> topk_distill_loss_grad(const Tensor& logits, const Tensor& teacher_logits,
+                                                                  const Tensor& teacher_index, const OptTensor& mask,
+                                                                  double temperature, double out_scale) {
+  D3PM_GUARD(logits);
+  Tensor loss, per, dz = grad_buffer(logits), ws = objective_workspace(logits);
+  distill_run(logits, teacher_logits, teacher_index, opt(mask), temperature, out_scale, nullptr, false, &loss, &per, dz, ws);
+  return {loss, per, dz, ws};
+}
+Tensor& topk_distill_grad_(Tensor& dz, const Tensor& logits, const Tensor& teacher_logits, const Tensor& teacher_index,
+                           const OptTensor& mask, double temperature, double out_scale, const Tensor& ws,
+                           const Tensor& upstream, bool only_if_rescaled) {
+  D3PM_GUARD(logits);
+  distill_run(logits, teacher_logits, teacher_index, opt(mask), temperature, out_scale, upstream_ptr(upstream, logits),
+              only_if_rescaled, nullptr, nullptr, dz, need_workspace(ws, logits));
+  return dz;
 }
 struct DistillBackward : public ObjectiveNode {
-  DistillArgs args;
+  double temperature, out_scale;
   std::string name() const override { return "TopKDistillLoss"; }
   void fill(const Tensor& logits, const std::vector<Tensor>& s, const Tensor& upstream, bool only, Tensor& dz) override {
-    Tensor ws = s[3];
-    distill_run(logits, s[0], s[1], s[2], args, upstream_ptr(upstream, logits), only, nullptr, nullptr, dz, ws);
+    D3PM_CALL("_topk_distill_grad_", topk_distill_grad_, dz, logits, s[0], s[1], as_opt(s[2]), temperature, out_scale, s[3],
+              upstream, only);
   }
 };
-// (loss [], per_token)
-std::tuple<Tensor, Tensor> topk_distill_loss(const Tensor& logits, const Tensor& teacher_logits_,
-                                             const Tensor& teacher_index_, const OptTensor& mask_, double temperature,
-                                             double out_scale) {
+std::tuple<Tensor, Tensor> topk_distill_loss_autograd(const Tensor& logits, const Tensor& teacher_logits_,
+                                                      const Tensor& teacher_index_, const OptTensor& mask_,
+                                                      double temperature, double out_scale) {
   need_no_tangent(logits, "logits");
   need_constant(teacher_logits_, "teacher_logits");
   const bool want = differentiated(logits);
-  const DistillArgs args{temperature, out_scale};
   Tensor rows, teacher_logits, teacher_index, mask, loss, per, dz, ws;
   {
     at::AutoDispatchBelowADInplaceOrView below;
+    if (!want)
+      return D3PM_CALL("topk_distill_loss", topk_distill_loss, logits, teacher_logits_, teacher_index_, mask_, temperature,
+                       out_scale);
     rows = as_rows(logits);
     teacher_logits = dense(teacher_logits_); teacher_index = dense(teacher_index_); mask = dense(opt(mask_));
-    if (want) dz = grad_buffer(logits);
-    distill_run(rows, teacher_logits, teacher_index, mask, args, nullptr, false, &loss, &per, dz, ws);
+    std::tie(loss, per, dz, ws) = D3PM_CALL("_topk_distill_loss", topk_distill_loss_grad, rows, teacher_logits,
+                                            teacher_index, as_opt(mask), temperature, out_scale);
   }
-  if (want) {
-    auto node = new_node<DistillBackward>();
-    node->save(logits, rows, {teacher_logits, teacher_index, mask, ws});
-    node->keep_gradient(std::move(dz));
-    node->args = args;
-    torch::autograd::set_history(loss, node);
-  }
+  auto node = new_node<DistillBackward>();
+  node->save(logits, rows, {teacher_logits, teacher_index, mask, ws});
+  node->keep_gradient(std::move(dz));
+  node->temperature = temperature;
+  node->out_scale = out_scale;
+  torch::autograd::set_history(loss, node);
   return {loss, per};
 }
 
 // ---- clipped policy loss with a KL term
 struct PolicyArgs { double temperature, clip_low, clip_high, kl_coeff, out_scale; };
-void policy_run(const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs, const Tensor& advantages,
-                const Tensor& ref_logprobs, const Tensor& mask, const PolicyArgs& args, const float* upstream,
-                bool only_if_rescaled, Tensor* loss, Tensor* lp, const Tensor& dz, Tensor& ws) {
-  D3PM_GUARD(logits);
+void policy_run(const Tensor& logits, const Tensor& tokens_, const Tensor& old_logprobs_, const Tensor& advantages_,
+                const Tensor& ref_logprobs_, const Tensor& mask_, const PolicyArgs& args, const float* upstream,
+                bool only_if_rescaled, Tensor* loss, Tensor* lp, const Tensor& dz, Tensor ws) {
+  const Tensor tokens = dense(tokens_), old_logprobs = dense_f32(old_logprobs_), advantages = dense_f32(advantages_),
+               ref_logprobs = dense_f32(ref_logprobs_), mask = dense(mask_);
   auto v = logits_view(logits, tokens.sizes(), "tokens");
   const int t_bytes = token_bytes(tokens, logits, "tokens");
   const float* old_lp = row_f32(old_logprobs, tokens, logits, "old_logprobs and tokens");
@@ -922,94 +998,149 @@ void policy_run(const Tensor& logits, const Tensor& tokens, const Tensor& old_lo
     auto fo = logits.options().dtype(at::kFloat);
     *loss = at::empty({}, fo);
     *lp = at::empty(tokens.sizes(), fo);
-    ws = objective_workspace(v.desc, logits);
   }
   check_rc(d3pm_policy_loss(&v.desc, tokens.data_ptr(), t_bytes, old_lp, adv, per_seq, ref, m, (float)args.temperature,
                             (float)args.clip_low, (float)args.clip_high, (float)args.kl_coeff, (float)args.out_scale,
                             upstream, only_if_rescaled, loss ? loss->data_ptr<float>() : nullptr,
-                            lp ? lp->data_ptr<float>() : nullptr, dz.defined() ? dz.data_ptr() : nullptr, ws.data_ptr(),
-                            ws.nbytes(), stream()));
+                            lp ? lp->data_ptr<float>() : nullptr, dz.defined() ? grad_ptr(dz, logits) : nullptr,
+                            ws.data_ptr(), ws.nbytes(), stream()));
+}
+// (loss [], logprobs)
+std::tuple<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs,
+                                       const Tensor& advantages, const OptTensor& ref_logprobs, const OptTensor& mask,
+                                       double temperature, double clip_low, double clip_high, double kl_coeff,
+                                       double out_scale) {
+  D3PM_GUARD(logits);
+  Tensor loss, lp;
+  policy_run(logits, tokens, old_logprobs, advantages, opt(ref_logprobs), opt(mask),
+             {temperature, clip_low, clip_high, kl_coeff, out_scale}, nullptr, false, &loss, &lp, Tensor(),
+             objective_workspace(logits));
+  return {loss, lp};
+}
+// (loss, logprobs, gradient, workspace)
+std::tuple<Tensor, Tensor, Tensor, Tensor> policy_loss_grad(
+    const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs, const Tensor& advantages,
+    const OptTensor& ref_logprobs, const OptTensor& mask, double temperature, double clip_low, double clip_high,
+    double kl_coeff, double out_scale) {
+  D3PM_GUARD(logits);
+  Tensor loss, lp, dz = grad_buffer(logits), ws = objective_workspace(logits);
+  policy_run(logits, tokens, old_logprobs, advantages, opt(ref_logprobs), opt(mask),
+             {temperature, clip_low, clip_high, kl_coeff, out_scale}, nullptr, false, &loss, &lp, dz, ws);
+  return {loss, lp, dz, ws};
+}
+Tensor& policy_grad_(Tensor& dz, const Tensor& logits, const Tensor& tokens, const Tensor& old_logprobs,
+                     const Tensor& advantages, const OptTensor& ref_logprobs, const OptTensor& mask, double temperature,
+                     double clip_low, double clip_high, double kl_coeff, double out_scale, const Tensor& ws,
+                     const Tensor& upstream, bool only_if_rescaled) {
+  D3PM_GUARD(logits);
+  policy_run(logits, tokens, old_logprobs, advantages, opt(ref_logprobs), opt(mask),
+             {temperature, clip_low, clip_high, kl_coeff, out_scale}, upstream_ptr(upstream, logits), only_if_rescaled,
+             nullptr, nullptr, dz, need_workspace(ws, logits));
+  return dz;
 }
 struct PolicyBackward : public ObjectiveNode {
   PolicyArgs args;
   std::string name() const override { return "PolicyLoss"; }
   void fill(const Tensor& logits, const std::vector<Tensor>& s, const Tensor& upstream, bool only, Tensor& dz) override {
-    Tensor ws = s[5];
-    policy_run(logits, s[0], s[1], s[2], s[3], s[4], args, upstream_ptr(upstream, logits), only, nullptr, nullptr, dz, ws);
+    D3PM_CALL("_policy_grad_", policy_grad_, dz, logits, s[0], s[1], s[2], as_opt(s[3]), as_opt(s[4]), args.temperature,
+              args.clip_low, args.clip_high, args.kl_coeff, args.out_scale, s[5], upstream, only);
   }
 };
-// (loss [], logprobs)
-std::tuple<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& tokens_, const Tensor& old_logprobs_,
-                                       const Tensor& advantages_, const OptTensor& ref_logprobs_, const OptTensor& mask_,
-                                       double temperature, double clip_low, double clip_high, double kl_coeff,
-                                       double out_scale) {
+std::tuple<Tensor, Tensor> policy_loss_autograd(const Tensor& logits, const Tensor& tokens_, const Tensor& old_logprobs_,
+                                                const Tensor& advantages_, const OptTensor& ref_logprobs_,
+                                                const OptTensor& mask_, double temperature, double clip_low,
+                                                double clip_high, double kl_coeff, double out_scale) {
   need_no_tangent(logits, "logits");
   need_constant(old_logprobs_, "old_logprobs");
   need_constant(advantages_, "advantages");
   need_constant(opt(ref_logprobs_), "ref_logprobs");
   const bool want = differentiated(logits);
-  const PolicyArgs args{temperature, clip_low, clip_high, kl_coeff, out_scale};
   Tensor rows, tokens, old_logprobs, advantages, ref_logprobs, mask, loss, lp, dz, ws;
   {
     at::AutoDispatchBelowADInplaceOrView below;
+    if (!want)
+      return D3PM_CALL("policy_loss", policy_loss, logits, tokens_, old_logprobs_, advantages_, ref_logprobs_, mask_,
+                       temperature, clip_low, clip_high, kl_coeff, out_scale);
     rows = as_rows(logits);
     tokens = dense(tokens_); old_logprobs = dense_f32(old_logprobs_); advantages = dense_f32(advantages_);
     ref_logprobs = dense_f32(opt(ref_logprobs_)); mask = dense(opt(mask_));
-    if (want) dz = grad_buffer(logits);
-    policy_run(rows, tokens, old_logprobs, advantages, ref_logprobs, mask, args, nullptr, false, &loss, &lp, dz, ws);
+    std::tie(loss, lp, dz, ws) = D3PM_CALL("_policy_loss", policy_loss_grad, rows, tokens, old_logprobs, advantages,
+                                           as_opt(ref_logprobs), as_opt(mask), temperature, clip_low, clip_high, kl_coeff,
+                                           out_scale);
   }
-  if (want) {
-    auto node = new_node<PolicyBackward>();
-    node->save(logits, rows, {tokens, old_logprobs, advantages, ref_logprobs, mask, ws});
-    node->keep_gradient(std::move(dz));
-    node->args = args;
-    torch::autograd::set_history(loss, node);
-  }
+  auto node = new_node<PolicyBackward>();
+  node->save(logits, rows, {tokens, old_logprobs, advantages, ref_logprobs, mask, ws});
+  node->keep_gradient(std::move(dz));
+  node->args = {temperature, clip_low, clip_high, kl_coeff, out_scale};
+  torch::autograd::set_history(loss, node);
   return {loss, lp};
 }
 
 // ---- preference loss of the pairs (p, p + B / 2)
+std::tuple<Tensor, Tensor, Tensor> preference_run(const Tensor& logits, const Tensor& tokens_, const Tensor& ref_logprobs_,
+                                                  const Tensor& mask_, double beta, double label_smoothing, bool average,
+                                                  double out_scale, const Tensor& dz) {
+  const Tensor tokens = dense(tokens_), ref_logprobs = dense_f32(ref_logprobs_), mask = dense(mask_);
+  auto v = logits_view(logits, tokens.sizes(), "tokens");
+  const int t_bytes = token_bytes(tokens, logits, "tokens");
+  const float* ref = ref_logprobs.defined() ? row_f32(ref_logprobs, tokens, logits, "ref_logprobs and tokens") : nullptr;
+  const uint8_t* m = mask_ptr(mask, tokens.sizes(), logits);
+  auto fo = logits.options().dtype(at::kFloat);
+  const Tensor loss = at::empty({}, fo), rewards = at::empty({v.desc.B}, fo), stats = at::empty({tokens.numel(), 4}, fo);
+  const Tensor ws = objective_workspace(logits);
+  check_rc(d3pm_preference_loss(&v.desc, tokens.data_ptr(), t_bytes, ref, m, (float)beta, (float)label_smoothing,
+                                average, (float)out_scale, loss.data_ptr<float>(), rewards.data_ptr<float>(),
+                                stats.data_ptr<float>(), dz.defined() ? grad_ptr(dz, logits) : nullptr, ws.data_ptr(),
+                                ws.nbytes(), stream()));
+  return {loss, rewards, stats};
+}
+// (loss [], rewards [B])
+std::tuple<Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& tokens, const OptTensor& ref_logprobs,
+                                           const OptTensor& mask, double beta, double label_smoothing, bool average,
+                                           double out_scale) {
+  D3PM_GUARD(logits);
+  auto [loss, rewards, stats] = preference_run(logits, tokens, opt(ref_logprobs), opt(mask), beta, label_smoothing,
+                                               average, out_scale, Tensor());
+  return {loss, rewards};
+}
+// (loss, rewards, gradient, row statistics)
+std::tuple<Tensor, Tensor, Tensor, Tensor> preference_loss_grad(const Tensor& logits, const Tensor& tokens,
+                                                                const OptTensor& ref_logprobs, const OptTensor& mask,
+                                                                double beta, double label_smoothing, bool average,
+                                                                double out_scale) {
+  D3PM_GUARD(logits);
+  const Tensor dz = grad_buffer(logits);
+  auto [loss, rewards, stats] = preference_run(logits, tokens, opt(ref_logprobs), opt(mask), beta, label_smoothing,
+                                               average, out_scale, dz);
+  return {loss, rewards, dz, stats};
+}
 struct PreferenceBackward : public ObjectiveNode {
   std::string name() const override { return "PreferenceLoss"; }
   void fill(const Tensor& logits, const std::vector<Tensor>& s, const Tensor& upstream, bool only, Tensor& dz) override {
-    token_grad_run(logits, s[0], 1.0, s[1], upstream, false, only, dz);
+    D3PM_CALL("_token_grad_", token_grad_, dz, logits, s[0], 1.0, s[1], upstream, false, only);
   }
 };
-// (loss [], rewards [B])
-std::tuple<Tensor, Tensor> preference_loss(const Tensor& logits, const Tensor& tokens_, const OptTensor& ref_logprobs_,
-                                           const OptTensor& mask_, double beta, double label_smoothing, bool average,
-                                           double out_scale) {
+std::tuple<Tensor, Tensor> preference_loss_autograd(const Tensor& logits, const Tensor& tokens_,
+                                                    const OptTensor& ref_logprobs, const OptTensor& mask, double beta,
+                                                    double label_smoothing, bool average, double out_scale) {
   need_no_tangent(logits, "logits");
-  need_constant(opt(ref_logprobs_), "ref_logprobs");
+  need_constant(opt(ref_logprobs), "ref_logprobs");
   const bool want = differentiated(logits);
   Tensor rows, tokens, loss, rewards, stats, dz;
   {
     at::AutoDispatchBelowADInplaceOrView below;
-    D3PM_GUARD(logits);
-    tokens = dense(tokens_);
-    const Tensor ref_logprobs = dense_f32(opt(ref_logprobs_)), mask = dense(opt(mask_));
+    if (!want)
+      return D3PM_CALL("preference_loss", preference_loss, logits, tokens_, ref_logprobs, mask, beta, label_smoothing,
+                       average, out_scale);
     rows = as_rows(logits);
-    auto v = logits_view(rows, tokens.sizes(), "tokens");
-    const int t_bytes = token_bytes(tokens, logits, "tokens");
-    const float* ref = ref_logprobs.defined() ? row_f32(ref_logprobs, tokens, logits, "ref_logprobs and tokens") : nullptr;
-    const uint8_t* m = mask_ptr(mask, tokens.sizes(), logits);
-    auto fo = logits.options().dtype(at::kFloat);
-    loss = at::empty({}, fo);
-    rewards = at::empty({v.desc.B}, fo);
-    stats = at::empty({tokens.numel(), 4}, fo);
-    if (want) dz = grad_buffer(logits);
-    const Tensor ws = objective_workspace(v.desc, logits);
-    check_rc(d3pm_preference_loss(&v.desc, tokens.data_ptr(), t_bytes, ref, m, (float)beta, (float)label_smoothing,
-                                  average, (float)out_scale, loss.data_ptr<float>(), rewards.data_ptr<float>(),
-                                  stats.data_ptr<float>(), want ? dz.data_ptr() : nullptr, ws.data_ptr(), ws.nbytes(),
-                                  stream()));
+    tokens = dense(tokens_);
+    std::tie(loss, rewards, dz, stats) = D3PM_CALL("_preference_loss", preference_loss_grad, rows, tokens, ref_logprobs,
+                                                   mask, beta, label_smoothing, average, out_scale);
   }
-  if (want) {
-    auto node = new_node<PreferenceBackward>();
-    node->save(logits, rows, {tokens, stats});
-    node->keep_gradient(std::move(dz));
-    torch::autograd::set_history(loss, node);
-  }
+  auto node = new_node<PreferenceBackward>();
+  node->save(logits, rows, {tokens, stats});
+  node->keep_gradient(std::move(dz));
+  torch::autograd::set_history(loss, node);
   return {loss, rewards};
 }
 
@@ -1054,13 +1185,27 @@ TORCH_LIBRARY(d3pm_mi355x, m) {
   m.def("lvb_reverse_step(" D3PM_PT "Tensor pred, Tensor x_t, Tensor t, Tensor? expo, int seed, int offset, "
         "Tensor? offset_dev, float last_class_div, int exclude_last_prefix) -> Tensor");
   m.def("corrupt(" D3PM_PT "Tensor x0, Tensor t, Tensor? expo, int seed, int offset, bool want_probs) -> (Tensor, Tensor)");
-  m.def("token_logprobs(Tensor logits, Tensor tokens, Tensor? mask, float temperature) -> Tensor");
-  m.def("topk_distill_loss(Tensor logits, Tensor teacher_logits, Tensor teacher_index, Tensor? mask, float temperature, "
-        "float out_scale) -> (Tensor, Tensor)");
-  m.def("policy_loss(Tensor logits, Tensor tokens, Tensor old_logprobs, Tensor advantages, Tensor? ref_logprobs, "
-        "Tensor? mask, float temperature, float clip_low, float clip_high, float kl_coeff, float out_scale) -> (Tensor, Tensor)");
-  m.def("preference_loss(Tensor logits, Tensor tokens, Tensor? ref_logprobs, Tensor? mask, float beta, "
-        "float label_smoothing, bool average, float out_scale) -> (Tensor, Tensor)");
+#define D3PM_TEMPERATURE "Tensor? mask, float temperature"
+#define D3PM_DISTILL "Tensor logits, Tensor teacher_logits, Tensor teacher_index, " D3PM_TEMPERATURE ", float out_scale"
+#define D3PM_POLICY "Tensor logits, Tensor tokens, Tensor old_logprobs, Tensor advantages, Tensor? ref_logprobs, " \
+                    D3PM_TEMPERATURE ", float clip_low, float clip_high, float kl_coeff, float out_scale"
+#define D3PM_PREFERENCE "Tensor logits, Tensor tokens, Tensor? ref_logprobs, Tensor? mask, float beta, " \
+                        "float label_smoothing, bool average, float out_scale"
+  m.def("token_logprobs(Tensor logits, Tensor tokens, " D3PM_TEMPERATURE ") -> Tensor");
+  m.def("topk_distill_loss(" D3PM_DISTILL ") -> (Tensor, Tensor)");
+  m.def("policy_loss(" D3PM_POLICY ") -> (Tensor, Tensor)");
+  m.def("preference_loss(" D3PM_PREFERENCE ") -> (Tensor, Tensor)");
+  // what their autograd kernels call
+  m.def("_token_logprobs(Tensor logits, Tensor tokens, " D3PM_TEMPERATURE ") -> (Tensor, Tensor)");
+  m.def("_topk_distill_loss(" D3PM_DISTILL ") -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("_policy_loss(" D3PM_POLICY ") -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("_preference_loss(" D3PM_PREFERENCE ") -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("_once_differentiable(Tensor grad, Tensor logits, Tensor upstream) -> Tensor");
+  m.def("_token_grad_(Tensor(a!) dlogits, Tensor logits, Tensor tokens, float temperature, Tensor stats, Tensor upstream, "
+        "bool per_row, bool only_if_rescaled) -> Tensor(a!)");
+  m.def("_topk_distill_grad_(Tensor(a!) dlogits, " D3PM_DISTILL ", Tensor workspace, Tensor upstream, "
+        "bool only_if_rescaled) -> Tensor(a!)");
+  m.def("_policy_grad_(Tensor(a!) dlogits, " D3PM_POLICY ", Tensor workspace, Tensor upstream, bool only_if_rescaled) -> Tensor(a!)");
 }
 
 TORCH_LIBRARY_IMPL(d3pm_mi355x, CUDA, m) {
@@ -1095,12 +1240,23 @@ TORCH_LIBRARY_IMPL(d3pm_mi355x, CUDA, m) {
   m.impl("topk_distill_loss", topk_distill_loss);
   m.impl("policy_loss", policy_loss);
   m.impl("preference_loss", preference_loss);
+  m.impl("_token_logprobs", token_logprobs_stats);
+  m.impl("_topk_distill_loss", topk_distill_loss_grad);
+  m.impl("_policy_loss", policy_loss_grad);
+  m.impl("_preference_loss", preference_loss_grad);
+  m.impl("_once_differentiable", once_differentiable);
+  m.impl("_token_grad_", token_grad_);
+  m.impl("_topk_distill_grad_", topk_distill_grad_);
+  m.impl("_policy_grad_", policy_grad_);
 }
 
 // the fine-tuning objectives bring their own autograd nodes
 TORCH_LIBRARY_IMPL(d3pm_mi355x, AutogradCUDA, m) {
-  m.impl("token_logprobs", token_logprobs);
-  m.impl("topk_distill_loss", topk_distill_loss);
-  m.impl("policy_loss", policy_loss);
-  m.impl("preference_loss", preference_loss);
+  m.impl("token_logprobs", token_logprobs_autograd);
+  m.impl("topk_distill_loss", topk_distill_loss_autograd);
+  m.impl("policy_loss", policy_loss_autograd);
+  m.impl("preference_loss", preference_loss_autograd);
+  for (const char* name : {"_token_logprobs", "_topk_distill_loss", "_policy_loss", "_preference_loss", "_token_grad_",
+                           "_topk_distill_grad_", "_policy_grad_", "_once_differentiable"})
+    m.impl(name, torch::autograd::autogradNotImplementedFallback());
 }

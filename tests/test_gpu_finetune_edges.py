@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_finetune import DTYPES, EPS, OBJECTIVES, call, check_grad, make, reference, to_dev
+from test_gpu_finetune import DTYPES, EPS, OBJECTIVES, TAU, build, call, check_grad, make, reference, to_dev
 
 pytestmark = pytest.mark.gpu
 
@@ -202,3 +202,70 @@ def test_backward_makes_no_second_copy(pkg, name, kind):
     grown = torch.cuda.max_memory_allocated() - before
     assert torch.equal(got, want)
     assert grown < (1.5 if name == "logprobs" else 0.5) * size      # (a log-probability's gradient is made in backward)
+
+
+@pytest.mark.parametrize("name", OBJECTIVES)
+def test_seen_by_dispatch_modes(pkg, name):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.ops = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.ops.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    c = to_dev(make(117, 4, 3, 20, "f32"))
+    z = c["logits"].requires_grad_(True)
+    up = c["up"] * c["mask"] if name == "logprobs" else None
+    want, = torch.autograd.grad(call(pkg, name, c, z)[0], z, up)
+    with Seen() as seen:
+        root, _ = call(pkg, name, c, z)
+    assert any(op.startswith("d3pm_mi355x.") for op in seen.ops), seen.ops
+    with Seen() as seen:
+        got, = torch.autograd.grad(root, z, up)
+    assert any(op.startswith("d3pm_mi355x.") for op in seen.ops), seen.ops
+    with Seen() as seen, torch.no_grad():
+        call(pkg, name, c, z)
+    assert any(op.startswith("d3pm_mi355x.") for op in seen.ops), seen.ops
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("name", OBJECTIVES)
+def test_selective_checkpoint(pkg, name):
+    """A checkpoint that keeps what these operators returned: they do not run again."""
+    from functools import partial
+    from torch.utils.checkpoint import CheckpointPolicy, checkpoint, create_selective_checkpoint_contexts
+    d = to_dev(make(107, 4, 5, 40, "f32"))
+    h = torch.randn(20, 16, generator=torch.Generator().manual_seed(1)).cuda().requires_grad_(True)
+    w = torch.randn(16, 40, generator=torch.Generator().manual_seed(2)).cuda().requires_grad_(True)
+    ran = []
+
+    def keep(ctx, op, *args, **kwargs):
+        mine = str(op).startswith("d3pm_mi355x.")
+        if mine:
+            ran.append(ctx.is_recompute)
+        return CheckpointPolicy.MUST_SAVE if mine else CheckpointPolicy.PREFER_RECOMPUTE
+
+    def part(h, w):
+        return call(pkg, name, d, (h @ w).view(4, 5, 40))[0]
+
+    root = part(h, w)
+    up = 1.5 * torch.ones_like(root)
+    want = torch.autograd.grad(root, (h, w), up)
+    root = checkpoint(part, h, w, use_reentrant=False, context_fn=partial(create_selective_checkpoint_contexts, keep))
+    got = torch.autograd.grad(root, (h, w), up)
+    assert ran and all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("name", OBJECTIVES)
+def test_under_func_grad(pkg, name):
+    c = to_dev(make(119, 4, 3, 20, "f32"))
+    z = c["logits"].clone().requires_grad_(True)
+    total = lambda z: (call(pkg, name, c, z)[0] * (c["up"] * c["mask"] if name == "logprobs" else 1.0)).sum()
+    want, = torch.autograd.grad(total(z), z)
+    assert torch.equal(torch.func.grad(total)(c["logits"]), want)
+    with pytest.raises(RuntimeError):                            # a gradient of the gradient
+        torch.func.grad(lambda z: torch.func.grad(total)(z).square().sum())(c["logits"])
