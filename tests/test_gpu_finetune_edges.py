@@ -1,12 +1,12 @@
 """The fine-tuning objectives where a call is allowed but unusual: upstream gradients that are no numbers at places that
-are not counted, derivatives that these losses do not have, far log-probabilities, long sums, rows that start anywhere,
-dispatch modes and transforms.  Inputs, definitions and tolerances as in test_gpu_finetune.py unless stated."""
+are not counted, derivatives that these losses do not have, far log-probabilities, long sums and means, rows that start
+anywhere, dispatch modes and transforms.  Inputs, definitions and tolerances as in test_gpu_finetune.py unless stated."""
 import math
 
 import pytest
 import torch
 
-from test_gpu_finetune import DTYPES, EPS, OBJECTIVES, TAU, build, call, check_grad, make, reference, to_dev
+from test_gpu_finetune import DTYPES, EPS, OBJECTIVES, call, check, check_grad, make, reference, to_dev
 
 pytestmark = pytest.mark.gpu
 
@@ -175,6 +175,21 @@ def test_ratios_of_improbable_tokens(pkg, V, tau):
     loss = fn(z.cuda(), y.cuda(), old.cuda(), torch.ones(4, 8, device="cuda"))
     want = -torch.exp(lp - old.double()).mean()
     assert abs(float(loss) - float(want)) <= (9 + (35 if V > 256 else 0)) * EPS * float(want.abs())
+
+
+@pytest.mark.parametrize("N", [16384, 16385, 50001])
+@pytest.mark.parametrize("name", ["distill", "policy"])
+def test_mean_over_many_counted_positions(pkg, name, N):
+    """Masks that the row launch counts itself, and longer ones that a launch ahead of it counts; the backward with another
+    upstream gradient finds that count again."""
+    d = make(N, 1, N, 20, "f32")
+    d["mask"] = torch.rand(1, N, generator=torch.Generator().manual_seed(N)) < 0.4
+    check(pkg, name, d)
+    out, grad, bound = reference(name, d)
+    c = to_dev(d)
+    z = c["logits"].requires_grad_(True)
+    g, = torch.autograd.grad(call(pkg, name, c, z)[0], z, torch.full((), 0.37, device="cuda"))
+    check_grad(g, float(torch.tensor(0.37)) * grad, bound, z.dtype, 0.37)
 
 
 @pytest.mark.parametrize("name", OBJECTIVES)
