@@ -339,7 +339,8 @@ __device__ __forceinline__ void fresh(u32x4 (&v)[NV]) {
 
 // Whether the j-th pieces of a row's lanes may hold any of its `full` pieces: those of rows of several waves, where the
 // answer is one branch, are passed over if not (a row fills at least half of its shape's pieces).  12288 rows of 70001
-// bf16 classes: 900 -> 751 us.  (Rows of one wave have no registers left for it: 99 -> 106 us at 2000 classes.)
+// bf16 classes: distillation 866 -> 709 us, policy loss 820 -> 655; 8192 of 100003: 671 -> 647 and 640 -> 641.  (Rows of
+// one wave have no registers left for it: 99 -> 106 us at 2000 classes.)
 template <int G, int NV>
 __device__ __forceinline__ bool holds(int j, int full) { return G <= 64 || j < NV / 2 || j * G < full; }
 
@@ -358,7 +359,8 @@ __device__ __forceinline__ void mask_pieces(u32x4 (&v)[NV], int full, int g) {
 // m and S of the group's row from its lanes' values, in two steps: of the wave (a wave takes its exponentials against its
 // own maximum, so a row of several waves needs one exchange, not two; the reference is kept off -inf, for a wave that
 // has only padding), and of the row.  KEEP: the pieces are needed again, for the gradient.
-// EXACT: S in 64 bits, as hi + lo.  A preference loss sums a sequence's log-ratios, which may nearly cancel, and a policy
+// EXACT: S in 64 bits, as hi + lo, from the elements on in a row of up to one wave, else from the lanes' float32 sums of two
+// chains each on.  A preference loss sums a sequence's log-ratios, which may nearly cancel, and a policy
 // loss means over advantages of both signs.  With EXACT in a row of up to one wave the rounding of each exponent x is kept
 // as x_lo, and exp2(x + x_lo) = exp2(x) (1 + ln 2 x_lo); over the many terms of longer rows it averages out.
 struct RowSum { float m, hi, lo; };
@@ -1072,9 +1074,11 @@ __global__ __launch_bounds__(PAIR_WG) void k_pair(PairArgs a) {
 
 // Pairs of few rows in one launch: a workgroup reads its pair's rows, sums, and makes the gradient from a second look at
 // them, which the caches still hold.  Rows' statistics wait in LDS (2 L float4) and go to memory for the backward.
-// 128 pairs of 263 x 24 float32 (four and a bit sweeps of the workgroup over its rows): 13.1 us against 17.4 in three
-// launches, and 4 us less of the host's time; at ten sweeps (600 x 24) 24.4 against 23.3, and 34 against 11 where a
-// single pair of 2 x 1024 rows has the chip to itself.  Hence up to five sweeps, and rows that a wave holds.
+// One launch against three, on the device: 128 pairs of 263 x 24 float32 (four and a bit sweeps of the workgroup over its
+// rows) 16.7 / 19.7 us, of 320 (five) 18.4 / 20.9, of 400 21.3 / 22.8, of 600 27.8 / 28.8, 1024 pairs of 263 46 / 65; a pair
+// alone, with three launches that spread it over the chip, 6.5 / 9.8 at 30 rows a sequence, 9.5 / 10.7 at 160, 13.7 / 11.2
+// at 320, 21.1 / 12.1 at 600.  Up to five sweeps, and rows that a wave holds: beyond, many pairs gain 4 to 7 % and few lose
+// half.
 constexpr int PAIR_SWEEPS = 5;
 constexpr long PAIR_BYTES = 128 << 10;
 constexpr int pair_lanes(int full) { return full <= 32 ? 8 : full <= 64 ? 16 : full <= 128 ? 32 : 64; }
@@ -1206,7 +1210,9 @@ static int launch_rows(const RowArgs& a, int* grid, hipStream_t s) {
   const int want = (a.N - 1) / Sh::ROWS + 1;
   // Parts of a wave: as many workgroups as the 256 compute units hold, which walk over the rows.  A row to a workgroup:
   // one each, as they come (5 to 10 % less than with walking ones), up to 1024 lanes, where a compute unit holds one
-  // and the next would wait for its last store (581 us against 631 at 4 x 2048 ragged rows of 100003 bf16 classes).
+  // and the next would wait for its last store (walking against as they come, distillation and policy loss: 648 / 678 and
+  // 641 / 675 us at 8192 rows of 100003 bf16 classes, 709 / 731 and 655 / 704 at 12288 of 70001, 808 / 812 and 806 / 814 at
+  // 8192 of 131072; float32 alone prefers the other: 432 / 425 and 417 / 415 at 4096 of 65528).
   *grid = std::min(want, G <= 64 ? 2048 : G < 1024 ? MAX_PARTIALS : 256);
   const size_t lds = DISTILL ? list_bytes(Sh::ROWS, a.k, NV < 16) : 0;
   if (a.dz) hipLaunchKernelGGL((k_rows<T, G, NV, DISTILL, true>), dim3(*grid), dim3(Sh::WG), lds, s, a);

@@ -4,8 +4,8 @@
 // allocator, and calls the C ABI of libd3pm_hip.so (include/d3pm_hip.h) on torch's current HIP stream.  No
 // arithmetic happens here.  The operators carry the reference function they stand for in their schema comment;
 // autograd nodes live in the Python facade, which calls these operators; those of the fine-tuning objectives live
-// here.  Status codes of the library become the exceptions the reference raises: D3PM_EINVAL -> ValueError, D3PM_EUNSUPPORTED -> NotImplementedError,
-// D3PM_EHIP -> RuntimeError.  Every operator makes the device of its first tensor current for the call and checks
+// here.  Status codes of the library become the exceptions the reference raises: D3PM_EINVAL -> ValueError,
+// D3PM_EUNSUPPORTED -> NotImplementedError, D3PM_EHIP -> RuntimeError.  Every operator makes the device of its first tensor current for the call and checks
 // every tensor's element count against the batch it describes before a pointer reaches the library: a mis-shaped
 // call raises, it does not read or write out of bounds.
 #include <ATen/ATen.h>
@@ -720,7 +720,8 @@ void* grad_ptr(const Tensor& dz, const Tensor& z) {
 Tensor grad_buffer(const Tensor& z) { return at::empty(z.sizes(), z.options().memory_format(at::MemoryFormat::Contiguous)); }
 
 // The autograd nodes of these losses are C++: at the sizes where the host is the bound (a protein batch), a Python
-// node and its saved tensors took 45 us of a 92 us forward and backward.  A node keeps what its gradient needs, and
+// node and its saved tensors took 40 us of a 96 us forward and backward (57 now, 50 of them torch's engine; in one thread
+// 52 and 31, 28 of them the engine).  A node keeps what its gradient needs, and
 // the gradient buffer that the loss launch filled for an upstream gradient of 1; backward hands that buffer over
 // after a launch that does it again only if the upstream gradient is another number, and a second backward
 // (retain_graph) fills a buffer of its own.  So does a backward that is captured into another graph than its forward, or

@@ -8,10 +8,10 @@ package: the gradient at the logits comes out of the launch that computes the lo
 
 Logits are float32, float16 or bfloat16 ``[..., V]`` on the GPU with any strides (where the classes do not lie side by
 side, or the positions of a sequence do not follow each other with one stride, they are copied into rows once, and the
-copy is kept for the gradient in their place); everything is computed in float32
-(sums over rows and sequences in float64) and the gradient is rounded once, to the logits' type.  ``mask`` (bool, the
-tokens' shape) says which positions count: the others' logits and labels are not looked at (they may hold NaN, or
-tokens that are none), their outputs and gradients are 0.  Tokens and classes outside ``[0, V)`` are clamped into it
+copy is kept for the gradient in their place); everything is computed in float32 (the join of a row's lanes, sums over rows
+and over sequences in float64) and the gradient is rounded once, to the logits' type.  ``mask`` (bool, the tokens' shape)
+says which positions count: the others' logits and labels are not looked at (they may hold NaN, or tokens that are none),
+their outputs and gradients are 0, whatever their upstream gradient.  Tokens and classes outside ``[0, V)`` are clamped into it
 (a negative ``teacher_index`` marks an entry that is not there).  Only the logits are differentiated, in reverse mode and
 once: any other floating input that requires a gradient, a forward-mode tangent and the gradient of a gradient are
 refused.

@@ -390,8 +390,8 @@ int d3pm_lvb_reverse_step(const d3pm_tables_f64* tb, const float* pred, long ld,
  * Fine-tuning objectives (no counterpart in the reference): losses at the
  * logits of a denoiser or a language model and their gradient there, for a
  * model that is distilled or tuned to preferences or rewards after its
- * training.  All arithmetic in float32, sums over rows and sequences in
- * float64; results are repeatable bit for bit.
+ * training.  All arithmetic in float32, the join of a row's lanes and sums
+ * over rows and sequences in float64; results are repeatable bit for bit.
  *
  * mask uint8 [B,L], 0 where a position is not counted (NULL: every position
  * is): its logits row and its entries of the other inputs are not looked at,
@@ -424,7 +424,8 @@ int d3pm_token_logprobs(const d3pm_logits* z, const void* tokens, int tok_bytes,
 
 /* Gradient of d3pm_token_logprobs (upstream float32 [B,L], upstream_per_row
  * != 0) or of d3pm_preference_loss (one upstream float32, upstream_per_row ==
- * 0, temperature 1; NULL: 1) from the row_stats that they left.
+ * 0, temperature 1; NULL: 1) from the row_stats that they left.  Rows that
+ * are not counted, which row_stats marks, get 0 whatever their upstream.
  * only_if_rescaled: dlogits holds the gradient for an upstream of 1 already,
  * as the loss call wrote it, and is left alone if *upstream is 1. */
 int d3pm_token_grad(const d3pm_logits* z, const void* tokens, int tok_bytes, float temperature,

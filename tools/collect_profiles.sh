@@ -4,6 +4,8 @@
 #                                       (every hot kernel at the bench's shapes, eager launches)
 #   tools/collect_profiles.sh bench     kernel trace of bench.py --no-graph --no-secondary (the headline step)
 #   tools/collect_profiles.sh dense     kernel trace + matrix-core counters of the K=256 image configuration
+#   tools/collect_profiles.sh finetune  kernel trace of every case of perf/operators.py, one process each (graph replays:
+#                                       their launches are traced as single ones), counters of the large ones
 #   tools/collect_profiles.sh roofline  kernel trace of bench.py --roofline-only: the dominant kernel over ten rotating
 #                                       buffer sets and nothing else of it (the launch sequence roofline.frac is quoted on)
 # One counter group per run, each run a process of its own with its own time limit; the first failing step ends
@@ -56,6 +58,22 @@ dense)
   echo "== dense K=256: matrix-core counters"
   timeout -s KILL 120 rocprofv3 --pmc SQ_VALU_MFMA_BUSY_CYCLES SQ_BUSY_CU_CYCLES SQ_INSTS_VALU_MFMA_MOPS_F32 SQ_INSTS_VALU_MFMA_F32 SQ_ACTIVE_INST_VALU SQ_WAVE_CYCLES SQ_WAIT_INST_ANY SQ_VALU_MFMA_COEXEC_CYCLES --output-format csv -d $O -o mfma -- python3 -u $K --reps 3 > $O/mfma.log
   sum $O/pmc_mfma.json $O/mfma_counter_collection.csv > $O/pmc_mfma.txt
+  ;;
+finetune)
+  F="$R/tools/finetune_bench.py --replays 8"
+  for c in logprobs_one_token logprobs_designs logprobs_weighted distill_protein distill_odd distill_large preference_one_pair preference_protein preference_long policy_protein policy_image policy_large; do
+    echo "== $c: kernel trace"
+    timeout -k 10 100 rocprofv3 --kernel-trace --stats --output-format csv -d $O -o $c -- python3 -u $F --only $c > $O/$c.log
+    echo $c >> $O/kernels.txt
+    (cd $R && python3 tools/finetune_bench.py --trace $O/${c}_kernel_trace.csv) >> $O/kernels.txt
+  done
+  for c in logprobs_weighted distill_large preference_long policy_image policy_large; do
+    for set in "SQ_BUSY_CU_CYCLES SQ_ACTIVE_INST_VALU SQ_INSTS_VALU SQ_WAVE_CYCLES" FETCH_SIZE WRITE_SIZE; do
+      echo "== $c: $set"
+      timeout -s KILL 100 rocprofv3 --pmc $set --output-format csv -d $O -o ${c}_${set%% *} -- python3 -u $F --only $c > $O/$c.log
+    done
+    sum $O/${c}_pmc.json $O/${c}_SQ_BUSY_CU_CYCLES_counter_collection.csv $O/${c}_FETCH_SIZE_counter_collection.csv $O/${c}_WRITE_SIZE_counter_collection.csv > $O/${c}_pmc.txt
+  done
   ;;
 *) echo "unknown: $WHAT"; exit 2;;
 esac
