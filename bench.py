@@ -46,7 +46,7 @@ SUB_BATCH = 1250               # reverse sampling: sequences per graph replay (1
 TRAFFIC_FILES = [os.path.join(ROOT, "profiles", f) for f in ("r03_kernels_pmc_hbm.json", "r02_kernels_pmc_hbm.json",
                                                              "r01_bench_pmc_hbm.json")]
 # `rocprofv3 --kernel-trace --stats` of `bench.py --roofline-only` (the rotating-buffer launch sequence alone)
-TRACE_FILES = [os.path.join(ROOT, "profiles", f) for f in ("r03_roofline_kernel_stats.csv",)]
+TRACE_FILES = [os.path.join(ROOT, "profiles", f) for f in ("roofline_kernel_stats.csv",)]
 
 
 # the headline kernel: gradient, no next-batch corruption, one pass (the workgroup covers its batch element)

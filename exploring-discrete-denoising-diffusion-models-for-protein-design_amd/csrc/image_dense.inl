@@ -590,121 +590,130 @@ __global__ __launch_bounds__(BLOCK, MFMA ? 2 : 1) void k_dense_tile(ImgArgs a, D
     __syncthreads();
     D3PM_PHASE(2);
     // ---- phase 3: per-token epilogue
-    if (MFMA && need_post) gather(0);
+    // The two ways of need_post are apart with the backward's registers: joined in every pass, the table rows and the
+    // contracted values are carried as merges through the second contraction (337 spilled registers, 535 us a launch
+    // instead of 303).
+    auto epilogue = [&](const bool post) {
+      if (MFMA && post) gather(0);
 #pragma unroll
-    for (int ps = 0; ps < NP; ++ps) {
-      const int tok = ps * C::TPP + slot;
-      const long pos = tile0 + tok;
-      const bool live = pos < p1;
-      const long n = (long)b * a.npos + (live ? pos : tile0);
-      float f2e[L::V];
-      if constexpr (MFMA && MODE != DENSE_LOSS) {
-        if (t == 0) load_slots<L>(e.logits + n * e.ld, g, K, -INFINITY, zkeep[0]);    // rare: 1 / T of the workgroups
-      }
-      if (need_post) {
-        if (ps + 1 < NP) gather(ps + 1);
-        load_slots<L>(s_f2 + (size_t)tok * LDK, g, K, 1.0f, f2e);
+      for (int ps = 0; ps < NP; ++ps) {
+        const int tok = ps * C::TPP + slot;
+        const long pos = tile0 + tok;
+        const bool live = pos < p1;
+        const long n = (long)b * a.npos + (live ? pos : tile0);
+        float f2e[L::V];
+        if constexpr (MFMA && MODE != DENSE_LOSS) {
+          if (t == 0) load_slots<L>(e.logits + n * e.ld, g, K, -INFINITY, zkeep[0]);    // rare: 1 / T of the workgroups
+        }
+        if (post) {
+          if (ps + 1 < NP) gather(ps + 1);
+          load_slots<L>(s_f2 + (size_t)tok * LDK, g, K, 1.0f, f2e);
 #pragma unroll
-        for (int v = 0; v < L::V; ++v) f2e[v] = fmaf(f2e[v], 1.0f / (PSC * PSC), eps);
-      }
-      if constexpr (MFMA && !GRAD) {
-        if (ps == NP - 1 && more) fetch_tile(tile0 + C::TM);
-      }
-      if constexpr (MODE == DENSE_LOSS) {
-        // kl = sum_j q_j log(q_j / p_j) with q ~ a.*b, p ~ a.*f2 (a = column x_t of Q_t + eps, b = row x0 of
-        // Qbar_{t-1} + eps, f2 = pi Qbar_{t-1} + eps): the reference's softmax(log a + log .) pairs folded, one
-        // log per class (of a ratio close to one where q is large).
-        const float ce = MFMA ? s_tokf[3 * tok] : cekeep[ps];
-        float vb = ce;
-        if (need_post) {
-          float av[L::V], bv[L::V], zm = 0, zt = 0;
+          for (int v = 0; v < L::V; ++v) f2e[v] = fmaf(f2e[v], 1.0f / (PSC * PSC), eps);
+        }
+        if constexpr (MFMA && !GRAD) {
+          if (ps == NP - 1 && more) fetch_tile(tile0 + C::TM);
+        }
+        if constexpr (MODE == DENSE_LOSS) {
+          // kl = sum_j q_j log(q_j / p_j) with q ~ a.*b, p ~ a.*f2 (a = column x_t of Q_t + eps, b = row x0 of
+          // Qbar_{t-1} + eps, f2 = pi Qbar_{t-1} + eps): the reference's softmax(log a + log .) pairs folded, one
+          // log per class (of a ratio close to one where q is large).
+          const float ce = MFMA ? s_tokf[3 * tok] : cekeep[ps];
+          float vb = ce;
+          if (post) {
+            float av[L::V], bv[L::V], zm = 0, zt = 0;
 #pragma unroll
-          for (int v = 0; v < L::V; ++v) {
-            const bool ok = valid(L::cls(g, v));
-            av[v] = ok ? f1n[ps % NZ][v] + eps : 0.0f;
-            bv[v] = f2n[ps % NZ][v] + eps;
-            zm = fmaf(av[v], f2e[v], zm);
-            zt = fmaf(av[v], bv[v], zt);
+            for (int v = 0; v < L::V; ++v) {
+              const bool ok = valid(L::cls(g, v));
+              av[v] = ok ? f1n[ps % NZ][v] + eps : 0.0f;
+              bv[v] = f2n[ps % NZ][v] + eps;
+              zm = fmaf(av[v], f2e[v], zm);
+              zt = fmaf(av[v], bv[v], zt);
+            }
+            zm = group_sum<L::G>(zm);
+            zt = group_sum<L::G>(zt);
+            const float izm = fast_rcp(zm), izt = fast_rcp(zt), zr = zm * izt;
+            float kl = 0, gf2[L::V];
+#pragma unroll
+            for (int v = 0; v < L::V; ++v) {
+              const float br = bv[v] * fast_rcp(f2e[v]);                     // b_j / f2_j
+              kl = fmaf(av[v] * bv[v], fast_log2(br * zr), kl);              // av = 0 on masked slots
+              if constexpr (GRAD) gf2[v] = live ? w_vb * av[v] * fmaf(-br, izt, izm) : 0.0f;
+            }
+            if constexpr (GRAD) {
+              if constexpr (L::VEC) {
+                store_slots<L>(s_f2 + (size_t)tok * LDK, g, K, gf2);
+              } else {
+#pragma unroll
+                for (int v = 0; v < L::V; ++v) {
+                  const int c = L::cls(g, v);
+                  if (c < K) s_f2[(size_t)tok * LDK + c] = gf2[v];
+                }
+              }
+            }
+            vb = group_sum<L::G>(kl) * izt * LN2;                            // nats, like ce
           }
-          zm = group_sum<L::G>(zm);
-          zt = group_sum<L::G>(zt);
-          const float izm = fast_rcp(zm), izt = fast_rcp(zt), zr = zm * izt;
-          float kl = 0, gf2[L::V];
+          if (g == 0 && live) { acc_vb += vb; acc_ce += ce; }
+        } else {
+          constexpr bool DEVICE_DRAW = MODE == DENSE_SAMPLE && NOISE == D3PM_NOISE_PHILOX;
+          float lm[L::V];
+          if (post && !DEVICE_DRAW) {
 #pragma unroll
-          for (int v = 0; v < L::V; ++v) {
-            const float br = bv[v] * fast_rcp(f2e[v]);                     // b_j / f2_j
-            kl = fmaf(av[v] * bv[v], fast_log2(br * zr), kl);              // av = 0 on masked slots
-            if constexpr (GRAD) gf2[v] = live ? w_vb * av[v] * fmaf(-br, izt, izm) : 0.0f;
+            for (int v = 0; v < L::V; ++v) lm[v] = logf(f1n[ps % NZ][v] + eps) + logf(f2e[v]);
           }
-          if constexpr (GRAD) {
-            if constexpr (L::VEC) {
-              store_slots<L>(s_f2 + (size_t)tok * LDK, g, K, gf2);
-            } else {
+          if constexpr (MODE == DENSE_POST) {
+            float r[L::V];
+#pragma unroll
+            for (int v = 0; v < L::V; ++v) r[v] = (t == 0) ? zkeep[ps % NKEEP][v] : lm[v];
+            if (live) store_slots<L>(e.out + n * K, g, K, r);
+          } else if constexpr (DEVICE_DRAW) {
+            // Noise drawn on the device: nothing to match bit for bit, so the draw is one uniform per token and an
+            // inverse CDF over the unnormalised posterior (a_j f2_j) -- no logarithm, no Gumbel transform, one Philox
+            // call per token instead of one per four classes.  t == 0: argmax of the logits, as with explicit noise.
+            int pick;
+            if (t == 0) {
+              float best = -INFINITY;
+              pick = 0x7fffffff;
 #pragma unroll
               for (int v = 0; v < L::V; ++v) {
                 const int c = L::cls(g, v);
-                if (c < K) s_f2[(size_t)tok * LDK + c] = gf2[v];
+                const float val = zkeep[ps % NKEEP][v];
+                if (valid(c) && (val > best || pick == 0x7fffffff)) { best = val; pick = c; }
               }
+              group_argmax<L::G>(best, pick);
+            } else {
+              float w[L::V];
+#pragma unroll
+              for (int v = 0; v < L::V; ++v) w[v] = valid(L::cls(g, v)) ? (f1n[ps % NZ][v] + eps) * f2e[v] : 0.0f;
+              const U4 r = philox4x32_10((uint64_t)n, e.offset, e.seed);
+              const float uu = u01_open(r.x);
+              pick = group_pick<L::G, L::V>(w, g, uu, tok_xt(ps), [](int gg, int vv) { return L::cls(gg, vv); });
             }
-          }
-          vb = group_sum<L::G>(kl) * izt * LN2;                            // nats, like ce
-        }
-        if (g == 0 && live) { acc_vb += vb; acc_ce += ce; }
-      } else {
-        constexpr bool DEVICE_DRAW = MODE == DENSE_SAMPLE && NOISE == D3PM_NOISE_PHILOX;
-        float lm[L::V];
-        if (need_post && !DEVICE_DRAW) {
-#pragma unroll
-          for (int v = 0; v < L::V; ++v) lm[v] = logf(f1n[ps % NZ][v] + eps) + logf(f2e[v]);
-        }
-        if constexpr (MODE == DENSE_POST) {
-          float r[L::V];
-#pragma unroll
-          for (int v = 0; v < L::V; ++v) r[v] = (t == 0) ? zkeep[ps % NKEEP][v] : lm[v];
-          if (live) store_slots<L>(e.out + n * K, g, K, r);
-        } else if constexpr (DEVICE_DRAW) {
-          // Noise drawn on the device: nothing to match bit for bit, so the draw is one uniform per token and an
-          // inverse CDF over the unnormalised posterior (a_j f2_j) -- no logarithm, no Gumbel transform, one Philox
-          // call per token instead of one per four classes.  t == 0: argmax of the logits, as with explicit noise.
-          int pick;
-          if (t == 0) {
+            if (g == 0 && live) e.sample[n] = pick;
+          } else {   // DENSE_SAMPLE, noise tensor given
             float best = -INFINITY;
-            pick = 0x7fffffff;
+            int besti = 0x7fffffff;
+            float u[L::V];
+            if (t > 0) load_slots<L>(e.noise + n * K, g, K, 0.5f, u);
 #pragma unroll
             for (int v = 0; v < L::V; ++v) {
               const int c = L::cls(g, v);
-              const float val = zkeep[ps % NKEEP][v];
-              if (valid(c) && (val > best || pick == 0x7fffffff)) { best = val; pick = c; }
+              float val;
+              if (t == 0) val = zkeep[ps % NKEEP][v];
+              else val = lm[v] + ((NOISE == D3PM_NOISE_GUMBEL) ? u[v] : gumbel_from_uniform(u[v]));
+              if (valid(c) && (val > best || besti == 0x7fffffff)) { best = val; besti = c; }
             }
-            group_argmax<L::G>(best, pick);
-          } else {
-            float w[L::V];
-#pragma unroll
-            for (int v = 0; v < L::V; ++v) w[v] = valid(L::cls(g, v)) ? (f1n[ps % NZ][v] + eps) * f2e[v] : 0.0f;
-            const U4 r = philox4x32_10((uint64_t)n, e.offset, e.seed);
-            const float uu = u01_open(r.x);
-            pick = group_pick<L::G, L::V>(w, g, uu, tok_xt(ps), [](int gg, int vv) { return L::cls(gg, vv); });
+            group_argmax<L::G>(best, besti);
+            if (g == 0 && live) e.sample[n] = besti;
           }
-          if (g == 0 && live) e.sample[n] = pick;
-        } else {   // DENSE_SAMPLE, noise tensor given
-          float best = -INFINITY;
-          int besti = 0x7fffffff;
-          float u[L::V];
-          if (t > 0) load_slots<L>(e.noise + n * K, g, K, 0.5f, u);
-#pragma unroll
-          for (int v = 0; v < L::V; ++v) {
-            const int c = L::cls(g, v);
-            float val;
-            if (t == 0) val = zkeep[ps % NKEEP][v];
-            else val = lm[v] + ((NOISE == D3PM_NOISE_GUMBEL) ? u[v] : gumbel_from_uniform(u[v]));
-            if (valid(c) && (val > best || besti == 0x7fffffff)) { best = val; besti = c; }
-          }
-          group_argmax<L::G>(best, besti);
-          if (g == 0 && live) e.sample[n] = besti;
         }
+        if constexpr (MFMA) __builtin_amdgcn_sched_barrier(0);
       }
-      if constexpr (MFMA) __builtin_amdgcn_sched_barrier(0);
-    }
+    };
+    if constexpr (MFMA && GRAD) {
+      if (need_post) epilogue(true);
+      else epilogue(false);
+    } else epilogue(need_post);
     if constexpr (MODE == DENSE_LOSS && GRAD) {
       if constexpr (MFMA) fetch_row(tile0, 0);
       else if (more) fetch_tile(tile0 + C::TM);

@@ -1136,8 +1136,8 @@ __global__ __launch_bounds__(1024) void k_hybrid_loss_pair32(
   bool first = true;
   for (;; base += step) {
     const bool work = ONE || base < p1;       // uniform over the wave
-    // the lane's 16 classes as eight pairs: the per-class arithmetic below is written on pairs so that it maps onto
-    // the packed float32 instructions (one issue slot for two classes)
+    // the lane's 16 classes as eight pairs, on which the per-class arithmetic below is written (an instruction to each
+    // class: the build has no packed float32 instructions)
     f2v e[HC / 2];
     float m = 0, inv = 0, l2s = 0, mneg = 0;
     if (work) {

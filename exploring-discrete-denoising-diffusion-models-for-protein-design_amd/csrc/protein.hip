@@ -425,8 +425,8 @@ __global__ __launch_bounds__(64) void k_lvb_digest32(d3pm_tables_f64 tb, float* 
 // slot's generic terms are those of a class of zero probability (taken out again with the same expressions, bit for
 // bit), and the gradient loop leaves a zero in the slot, over which the token's own value for x0 is stored.
 // cs = grad_scale / npos, ces = ce_grad_scale / npos from the host.
-// T = float for one class, f2v for a pair of classes (the class loops run on pairs: packed float32 instructions,
-// one issue slot for two classes).
+// T = float for one class, f2v for a pair of classes (the class loops run on pairs; an instruction to each
+// class: the build has no packed float32 instructions).
 __device__ __forceinline__ float rcp_each(float v) { return __builtin_amdgcn_rcpf(v); }
 __device__ __forceinline__ f2v rcp_each(f2v v) { return f2v{__builtin_amdgcn_rcpf(v.x), __builtin_amdgcn_rcpf(v.y)}; }
 __device__ __forceinline__ f2v exp2_each(f2v v) { return f2v{__builtin_amdgcn_exp2f(v.x), __builtin_amdgcn_exp2f(v.y)}; }

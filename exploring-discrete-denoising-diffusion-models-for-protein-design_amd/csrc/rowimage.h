@@ -112,7 +112,7 @@ struct RowImage {
         *reinterpret_cast<piece_t*>(img + lane * STRIDE + j * PB) = piece_t{z[2 * j], z[2 * j + 1]};
     }
   }
-  // The same with the row as LD / 2 pairs of neighbouring elements (arithmetic on pairs maps onto packed float32).
+  // The same with the row as LD / 2 pairs of neighbouring elements.
   __device__ static __forceinline__ void read_row_pairs(const char* img, int lane, f2v (&z)[LD / 2]) {
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) {

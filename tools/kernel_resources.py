@@ -23,7 +23,7 @@ import yaml
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "exploring-discrete-denoising-diffusion-models-for-protein-design_amd", "csrc")
 SOURCES = ["tables.hip", "image_structured.hip", "protein.hip", "logistic.hip", "finetune.hip"]
-EXTRA_FLAGS = {"finetune.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]}
+DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]         # as the build has them
 LLVM = "/opt/rocm/lib/llvm/bin"
 
 
@@ -36,7 +36,7 @@ def demangle(names):
 def device_object(src: str, outdir: str) -> str:
     obj = os.path.join(outdir, src.replace(".hip", ".gfx950.o"))
     cmd = ["/opt/rocm/bin/hipcc", "-O3", "--offload-arch=gfx950", "--offload-device-only", "-std=c++17", "-c",
-           os.path.join(CSRC, src), "-o", obj] + EXTRA_FLAGS.get(src, []) + os.environ.get("D3PM_HIPCC_FLAGS", "").split()
+           os.path.join(CSRC, src), "-o", obj] + DEVICE_FLAGS + os.environ.get("D3PM_HIPCC_FLAGS", "").split()
     subprocess.run(cmd, cwd=CSRC, check=True)
     # the compiler writes an offload bundle: take the gfx950 code object out of it
     elf = obj.replace(".o", ".co")

@@ -1,29 +1,22 @@
 // Micro-benchmark: VALU issue rate per SIMD as a function of waves per SIMD and instruction kind.
 // Each wave runs ITER iterations of 16 independent operations; the grid places `wps` waves on every SIMD of the chip.
-//   hipcc -O3 --offload-arch=gfx950 valu_rate.hip -o valu_rate.bin
+//   hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops valu_rate.hip -o valu_rate.bin
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>
 
-typedef float f2 __attribute__((ext_vector_type(2)));
-
-enum { FMA, PKFMA, PKMUL, PKADD, EXP, RCP, LOG, DPPADD, FMA_EXP4, CNDMASK, FMA_DEP };
+enum { FMA, EXP, RCP, LOG, DPPADD, FMA_EXP4, CNDMASK, FMA_DEP };
 
 template <int MODE>
 __global__ void k(float* out, int iters) {
   float a[16];
-  f2 p[16];
-  for (int i = 0; i < 16; ++i) { a[i] = threadIdx.x * 0.001f + i; p[i] = f2{a[i], a[i] + 0.5f}; }
+  for (int i = 0; i < 16; ++i) a[i] = threadIdx.x * 0.001f + i;
   const float b = 1.0001f, c = 0.5f;
-  const f2 b2 = {1.0001f, 0.9999f}, c2 = {0.5f, 0.25f};
   for (int it = 0; it < iters; ++it) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       if (MODE == FMA) a[i] = __builtin_fmaf(a[i], b, c);
       if (MODE == FMA_DEP) a[0] = __builtin_fmaf(a[0], b, c);
-      if (MODE == PKFMA) asm volatile("v_pk_fma_f32 %0, %1, %2, %3" : "=v"(p[i]) : "v"(p[i]), "v"(b2), "v"(c2));
-      if (MODE == PKMUL) asm volatile("v_pk_mul_f32 %0, %1, %2" : "=v"(p[i]) : "v"(p[i]), "v"(b2));
-      if (MODE == PKADD) asm volatile("v_pk_add_f32 %0, %1, %2" : "=v"(p[i]) : "v"(p[i]), "v"(c2));
       if (MODE == EXP) a[i] = __builtin_amdgcn_exp2f(a[i]);
       if (MODE == RCP) a[i] = __builtin_amdgcn_rcpf(a[i]);
       if (MODE == LOG) a[i] = __builtin_amdgcn_logf(a[i]);
@@ -36,7 +29,7 @@ __global__ void k(float* out, int iters) {
     }
   }
   float s = 0;
-  for (int i = 0; i < 16; ++i) s += a[i] + p[i].x + p[i].y;
+  for (int i = 0; i < 16; ++i) s += a[i];
   if (s == 123.456f) out[0] = s;
 }
 
@@ -65,9 +58,6 @@ void run(const char* name, int per_iter) {
 int main() {
   run<FMA>("v_fma_f32", 16);
   run<FMA_DEP>("v_fma_f32 dependent chain", 16);
-  run<PKFMA>("v_pk_fma_f32", 16);
-  run<PKMUL>("v_pk_mul_f32", 16);
-  run<PKADD>("v_pk_add_f32", 16);
   run<EXP>("v_exp_f32", 16);
   run<RCP>("v_rcp_f32", 16);
   run<LOG>("v_log_f32", 16);

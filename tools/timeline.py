@@ -1,7 +1,8 @@
 #!/usr/bin/env python3
 """In-kernel timeline of the fused loss kernel (debug build of the library).
 
-    hipcc -O3 --offload-arch=gfx950 -fPIC -std=c++17 -shared -DD3PM_TIMELINE [-DD3PM_TL_ROWS] \
+    hipcc -O3 --offload-arch=gfx950 -fPIC -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops \
+        -shared -DD3PM_TIMELINE [-DD3PM_TL_ROWS] \
         csrc/tables.hip csrc/image_structured.hip csrc/protein.hip csrc/logistic.hip -o tools/micro/libd3pm_timeline.so
     D3PM_LIB=tools/micro/libd3pm_timeline.so python tools/timeline.py
 
