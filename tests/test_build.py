@@ -24,3 +24,18 @@ def test_no_packed_float32_instructions(source, tmp_path):
     text = subprocess.run([os.path.join(LLVM, "llvm-objdump"), "-d", code], check=True, capture_output=True, text=True).stdout
     assert "s_endpgm" in text
     assert not re.search(r"\bv_pk_(add|mul|fma)_f32\b", text)
+
+
+def test_build_compiles_whenever_it_is_called(monkeypatch):
+    """Also where the libraries are newer than their sources: it is the check that the sources compile."""
+    ran = []
+
+    class Compiled:
+        def wait(self):
+            return 0
+
+    monkeypatch.setattr(ge.subprocess, "Popen", lambda cmd, **k: ran.append(cmd[-1]) or Compiled())
+    monkeypatch.setattr(ge.subprocess, "run", lambda cmd, **k: ran.append(cmd[-1]))
+    ge.build()
+    assert [os.path.basename(o) for o in ran[:len(ge.SOURCES)]] == [s.replace(".hip", ".o") for s in ge.SOURCES]
+    assert len(ran) == len(ge.SOURCES) + 2                      # and the two links
